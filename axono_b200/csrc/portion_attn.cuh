@@ -1,0 +1,125 @@
+// What the kernels of attention over a paged cache for portions share: the blocks of rows that a launch is cut into, the rows and keys
+// of a block, and where partial results of divided keys go.
+//
+// Sequence b brings the rows row_start[b] .. row_start[b + 1] - 1, the last of its seq_lens[b] cached tokens; row i of its c rows stands
+// at position t = seq_lens[b] - c + i and sees the keys max(0, t + 1 - window) .. t (window 0: from 0).  A block is `tokens` rows of one
+// sequence times the query heads of one KV head, so that a tile of keys is read once for all of them.  Lengths and rows live in device
+// memory: the host knows bounds, makes the grid for them, and a CTA finds its block itself or leaves.
+#pragma once
+
+#include <math.h>
+
+#include "common.cuh"
+
+namespace axb {
+
+constexpr int kPortionKeys = 64;  // keys of a tile, which lies in one page
+
+struct PortionParams {
+  const void *q;
+  void *out;
+  const void *k_pages, *v_pages;
+  const int32_t *block_table, *seq_lens, *row_start;
+  int rows, batch, hq, hkv, group, d, page_tokens, max_blocks, num_pages, window;
+  int max_keys;                  // keys of a sequence that the grid is made for
+  int tokens, blocks;            // rows of a block; blocks that the rows can need at most
+  int parts, tiles_per_part;     // parts that a block's tiles can need at most
+  float scale_log2;              // of scores, in powers of two
+  unsigned long long wait_ns;
+  // with parts > 1, results of blocks with divided keys: un-normalised sums (part, row, head, d), their (maximum, denominator), and of
+  // every row the number of its parts
+  float *sums;
+  float2 *ml;
+  int32_t *row_parts;
+};
+
+struct PortionBlock {
+  int seq, row0, rows;     // its first row and how many
+  int first_pos;           // position of the first row
+  int key_limit;           // keys of the sequence that may be read
+  int tile0, tiles, parts; // tiles of all its keys, and into how many parts they are divided (at least one)
+};
+
+// Finds block `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a block of
+// at most 1024; the result is for all.  `found` is false beyond the last block.
+__device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block) {
+  __shared__ PortionBlock s_block;
+  __shared__ int s_sums[32], s_found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+  if (threadIdx.x == 0) s_found = 0;
+  int before = 0;  // blocks of the sequences before this round's
+  for (int base = 0; base < p.batch; base += blockDim.x) {
+    const int b = base + threadIdx.x;
+    int r0 = 0, r1 = 0, len = 0;
+    if (b < p.batch) {
+      r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
+      if (r0 < 0 || r1 < r0 || r1 > p.rows) {
+        atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
+        r0 = r1 = 0;
+      }
+    }
+    const int mine = (r1 - r0 + p.tokens - 1) / p.tokens;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 31) s_sums[warp] = upto;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int n = s_sums[w];
+      if (w < warp) upto += n;
+      total += n;
+    }
+    const int at = index - before - (upto - mine);  // among this sequence's blocks
+    if (at >= 0 && at < mine) {
+      const int first = (mine - 1 - at) * p.tokens, count = r1 - r0;
+      PortionBlock f;
+      f.seq = b;
+      f.row0 = r0 + first;
+      f.rows = min(p.tokens, count - first);
+      f.first_pos = len - count + first;
+      f.key_limit = min(max(len, 0), p.max_keys);
+      if (len > p.max_keys) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
+      const int end = min(f.first_pos + f.rows, f.key_limit);
+      const int begin = p.window ? max(0, f.first_pos + 1 - p.window) : 0;
+      f.tile0 = begin / kPortionKeys;
+      f.tiles = end > begin ? (end + kPortionKeys - 1) / kPortionKeys - f.tile0 : 0;
+      f.parts = max(1, (f.tiles + p.tiles_per_part - 1) / p.tiles_per_part);
+      s_block = f;
+      s_found = 1;
+    }
+    before += total;
+    __syncthreads();
+    if (s_found || before > index) break;
+  }
+  block = s_block;
+  return s_found;
+}
+
+__host__ __device__ inline int portion_part_begin(int tiles, int part, int parts) { return (int)((int64_t)tiles * part / parts); }
+
+// Where row (of the launch) and head of a part stand among the partial results.
+__device__ __forceinline__ size_t portion_place(const PortionParams &p, int part, int row, int head) {
+  return ((size_t)part * p.rows + row) * p.hq + head;
+}
+
+// The page of a tile, or num_pages (which TMA reads as zeros) where the table has none.
+__device__ __forceinline__ int portion_page(const PortionParams &p, int seq, int tile) {
+  const int64_t slot = (int64_t)tile * kPortionKeys / p.page_tokens;
+  if (slot >= p.max_blocks) return p.num_pages;
+  const int page = p.block_table[(int64_t)seq * p.max_blocks + slot];
+  if (page >= 0 && page < p.num_pages) return page;
+  atomicOr(&g_error_word, AXB200_ERR_BAD_PAGE);
+  return p.num_pages;
+}
+
+// FLOAT16 on the tensor cores (portion_attn.cu) and anything on the FMA pipe (portion_attn_fma.cu): attention and, for p.parts > 1,
+// partial results.
+bool portions_on_tensor_cores(const PortionParams &p, int dtype);
+int portions_f16(const PortionParams &p, cudaStream_t st);
+int portions_fma(const PortionParams &p, int dtype, cudaStream_t st);
+
+}  // namespace axb

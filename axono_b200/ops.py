@@ -598,6 +598,225 @@ def scaled_dot_product_attention(q, k, v, is_causal: bool = False):
     return out
 
 
+# ---- portions: rows that bring several sequences their next tokens ---------------------------------------------
+_TURN_DTYPES = {torch.float16: _capi.FLOAT16, torch.bfloat16: _capi.BFLOAT16, torch.float32: _capi.FLOAT32}
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling=None, device="cuda"):
+    """(inv_freq, factor) of a rotation over rot_dim elements: theta^(-2i / rot_dim) as a device tensor of rot_dim / 2 doubles, and
+    what cosines and sines are multiplied with.  scaling stretches a context: None, or a dict with `kind` and
+      linear  factor: all positions divided by it
+      ntk     factor: theta grows so that the slowest pair turns `factor` times slower and the fastest as before
+      smooth  factor, original (tokens the model was trained on), low (1.0), high (4.0): pairs that turn more than `high` times in
+              them stay, those with fewer than `low` turns are divided by factor, in between a linear blend
+      yarn    factor, original, slow (1.0), fast (32.0) and optionally attention_factor: the same between `slow` and `fast` turns,
+              the blend linear over the pairs' numbers, and cosines and sines times 0.1 ln(factor) + 1."""
+    import math
+
+    op = "rope_frequencies"
+    if rot_dim <= 0 or rot_dim % 2 or not theta > 0:
+        raise RuntimeError(f"{op}: rot_dim has to be even and positive, theta positive")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    freq, factor = float(theta) ** (-2 * i / rot_dim), 1.0
+    if scaling is not None:
+        kind, stretch = scaling.get("kind"), float(scaling.get("factor", 0.0))
+        if kind not in ("linear", "ntk", "smooth", "yarn") or stretch < 1.0:
+            raise RuntimeError(f"{op}: kind linear, ntk, smooth or yarn, and a factor of at least 1")
+        if kind == "linear":
+            freq = freq / stretch
+        elif kind == "ntk":
+            if rot_dim == 2:
+                raise RuntimeError(f"{op}: ntk needs more than one pair")
+            freq = (float(theta) * stretch ** (rot_dim / (rot_dim - 2))) ** (-2 * i / rot_dim)
+        else:
+            original = float(scaling.get("original", 0))
+            if original <= 0:
+                raise RuntimeError(f"{op}: {kind} needs `original`, the tokens the model was trained on")
+            if kind == "smooth":
+                low, high = float(scaling.get("low", 1.0)), float(scaling.get("high", 4.0))
+                if not 0 < low < high:
+                    raise RuntimeError(f"{op}: low has to be positive and below high")
+                kept = ((original * freq / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+            else:
+                slow, fast = float(scaling.get("slow", 1.0)), float(scaling.get("fast", 32.0))
+                if not 0 < slow < fast or not theta > 1:
+                    raise RuntimeError(f"{op}: slow has to be positive and below fast, theta above 1")
+                pair_of = lambda turns: rot_dim * math.log(original / (2 * math.pi * turns)) / (2 * math.log(theta))  # noqa: E731
+                first, last = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim - 1)
+                kept = 1 - ((i - first) / max(last - first, 1e-3)).clamp(0, 1)
+                factor = scaling.get("attention_factor")
+                factor = 0.1 * math.log(stretch) + 1.0 if factor is None else float(factor)
+            freq = freq / stretch * (1 - kept) + freq * kept
+    return freq.to(device), factor
+
+
+def _on_device(ref, op, *tensors):
+    for t in tensors:
+        if t is not None and t.device != ref.device:
+            raise RuntimeError(f"{op}: tensors on different devices")
+
+
+def _launch_on(t, call, *args):
+    """The call with t's device as the current one (a launch goes to the current device whatever its stream)."""
+    if t.device.index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(t.device):
+        return call(*args)
+
+
+def _rotation(op, d, inv_freq, pos, rows, mrope_section, pos_needed):
+    """(rot_dim, mrope, h, w, pos) of the operators below."""
+    if inv_freq is None:
+        return 0, 0, 0, 0, None
+    if inv_freq.dtype != torch.float64:
+        _capi.check(3, op)
+    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= d or not inv_freq.is_contiguous():
+        _capi.check(4, op)
+    mrope = mrope_section is not None
+    if pos is None:
+        if pos_needed:
+            raise RuntimeError(f"{op}: a rotation needs positions")
+    elif pos.dtype != torch.int64:
+        _capi.check(3, op)
+    elif tuple(pos.shape) != ((3, rows) if mrope else (rows,)):
+        _capi.check(4, op)
+    _, h, w = mrope_section if mrope and pos is not None else (0, 0, 0)
+    return 2 * inv_freq.numel(), int(mrope and pos is not None), int(h), int(w), None if pos is None else _c(pos)
+
+
+def _head_rows(x, op):
+    """x (rows, heads, d) as it is where each row is contiguous, else a contiguous copy; and its row stride."""
+    if x.dim() != 3:
+        _capi.check(4, op)
+    if not (x.stride(2) == 1 and x.stride(1) == x.shape[2] and x.stride(0) >= x.shape[1] * x.shape[2]) and not x.is_contiguous():
+        x = x.contiguous()
+    return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
+
+
+def _norm_weight(w, x, d, op):
+    if w is not None and (w.dtype != x.dtype or tuple(w.shape) != (d,) or not w.is_contiguous()):
+        _capi.check(4, op)
+
+
+def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False, factor: float = 1.0,
+                 mrope_section=None):
+    """RMS norm of every head of q (rows, hq, d) and k (rows, hkv, d) - where its weight (d) is given - and the rotation of its first
+    2 * len(inv_freq) elements by position, in one launch; both may be column slices of a QKV product, either may be None.  pos
+    int64 (rows), or (3, rows) with mrope_section=(t, h, w); inv_freq and factor as `rope_frequencies` gives them (inv_freq None: no
+    rotation); pairs (i, i + n), or (2i, 2i + 1) with interleaved.  fp16, bf16 or fp32; angles in double, the rest in fp32, one
+    rounding.  Returns new contiguous (q, k)."""
+    op = "qk_norm_rope"
+    x = q if q is not None else k
+    if x is None:
+        _capi.check(7, op)
+    if not x.is_cuda:
+        raise RuntimeError(f"{op}: expected CUDA tensors (this package has no CPU path)")
+    dt = _TURN_DTYPES.get(x.dtype)
+    if dt is None:
+        _capi.check(3, op)
+    rows, _, d = x.shape if x.dim() == 3 else _capi.check(4, op)
+    args, outs = [], []
+    for t, w in ((q, q_weight), (k, k_weight)):
+        if t is None:
+            args.append((None, 0, 0))
+            outs.append(None)
+            continue
+        t, ld = _head_rows(t, op)
+        if t.dtype != x.dtype:
+            _capi.check(3, op)
+        if t.shape[0] != rows or t.shape[2] != d:
+            _capi.check(4, op)
+        _norm_weight(w, x, d, op)
+        args.append((t, ld, t.shape[1]))
+        outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
+    rot_dim, mrope, h, w, pos = _rotation(op, d, inv_freq, pos, rows, mrope_section, True)
+    _on_device(x, op, q, k, pos, inv_freq, q_weight, k_weight)
+    (tq, q_ld, hq), (tk, k_ld, hkv) = args
+    _call(_launch_on(x, _capi.lib().axb200_qk_norm_rope, _ptr(tq), q_ld, _ptr(tk), k_ld, _ptr(q_weight), _ptr(k_weight), float(eps),
+                     _ptr(pos), _ptr(inv_freq), rot_dim, int(interleaved), float(factor), mrope, h, w, _ptr(outs[0]), _ptr(outs[1]),
+                     rows, hq, hkv, d, dt, _stream(x)), op)
+    return tuple(outs)
+
+
+def _portion_tables(op, ref, k_pages, v_pages, block_table, seq_lens, row_start):
+    """batch of the operators below; everything that a kernel would follow blindly is checked here."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or block_table.dim() != 2 or seq_lens.dim() != 1 or row_start.dim() != 1:
+        _capi.check(4, op)
+    if k_pages.dtype != ref.dtype or v_pages.dtype != ref.dtype or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
+            or row_start.dtype != torch.int32:
+        _capi.check(3, op)
+    batch = row_start.numel() - 1
+    if batch < 1 or seq_lens.numel() < batch or block_table.shape[0] < batch:
+        _capi.check(4, op)
+    for t in (k_pages, v_pages, block_table, seq_lens, row_start):
+        if not t.is_contiguous():
+            raise RuntimeError(f"{op}: pages and tables must be contiguous")
+    _on_device(ref, op, k_pages, v_pages, block_table, seq_lens, row_start)
+    return batch
+
+
+def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens, row_start,
+                                  pos=None, inv_freq=None, interleaved=False, factor=1.0, mrope_section=None, advance=True, out=None):
+    """`qkv_norm_rope_append` for rows that bring several sequences their next tokens: sequence b owns the rows row_start[b] ..
+    row_start[b + 1] - 1 of qkv (rows, (hq + 2 * hkv) * d) (rows may be strided), row_start int32 (batch + 1) on the device.  Per-head
+    norm and rotation as in `qk_norm_rope` (pos None: the slot; inv_freq None: no rotation); keys and values go behind the seq_lens[b]
+    cached tokens, which grow by the portion (advance, the first layer of a step), or into the last of them (later layers).  Returns
+    the turned q (rows, hq, d); rows of no sequence are left as they are in `out`."""
+    op = "qkv_norm_rope_append_portions"
+    dt = _dt(qkv, op)
+    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+        _capi.check(4, op)
+    batch = _portion_tables(op, qkv, k_pages, v_pages, block_table, seq_lens, row_start)
+    num_pages, hkv, page_tokens, d = k_pages.shape
+    rows = qkv.shape[0]
+    ld = qkv.stride(0) if rows > 1 else qkv.shape[1]
+    if qkv.shape[1] != (n_q_heads + 2 * hkv) * d or ld < qkv.shape[1]:
+        _capi.check(4, op)
+    for w in (q_norm_weight, k_norm_weight):
+        _norm_weight(w, qkv, d, op)
+    rot_dim, mrope, h, w, pos = _rotation(op, d, inv_freq, pos, rows, mrope_section, False)
+    if out is None:
+        out = torch.empty((rows, n_q_heads, d), dtype=qkv.dtype, device=qkv.device)
+    elif tuple(out.shape) != (rows, n_q_heads, d) or out.dtype != qkv.dtype or not out.is_contiguous():
+        _capi.check(4, op)
+    _on_device(qkv, op, pos, inv_freq, q_norm_weight, k_norm_weight, out)
+    _call(_launch_on(qkv, _capi.lib().axb200_qkv_norm_rope_append_portions, qkv.data_ptr(), ld, _ptr(q_norm_weight), _ptr(k_norm_weight),
+                     float(eps), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+                     row_start.data_ptr(), _ptr(pos), _ptr(inv_freq), rot_dim, int(interleaved), float(factor), mrope, h, w, rows, batch,
+                     n_q_heads, hkv, d, page_tokens, block_table.shape[1], num_pages, dt, int(advance), _stream(qkv)), op)
+    return out
+
+
+def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row_start, max_seq_len, window: int = 0, out=None):
+    """Causal attention of portions over a paged cache that holds them: q (rows, hq, d), sequence b's rows row_start[b] ..
+    row_start[b + 1] - 1 are the last of its seq_lens[b] tokens (`qkv_norm_rope_append_portions` has appended them); each attends the
+    tokens up to its own, the last `window` of them where that is not 0.  max_seq_len: host bound of the lengths.  Returns (rows, hq,
+    d); rows of no sequence are left as they are in `out`."""
+    op = "gqa_attention_portions_paged"
+    dt = _dt(q, op)
+    if q.dim() != 3:
+        _capi.check(4, op)
+    batch = _portion_tables(op, q, k_pages, v_pages, block_table, seq_lens, row_start)
+    rows, hq, d = q.shape
+    num_pages, hkv, page_tokens, dk = k_pages.shape
+    if dk != d or hkv == 0 or hq % hkv:
+        _capi.check(4, op)
+    q = _c(q)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        _capi.check(4, op)
+    _on_device(q, op, out)
+    lib = _capi.lib()
+    sizes = (hq, hkv, d, page_tokens, block_table.shape[1])
+    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, *sizes, int(max_seq_len), int(window), dt)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone: streams may overlap
+    _call(_launch_on(q, lib.axb200_gqa_attention_portions_paged, q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                     block_table.data_ptr(), seq_lens.data_ptr(), row_start.data_ptr(), rows, batch, *sizes, num_pages, int(max_seq_len),
+                     int(window), dt, _ptr(ws), need, _stream(q)), op)
+    return out
+
+
 # ---- operators of the language models (fp32 or bf16; residual, scores, norms and routers in fp32) -----------
 _LM_DTYPES = {torch.bfloat16: _capi.BFLOAT16, torch.float32: _capi.FLOAT32}
 

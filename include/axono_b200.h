@@ -55,7 +55,8 @@ enum {
   AXB200_ERR_BAD_PAGE = 2u,       /* a block-table entry was outside [0, num_pages) */
   AXB200_ERR_CAPACITY = 4u,       /* an append found its sequence at capacity, or a decode call found
                                      seq_lens[b] above max_seq_len / the pages (the excess is not read) */
-  AXB200_ERR_BAD_INDEX = 8u       /* an embedding id was outside [0, vocab) */
+  AXB200_ERR_BAD_INDEX = 8u,      /* an embedding id was outside [0, vocab) */
+  AXB200_ERR_BAD_ROWS = 16u       /* a table of row offsets does not count up, or passes the rows of its launch */
 };
 
 const char *axb200_version(void);
@@ -400,6 +401,48 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
                             int page_tokens, int max_blocks, int num_pages,
                             int64_t max_seq_len, int dtype,
                             void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- portions: rows that bring several sequences their next tokens ------------------------------------------
+ * A launch of `rows` rows: sequence b (row b of block_table) owns the rows row_start[b] .. row_start[b + 1] - 1, a whole prompt, a
+ * portion of one, a token or none; row_start int32 (batch + 1) counts up, in device memory like the lengths, so that a captured graph
+ * follows both.  Rows before row_start[0] and from row_start[batch] on belong to none and are left as they are, in the outputs too.  An
+ * entry of row_start that does not count up or passes `rows` sets AXB200_ERR_BAD_ROWS; what it names is left out.  Pages as in
+ * axb200_gqa_decode_paged.  No counterparts in the reference.
+ *
+ * Rotation of these operators: the first rot_dim elements of a head (even, 0: none) in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with
+ * `interleaved`, by the angle position * inv_freq[i], cosine and sine times `factor` (1, or what a stretched context asks for).
+ * inv_freq: device, double (rot_dim / 2); the angle is formed and reduced in double.  mrope: pos (3, rows) and the axis of pair i as in
+ * axb200_kv_append_rope; else pos (rows).  Norms: x / sqrt(mean(x^2) + eps) * weight per head where a weight (d) is given.  fp32
+ * throughout, one rounding at the end.  d <= 256.
+ *
+ *   qk_norm_rope: norm and rotation of q (rows, hq, d) and k (rows, hkv, d), rows q_ld and k_ld elements apart (column slices of a QKV
+ *     product), to contiguous q_out and k_out; q_out may be q where its rows are contiguous, likewise k.  hq or hkv may be 0.  FLOAT16,
+ *     BFLOAT16, FLOAT32.
+ *   qkv_norm_rope_append_portions: qkv (rows, ld) holds per row hq query heads, hkv key heads, hkv value heads; the turned queries go to
+ *     q_out (rows, hq, d), keys and values into the pages: with `advance` (the first layer of a step) behind the seq_lens[b] cached
+ *     tokens, whose number then grows by the portion; else (later layers) into the last slots of seq_lens[b], which counts them already.
+ *     pos NULL: a row's position is its slot.  A portion that does not fit sets AXB200_ERR_CAPACITY, nothing of it is appended and its
+ *     length stays; a page outside the pool sets AXB200_ERR_BAD_PAGE, its rows are not written and the length stays.  FLOAT16, FLOAT32.
+ *   gqa_attention_portions_paged: q, out (rows, hq, d): row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
+ *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
+ *     counts the portion.  A row that sees no key gets zeros.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
+ *     sets AXB200_ERR_CAPACITY and its keys beyond are not read.  FLOAT16, FLOAT32.  workspace: at least the bytes that
+ *     portions_workspace_bytes gives for the same arguments (0: none), 16-byte aligned, of this call alone until its kernels are done. */
+int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *q_norm_w, const void *k_norm_w, float eps,
+                        const int64_t *pos, const double *inv_freq, int rot_dim, int interleaved, float factor, int mrope, int h_sec,
+                        int w_sec, void *q_out, void *k_out, int64_t rows, int hq, int hkv, int d, int dtype, void *stream);
+int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
+                                         void *k_pages, void *v_pages, const int32_t *block_table, int32_t *seq_lens,
+                                         const int32_t *row_start, const int64_t *pos, const double *inv_freq, int rot_dim,
+                                         int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
+                                         int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
+                                         void *stream);
+size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
+                                                     int64_t max_seq_len, int window, int dtype);
+int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,
+                                        const int32_t *seq_lens, const int32_t *row_start, int64_t rows, int batch, int hq, int hkv,
+                                        int d, int page_tokens, int max_blocks, int num_pages, int64_t max_seq_len, int window,
+                                        int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- RoPE family (stand-alone ops) --------------------------------------------------------
  * x/out (rows,heads,dim); out may alias x. */

@@ -1,0 +1,436 @@
+"""Operators for rows that bring several sequences their next tokens: head norms with rotation, the append to a paged cache, and
+attention over it - each against the definition in 64 bits where lengths, pages, masks, alignments and values can go wrong."""
+import math
+
+import pytest
+import torch
+
+from portion_helpers import Cache, attend_all, attend_tolerance, row_table, turn
+
+pytestmark = pytest.mark.gpu
+EPS = 1e-6
+
+
+def rnd(shape, dtype, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+
+def freqs(rot, theta=1e4):
+    return theta ** (-torch.arange(0, rot, 2, dtype=torch.float64, device="cuda") / rot) if rot else None
+
+
+def weights(d, dtype, norm):
+    return (1 + rnd((d,), dtype, 7, 0.2), 1 - rnd((d,), dtype, 8, 0.2)) if norm else (None, None)
+
+
+def check_turn(out, ref):
+    """One rounding of the type, and fp32 arithmetic: a norm's sum and the two products of a pair, whose terms are as large as the
+    head's largest element; 2^-20 covers both (the sum of 256 squares is off by 2^-21 at most in pairs of chains)."""
+    err = (out.double() - ref).abs()
+    half = torch.finfo(out.dtype).eps / 2
+    small = torch.finfo(out.dtype).smallest_normal * torch.finfo(out.dtype).eps
+    assert (err <= ref.abs() * half * (1 + 2.0 ** -10) + ref.abs().amax(-1, keepdim=True) * 2.0 ** -20 + small).all(), err.max()
+
+
+# ---- norm and rotation ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rot", [(128, 128), (128, 64), (64, 64), (80, 40), (96, 96), (256, 256), (256, 32), (20, 6), (33, 32), (8, 8),
+                                   (2, 2), (128, 0)])
+def test_turn(dtype, d, rot):
+    from axono_b200 import ops
+
+    for rows, hq, hkv, interleaved, norm in ((1, 4, 2, False, True), (37, 5, 1, True, False), (70, 24, 3, False, True), (3, 1, 1, True, True)):
+        qkv = rnd((rows, (hq + 2 * hkv) * d), dtype, rows)
+        q, k = qkv[:, :hq * d].view(rows, hq, d), qkv[:, hq * d:(hq + hkv) * d].view(rows, hkv, d)
+        pos = torch.randint(0, 200000, (rows,), generator=torch.Generator().manual_seed(rows)).cuda()
+        wq, wk = weights(d, dtype, norm)
+        before = qkv.clone()
+        oq, ok = ops.qk_norm_rope(q, k, pos if rot else None, freqs(rot), wq, wk, EPS, interleaved=interleaved, factor=1.25)
+        assert torch.equal(qkv, before) and oq.is_contiguous() and ok.is_contiguous()
+        check_turn(oq, turn(q, wq, EPS, pos, freqs(rot), interleaved, 1.25))
+        check_turn(ok, turn(k, wk, EPS, pos, freqs(rot), interleaved, 1.25))
+    assert ops.last_error() == 0
+
+
+def test_turn_on_three_axes_and_far_positions():
+    from axono_b200 import ops
+
+    rows, section = 40, (24, 20, 20)
+    for rot, far in ((128, 1 << 20), (64, (1 << 31) - 1), (128, 1 << 40)):
+        q, k = rnd((rows, 4, 128), torch.float32, 1), rnd((rows, 2, 128), torch.float32, 2)
+        pos = torch.randint(0, far, (3, rows), generator=torch.Generator().manual_seed(3)).cuda()
+        pos[:, 0] = 0
+        if far >= 1 << 40:
+            pos = pos[:, :1]  # an angle in double is off by 2^-13 of a radian at 2^40: only the origin is exact
+            q, k = q[:1], k[:1]
+        oq, ok = ops.qk_norm_rope(q, k, pos, freqs(rot), eps=EPS, mrope_section=section)
+        slack = 2.0 ** -52 * far * 4  # of the angle, in double
+        for out, x in ((oq, q), (ok, k)):
+            ref = turn(x, None, EPS, pos, freqs(rot), section=section)
+            err = (out.double() - ref).abs()
+            assert (err <= ref.abs() * 2.0 ** -23 + ref.abs().amax(-1, keepdim=True) * (2.0 ** -20 + (slack if far < 1 << 40 else 0))).all()
+
+
+def test_turn_takes_any_alignment_and_one_of_the_two():
+    from axono_b200 import ops
+
+    buf = rnd((9 * 6 * 64 + 1,), torch.float16)
+    q = buf[1:].view(9, 6, 64)  # two bytes off
+    pos = torch.arange(9, device="cuda")
+    oq, none = ops.qk_norm_rope(q, None, pos, freqs(64), interleaved=True)
+    assert none is None
+    check_turn(oq, turn(q, None, EPS, pos, freqs(64), True))
+    none, ok = ops.qk_norm_rope(None, q.transpose(0, 1).contiguous().transpose(0, 1), pos, freqs(64))  # heads outermost: copied
+    assert none is None
+    check_turn(ok, turn(q, None, EPS, pos, freqs(64)))
+    wide = rnd((9, 400), torch.float32)
+    view = wide[:, 3:3 + 5 * 64].view(9, 5, 64)  # rows of 400, 12 bytes off
+    check_turn(ops.qk_norm_rope(view, None, pos, freqs(32))[0], turn(view, None, EPS, pos, freqs(32)))
+
+
+def test_turn_keeps_infinities_and_nan_in_their_heads():
+    from axono_b200 import ops
+
+    q = rnd((5, 4, 128), torch.float16)
+    q[1, 2, 5], q[3, 0, 0] = math.nan, math.inf
+    w = torch.ones(128, dtype=torch.float16, device="cuda")
+    out, _ = ops.qk_norm_rope(q, None, torch.arange(5, device="cuda"), freqs(128), w)
+    bad = ~torch.isfinite(out).all(-1)
+    expect = torch.zeros((5, 4), dtype=torch.bool, device="cuda")
+    expect[1, 2] = expect[3, 0] = True
+    assert torch.equal(bad, expect)
+
+
+# ---- append -----------------------------------------------------------------------------------------------------------
+
+PORTIONS = [((1,), (0,)), ((3, 0, 5, 1), (62, 10, 0, 127)), ((130, 64, 1), (1, 64, 500)), ((0, 0, 7, 0), (5, 0, 63, 9)),
+            (tuple(i % 4 for i in range(300)), tuple(i % 7 for i in range(300)))]
+
+
+@pytest.mark.parametrize("dtype,d,rot,hq,hkv,page", [(torch.float16, 128, 128, 16, 8, 64), (torch.float32, 64, 32, 3, 1, 128),
+                                                     (torch.float16, 80, 80, 6, 2, 64), (torch.float32, 36, 6, 2, 2, 64),
+                                                     (torch.float16, 256, 0, 2, 1, 192)])
+@pytest.mark.parametrize("counts,cached", PORTIONS)
+@pytest.mark.parametrize("advance", [True, False])
+def test_append(dtype, d, rot, hq, hkv, page, counts, cached, advance):
+    from axono_b200 import ops
+
+    lens = [n + c for n, c in zip(counts, cached)]
+    cache = Cache(lens, hkv, d, dtype, page)
+    starts, rows = row_table(counts, first=2), sum(counts) + 5  # rows of no sequence before and behind
+    qkv = rnd((rows, (hq + 2 * hkv) * d + 8), dtype, 11)[:, :(hq + 2 * hkv) * d]
+    wq, wk = weights(d, dtype, rot != 6)
+    axes = rot == 128
+    pos = torch.randint(0, 40000, (3, rows), generator=torch.Generator().manual_seed(5)).cuda() if axes else None
+    section = (24, 20, 20) if axes else None
+    before = torch.tensor(cached if advance else lens, dtype=torch.int32, device="cuda")
+    lengths, k0, v0 = before.clone(), cache.k_pages.clone(), cache.v_pages.clone()
+    out = torch.full((rows, hq, d), 7.0, dtype=dtype, device="cuda")
+    got = ops.qkv_norm_rope_append_portions(qkv, hq, wq, wk, EPS, cache.k_pages, cache.v_pages, cache.table, lengths, starts, pos=pos,
+                                            inv_freq=freqs(rot), interleaved=rot == 32, factor=0.75, mrope_section=section,
+                                            advance=advance, out=out)
+    assert got is out and ops.last_error() == 0
+    assert lengths.tolist() == lens
+    assert (out[:2] == 7).all() and (out[rows - 3:] == 7).all()
+    touched = torch.zeros(k0.shape[:3], dtype=torch.bool, device="cuda")
+    at = 2
+    for b, (n, c) in enumerate(zip(counts, cached)):
+        if not n:
+            continue
+        r = slice(at, at + n)
+        at += n
+        where = torch.arange(c, c + n, device="cuda") if pos is None else pos[:, r]
+        q, k, v = qkv[r].split([hq * d, hkv * d, hkv * d], 1)
+        check_turn(out[r], turn(q.reshape(n, hq, d), wq, EPS, where, freqs(rot), rot == 32, 0.75, section))
+        keys, values = cache.read(b, c, n)
+        check_turn(keys, turn(k.reshape(n, hkv, d), wk, EPS, where, freqs(rot), rot == 32, 0.75, section))
+        assert torch.equal(values, v.reshape(n, hkv, d))
+        page_, place = cache.place(b, c, n)
+        touched[page_, :, place] = True
+    same = lambda a, b: torch.equal(a[~touched].view(torch.uint8), b[~touched].view(torch.uint8))  # noqa: E731  (NaN equals itself)
+    assert same(cache.k_pages, k0) and same(cache.v_pages, v0)
+
+
+def test_append_of_one_token_each_gives_the_keys_of_the_single_token_operator():
+    """Near the beginning, where a product of position and frequency in fp32 is exact enough: norms and rotation agree to the
+    roundings of the single-token form (which also rounds between norm and rotation)."""
+    from axono_b200 import ops
+
+    batch, hq, hkv, d = 5, 8, 4, 128
+    qkv, (wq, wk) = rnd((batch, (hq + 2 * hkv) * d), torch.float16, 3), weights(d, torch.float16, True)
+    caches = [Cache([40 + b for b in range(batch)], hkv, d, torch.float16, more=1) for _ in range(2)]
+    q1 = ops.qkv_norm_rope_append(qkv, hq, wq, wk, EPS, caches[0].k_pages, caches[0].v_pages, caches[0].table, caches[0].lens, theta=1e4)
+    q2 = ops.qkv_norm_rope_append_portions(qkv, hq, wq, wk, EPS, caches[1].k_pages, caches[1].v_pages, caches[1].table, caches[1].lens,
+                                           row_table([1] * batch), inv_freq=freqs(128))
+    assert torch.equal(caches[0].lens, caches[1].lens)
+    for b in range(batch):
+        (k1, v1), (k2, v2) = (c.read(b, 40 + b, 1) for c in caches)
+        assert torch.equal(v1, v2)
+        assert (k1.double() - k2.double()).abs().max() <= 2.0 ** -9 * k1.abs().max()
+    assert (q1.double() - q2.double()).abs().max() <= 2.0 ** -9 * q1.abs().max()
+
+
+def test_append_reports_what_does_not_fit_and_bad_tables():
+    from axono_b200 import _capi, ops
+
+    hq, hkv, d = 2, 1, 64
+    cache = Cache([60, 60, 60], hkv, d, torch.float16, more=4)  # one page each: room for 4
+    lens0, k0 = cache.lens.clone(), cache.k_pages.clone()
+    qkv = rnd((12, (hq + 2 * hkv) * d), torch.float16)
+    run = lambda starts, table=None: ops.qkv_norm_rope_append_portions(  # noqa: E731
+        qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table if table is None else table, cache.lens, starts,
+        inv_freq=freqs(64), out=torch.zeros((12, hq, d), dtype=torch.float16, device="cuda"))
+    q = run(row_table([4, 5, 3]))  # the second does not fit
+    assert ops.last_error() == 4
+    assert cache.lens.tolist() == [64, 60, 63]
+    assert torch.isnan(cache.read(1, 60, 4)[0]).all() and torch.isfinite(cache.read(0, 60, 4)[0]).all()
+    check_turn(q[4:9], turn(qkv[4:9, :hq * d].reshape(5, hq, d), None, EPS, torch.arange(60, 65, device="cuda"), freqs(64)))
+    cache.lens.copy_(lens0)
+    cache.k_pages.copy_(k0)
+    bad = cache.table.clone()
+    bad[2, 0] = cache.k_pages.shape[0]
+    bad[0, 0] = -1
+    run(row_table([1, 1, 1]), bad)
+    assert ops.last_error() == 2
+    assert cache.lens.tolist() == [60, 61, 60]
+    cache.lens.copy_(lens0)
+    run(torch.tensor([0, 2, 1, 3], dtype=torch.int32, device="cuda"))  # falls
+    assert ops.last_error() & 16
+    cache.lens.copy_(lens0)
+    run(torch.tensor([0, 2, 4, 13], dtype=torch.int32, device="cuda"))  # passes the rows
+    assert ops.last_error() & 16
+    assert cache.lens.tolist() == [62, 62, 60]
+    cache.lens.copy_(torch.tensor([1, 60, 60]))
+    cache.lens[0] = 1
+    ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([3, 0, 0]),
+                                      advance=False)  # a length that cannot count three rows
+    assert ops.last_error() == 4
+    assert _capi.lib().axb200_last_error() == 0
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+
+def run_attention(counts, cached, hq, hkv, d, dtype, page=64, window=0, seed=0, spread=1.0, first=0, behind=0, bound=None, cache=None):
+    from axono_b200 import ops
+
+    lens = [n + c for n, c in zip(counts, cached)]
+    cache = cache or Cache(lens, hkv, d, dtype, page, seed)
+    starts = row_table(counts, first)
+    rows = sum(counts) + first + behind
+    q = rnd((rows, hq, d), dtype, seed + 1, spread)
+    out = torch.full_like(q, 7.0)
+    got = ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, bound or max(max(lens), 1),
+                                           window=window, out=out)
+    assert got is out
+    assert (out[:first] == 7).all() and (out[rows - behind:] == 7).all()
+    return q, cache, starts.tolist(), out
+
+
+def check_attention(q, cache, counts, starts, out, window=0):
+    for rows, ref, mag, top in attend_all(q, cache, counts, starts, window):
+        err = (out[rows].double() - ref).abs()
+        tol = attend_tolerance(q.dtype, ref, mag, top)
+        assert (err <= tol).all(), (float(err.max()), float((err / tol.clamp_min(1e-30)).max()))
+
+
+SHAPES = [(16, 8, 128), (4, 4, 64), (12, 4, 80), (8, 1, 96), (6, 2, 40), (7, 1, 128), (2, 2, 8), (3, 1, 72), (32, 1, 64)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+@pytest.mark.parametrize("counts,cached", [((1,), (0,)), ((1, 5, 0, 2), (63, 64, 3, 1)), ((130, 64, 1), (1, 0, 500)), ((257,), (0,)),
+                                           ((40, 3), (1000, 127))])
+def test_attention(dtype, hq, hkv, d, counts, cached):
+    from axono_b200 import ops
+
+    for window in (0, 1, 70):
+        q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, dtype, window=window, first=1, behind=3)
+        check_attention(q, cache, counts, starts, out, window)
+    assert ops.last_error() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d,page", [(4, 2, 20, 64), (4, 4, 256, 128), (2, 1, 136, 64), (130, 1, 64, 64), (260, 2, 16, 64), (3, 1, 33, 192)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_attention_of_unusual_heads(dtype, hq, hkv, d, page):
+    counts, cached = (5, 0, 70), (100, 3, 0)
+    q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, dtype, page, spread=3.0)
+    check_attention(q, cache, counts, starts, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_attention_over_long_caches(dtype):
+    """Few rows over many keys, divided among CTAs and joined, and a loose bound of the lengths."""
+    counts, cached = (2, 1, 17), (9000, 5000, 70)
+    for window, bound in ((0, None), (0, 20000), (4097, None), (130, None)):
+        q, cache, starts, out = run_attention(counts, cached, 8, 2, 128, dtype, window=window, spread=2.0, bound=bound, first=2, behind=1)
+        check_attention(q, cache, counts, starts, out, window)
+
+
+def test_attention_of_a_long_prompt():
+    counts, cached = (1111, 700), (0, 1500)
+    for dtype in (torch.float16, torch.float32):
+        q, cache, starts, out = run_attention(counts, cached, 4, 2, 128, dtype)
+        check_attention(q, cache, counts, starts, out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_ignores_values_that_a_row_cannot_see(dtype, d):
+    """Infinities and NaN in keys and values of later tokens and before a window touch only the rows that see them; stale bytes
+    behind a sequence's end are NaN in every test here."""
+    from axono_b200 import ops
+
+    counts, cached, window = (90, 4), (50, 300), 60
+    lens = [n + c for n, c in zip(counts, cached)]
+    for bad in (math.inf, math.nan):
+        cache = Cache(lens, 2, d, dtype)
+        for b, at in ((0, 100), (1, 301), (1, 200)):
+            cache.v[b][at, 1, 3] = bad
+            if bad != bad:
+                cache.k[b][at, 0, 2] = bad
+            cache.write(b, 0, cache.k[b], cache.v[b])
+        q, cache, starts, out = run_attention(counts, cached, 4, 2, d, dtype, window=window, cache=cache)
+        for b, (n, c) in enumerate(zip(counts, cached)):
+            pos = torch.arange(c, c + n, device="cuda")
+            hit = torch.zeros(n, dtype=torch.bool, device="cuda")
+            for bb, at in ((0, 100), (1, 301), (1, 200)):
+                if bb == b:
+                    hit |= (pos >= at) & (pos < at + window)
+            rows = out[starts[b]:starts[b] + n]
+            assert torch.isfinite(rows[~hit]).all()
+            v_bad = rows[:, 2:, 3]  # heads of KV head 1, the element
+            assert (v_bad[hit] == bad).all() if bad == math.inf else torch.isnan(v_bad[hit]).all()
+            others = torch.ones(d, dtype=torch.bool, device="cuda")
+            others[3] = False
+            assert torch.isfinite(rows[:, 2:][..., others]).all()
+            assert torch.isfinite(rows[:, :2]).all() if bad == math.inf else torch.isnan(rows[:, :2][hit]).all()
+        clean = [cache.v[b].clone() for b in range(2)]
+        for b in range(2):
+            clean[b][~torch.isfinite(clean[b])] = 0
+            cache.k[b][~torch.isfinite(cache.k[b])] = 0
+        cache.v = clean
+        for rows, ref, mag, top in attend_all(q, cache, counts, starts, window):
+            b = 0 if rows.start == starts[0] else 1
+            pos = torch.arange(cached[b], cached[b] + counts[b], device="cuda")
+            hit = torch.zeros(counts[b], dtype=torch.bool, device="cuda")
+            for bb, at in ((0, 100), (1, 301), (1, 200)):
+                if bb == b:
+                    hit |= (pos >= at) & (pos < at + window)
+            err = (out[rows].double() - ref).abs()[~hit]
+            assert (err <= attend_tolerance(dtype, ref, mag, top)[~hit]).all()
+    assert ops.last_error() == 0
+
+
+def test_attention_with_sharp_and_extreme_scores():
+    """Scores up to the largest that fp16 inputs reach, one key that carries all the weight, and equal scores."""
+    from axono_b200 import ops
+
+    for dtype in (torch.float16, torch.float32):
+        for spread in (60.0, 2000.0, 0.0):
+            counts, cached = (65, 2), (10, 700)
+            q, cache, starts, out = run_attention(counts, cached, 4, 2, 64, dtype, spread=spread)
+            check_attention(q, cache, counts, starts, out)
+    assert ops.last_error() == 0
+
+
+def test_attention_reports_lengths_and_tables_that_are_wrong():
+    from axono_b200 import ops
+
+    cache = Cache([200, 100], 2, 64, torch.float16, poison=0.0)
+    q = rnd((8, 4, 64), torch.float16)
+    run = lambda starts, lens=None, table=None, bound=200: ops.gqa_attention_portions_paged(  # noqa: E731
+        q, cache.k_pages, cache.v_pages, cache.table if table is None else table, cache.lens if lens is None else lens, starts, bound,
+        out=torch.full_like(q, 7.0))
+    good = run(row_table([4, 4]))
+    assert ops.last_error() == 0
+    out = run(row_table([4, 4]), bound=128)  # the first sequence is longer than the bound: its first 128 keys
+    assert ops.last_error() == 4 and torch.isfinite(out).all() and torch.equal(out[4:], good[4:])
+    table = cache.table.clone()
+    table[0, 1] = -5
+    out = run(row_table([4, 4]), table=table)
+    assert ops.last_error() == 2 and torch.isfinite(out).all() and torch.equal(out[4:], good[4:])
+    out = run(torch.tensor([0, 4, 9], dtype=torch.int32, device="cuda"))
+    assert ops.last_error() == 16 and torch.equal(out[:4], good[:4]) and (out[4:] == 7).all()
+    out = run(row_table([4, 4]), lens=torch.tensor([200, 2], dtype=torch.int32, device="cuda"))  # two of the rows stand before the sequence
+    assert ops.last_error() == 0 and (out[4:6] == 0).all() and torch.isfinite(out).all() and not (out[6:] == 0).all()
+    out = run(row_table([4, 4]), lens=torch.tensor([200, 0], dtype=torch.int32, device="cuda"))
+    assert ops.last_error() == 0 and (out[4:] == 0).all()
+
+
+def test_attention_beyond_32_bits_of_a_pool():
+    """Pages at the end of pools of more than 2^31 elements."""
+    from axono_b200 import ops
+
+    hkv, d, page, lens = 8, 128, 64, [150, 90]
+    pages = (1 << 31) // (hkv * d * page) + 40
+    small = Cache(lens, hkv, d, torch.float16)
+    big = [torch.empty((pages, hkv, page, d), dtype=torch.float16, device="cuda") for _ in range(2)]
+    shift = pages - small.k_pages.shape[0]
+    for pool, src in zip(big, (small.k_pages, small.v_pages)):
+        pool[shift:] = src
+    small.k_pages, small.v_pages, small.table = *big, torch.where(small.table < src.shape[0], small.table + shift, pages + 1).to(torch.int32)
+    counts = (20, 90)
+    q, cache, starts, out = run_attention(counts, (130, 0), 16, hkv, d, torch.float16, cache=small)
+    check_attention(q, cache, counts, starts, out)
+    # and appended there
+    qkv, lengths = rnd((110, 32 * d), torch.float16, 5), small.lens.clone()
+    ops.qkv_norm_rope_append_portions(qkv, 16, None, None, EPS, *big, small.table, lengths, row_table(counts), advance=False)
+    for b, (r0, n, c) in enumerate(((0, 20, 130), (20, 90, 0))):
+        k, v = small.read(b, c, n)
+        assert torch.equal(k.reshape(n, -1), qkv[r0:r0 + n, 16 * d:24 * d]) and torch.equal(v.reshape(n, -1), qkv[r0:r0 + n, 24 * d:])
+    assert ops.last_error() == 0
+
+
+def test_other_streams_graphs_and_two_calls_at_once():
+    """A captured pair of append and attention follows lengths and row tables that change between replays, and gives what eager
+    calls on two streams at once give."""
+    from axono_b200 import ops
+
+    hq, hkv, d, rows = 8, 2, 128, 40
+    cache = Cache([700, 300, 90], hkv, d, torch.float16, more=40, poison=0.0)
+    lens0 = cache.lens.clone()
+    qkv = rnd((rows, (hq + 2 * hkv) * d), torch.float16, 3)
+    starts = row_table([10, 20, 10])
+    out = torch.zeros((rows, hq, d), dtype=torch.float16, device="cuda")
+
+    def step(lens, starts, out, k=None, v=None):
+        k, v = (cache.k_pages, cache.v_pages) if k is None else (k, v)
+        q = ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, k, v, cache.table, lens, starts, inv_freq=freqs(128))
+        return ops.gqa_attention_portions_paged(q, k, v, cache.table, lens, starts, 800, out=out)
+
+    def eager(counts):
+        lens, k, v = lens0.clone(), cache.k_pages.clone(), cache.v_pages.clone()
+        return step(lens, row_table(counts), torch.zeros_like(out), k, v).clone(), lens
+
+    first, lens1 = eager([10, 20, 10])
+    second, lens2 = eager([1, 0, 33])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    lens = lens0.clone()
+    with torch.cuda.stream(side):
+        step(lens, starts, out)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(lens, starts, out)
+    for counts, expect, after in (([10, 20, 10], first, lens1), ([1, 0, 33], second, lens2), ([10, 20, 10], first, lens1)):
+        lens.copy_(lens0)
+        starts.copy_(row_table(counts))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, expect) and torch.equal(lens, after)
+    # two streams at once, each with its own outputs
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [torch.zeros_like(out) for _ in range(2)]
+    caches = [(cache.k_pages.clone(), cache.v_pages.clone()) for _ in range(2)]
+    tables = [row_table([10, 20, 10]), row_table([1, 0, 33])]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, o, t, (k, v) in zip(streams, outs, tables, caches):
+            with torch.cuda.stream(s):
+                step(lens0.clone(), t, o, k, v)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], first) and torch.equal(outs[1], second)
+    assert ops.last_error() == 0
