@@ -3,8 +3,6 @@
 
 namespace axb {
 
-int portion_fma_tokens(int group);
-
 namespace {
 
 constexpr int kSms = 148;
@@ -26,18 +24,20 @@ join_portions_kernel(const PortionParams p) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float shift = m == -INFINITY ? 0.f : m;
+  bool some = false;
   float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int k = 0; k < parts; ++k) {
     const size_t place = portion_place(p, k, row, head);
     const float2 ml = p.ml[place];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key
+    some = some || ml.y != 0.f;
+    if (ml.x == -INFINITY && ml.y <= 0.f) continue;  // no key, or no score above -inf
     const float w = exp2f(ml.x - shift);
     l = fmaf(w, ml.y, l);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (lane + 32 * j < p.d) acc[j] = fmaf(w, p.sums[place * p.d + lane + 32 * j], acc[j]);
   }
-  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : NAN;
+  const float inv = portion_inverse(l, some);
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (lane + 32 * j < p.d) stf(static_cast<T *>(p.out) + ((size_t)row * p.hq + head) * p.d + lane + 32 * j, acc[j] * inv);
@@ -45,8 +45,12 @@ join_portions_kernel(const PortionParams p) {
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Rows per block and how the keys are divided, from sizes and bounds alone.
-void plan_portions(PortionParams &p, int64_t max_seq_len, int dtype, int tokens) {
+// Rows per block and how the keys are divided, from sizes and bounds alone.  In units of a tile's time: blocks that all run at once take
+// their longest part, else an even share of all and half of the last; a block or part costs kPartCost tiles beside its own, joining
+// kJoinCost and the way of the partial results to memory and back.  A part has 512 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 32768 keys are
+// 2048 products.
+constexpr double kPartCost = 6, kJoinCost = 8, kJoinBytes = 1.4e6;  // bytes moved in a tile's time
+void plan_portions(PortionParams &p, int64_t max_seq_len, int tokens, int places) {
   p.tokens = tokens;
   const int some = p.rows < p.batch ? p.rows : p.batch;  // sequences with rows: each may add a block that is not full
   p.blocks = some + (p.rows - some) / tokens;
@@ -58,12 +62,16 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, int dtype, int tokens)
     tiles = seen < tiles ? seen : tiles;
   }
   tiles = tiles < 1 ? 1 : tiles;
-  const int64_t units = (int64_t)p.blocks * p.hkv;
-  int64_t parts = units < 2 * kSms ? 2 * kSms / units : 1;
-  parts = parts < tiles / 4 ? parts : tiles / 4;
-  parts = parts < 1 ? 1 : parts;
-  p.tiles_per_part = (int)((tiles + parts - 1) / parts);
-  p.parts = (int)((tiles + p.tiles_per_part - 1) / p.tiles_per_part);
+  const double units = (double)p.blocks * p.hkv, per_part = (double)p.rows * p.hq * (p.d + 2) * sizeof(float);
+  double best = INFINITY;
+  p.parts = 1, p.tiles_per_part = (int)tiles;
+  for (int parts = (int)((tiles + 511) / 512); parts <= 128 && (parts == 1 || parts <= tiles / 2); ++parts) {
+    if (parts > 1 && parts * per_part > (double)((size_t)2 << 30) && best < INFINITY) break;
+    const int each = (int)((tiles + parts - 1) / parts);
+    double time = units * parts <= places ? each + kPartCost : units * parts / places * (each + kPartCost) + 0.5 * each;
+    if (parts > 1) time += kJoinCost + 2 * parts * per_part / kJoinBytes;
+    if (time < best) best = time, p.parts = (int)((tiles + each - 1) / each), p.tiles_per_part = each;
+  }
 }
 
 size_t portion_scratch(PortionParams &p, void *base) {
@@ -85,15 +93,18 @@ bool portion_sizes_ok(int64_t rows, int batch, int hq, int hkv, int d, int page_
          (int64_t)max_blocks * page_tokens <= 0x7fffffff - 4096 && window >= 0;
 }
 
+// Everything but addresses.  The plan of the tensor-core kernel where that takes the sizes.
 PortionParams portion_params(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks, int num_pages,
-                             int64_t max_seq_len, int window, int dtype) {
+                             int64_t max_seq_len, int window, bool umma) {
   PortionParams p{};
   p.rows = (int)rows, p.batch = batch, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.d = d;
   p.page_tokens = page_tokens, p.max_blocks = max_blocks, p.num_pages = num_pages, p.window = window;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
-  plan_portions(p, max_seq_len, dtype, portion_fma_tokens(p.group));
+  plan_portions(p, max_seq_len, umma ? portion_umma_tokens(p.group) : portion_fma_tokens(p.group), 2 * kSms);
   return p;
 }
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
 }  // namespace axb
@@ -103,8 +114,14 @@ extern "C" {
 size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
                                                      int64_t max_seq_len, int window, int dtype) {
   if (!axb::portion_sizes_ok(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window) || rows == 0 || hq % hkv) return 0;
-  axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, dtype);
-  return axb::portion_scratch(p, nullptr);
+  const auto need = [&](bool umma) {
+    axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, umma);
+    return axb::portion_scratch(p, nullptr);
+  };
+  const size_t fma = need(false);
+  if (!axb::portion_umma_sizes(hq / hkv, d, dtype)) return fma;
+  const size_t umma = need(true);
+  return umma > fma ? umma : fma;  // which kernel serves a call depends on its addresses too
 }
 
 int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,
@@ -117,8 +134,10 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
   if (hq % hkv) return AXB200_SHAPE_MISMATCH;
   if (rows == 0) return AXB200_OK;
   if (!q || !out || !k_pages || !v_pages || !block_table || !seq_lens || !row_start) return AXB200_INVALID_PTR;
+  const bool umma = axb::portion_umma_sizes(hq / hkv, d, dtype) && axb::aligned16(q) && axb::aligned16(out) && axb::aligned16(k_pages) &&
+                    axb::aligned16(v_pages);
   axb::PortionParams p =
-      axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, num_pages, max_seq_len, window, dtype);
+      axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, num_pages, max_seq_len, window, umma);
   const size_t need = axb::portion_scratch(p, workspace);
   if (need && (!workspace || workspace_bytes < need)) return AXB200_OUT_OF_MEMORY;
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return AXB200_INVALID_PTR;
@@ -126,7 +145,7 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
   p.block_table = block_table, p.seq_lens = seq_lens, p.row_start = row_start;
   p.wait_ns = axb::wait_limit_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = axb::portions_fma(p, dtype, st);
+  const int rc = umma ? axb::portions_umma(p, st) : axb::portions_fma(p, dtype, st);
   if (rc != AXB200_OK || p.parts <= 1) return rc;
   const unsigned ctas = (unsigned)((rows * hq + 7) / 8);
   return dtype == AXB200_FLOAT32 ? axb::launch_dependent(axb::join_portions_kernel<float>, dim3(ctas), dim3(256), 0, st, p)

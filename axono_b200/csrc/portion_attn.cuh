@@ -40,11 +40,19 @@ struct PortionBlock {
   int tile0, tiles, parts; // tiles of all its keys, and into how many parts they are divided (at least one)
 };
 
-// Finds block `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a block of
-// at most 1024; the result is for all.  `found` is false beyond the last block.
-__device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block) {
-  __shared__ PortionBlock s_block;
-  __shared__ int s_sums[32], s_found;
+// What find_portion_block needs of shared memory.  An argument: static shared memory in front of tiles on 1024-byte boundaries would
+// take as much as that.
+struct PortionSearch {
+  PortionBlock block;
+  int found, sums[32];
+};
+
+// Finds block `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a CTA;
+// false beyond the last block.
+__device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block, PortionSearch *search) {
+  PortionBlock &s_block = search->block;
+  int *s_sums = search->sums;
+  volatile int &s_found = search->found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
   if (threadIdx.x == 0) s_found = 0;
   int before = 0;  // blocks of the sequences before this round's
@@ -116,10 +124,17 @@ __device__ __forceinline__ int portion_page(const PortionParams &p, int seq, int
   return p.num_pages;
 }
 
-// FLOAT16 on the tensor cores (portion_attn.cu) and anything on the FMA pipe (portion_attn_fma.cu): attention and, for p.parts > 1,
-// partial results.
-bool portions_on_tensor_cores(const PortionParams &p, int dtype);
-int portions_f16(const PortionParams &p, cudaStream_t st);
+// 1 / l; no key gives zero, and scores that are all -inf give NaN, as 0 / 0 does in the definition.
+__device__ __forceinline__ float portion_inverse(float l, bool some_key) { return l > 0.f ? 1.0f / l : l == 0.f && !some_key ? 0.f : NAN; }
+// (maximum in powers of two, denominator) of a part; -1 as denominator: keys, but scores of -inf alone.
+__device__ __forceinline__ float2 portion_ml(float m, float l, bool some_key) { return make_float2(m, l == 0.f && some_key ? -1.f : l); }
+
+// What serves a call: FLOAT16 on the tensor cores (portion_attn_umma.cu), all else on the FMA pipe (portion_attn_fma.cu).  Each gives its
+// rows per block, and with p.parts > 1 partial results.
+bool portion_umma_sizes(int group, int d, int dtype);
+int portion_umma_tokens(int group);
+int portions_umma(const PortionParams &p, cudaStream_t st);
+int portion_fma_tokens(int group);
 int portions_fma(const PortionParams &p, int dtype, cudaStream_t st);
 
 }  // namespace axb

@@ -23,6 +23,7 @@ template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kThreads)
 portion_fma_kernel(const PortionParams p) {
   extern __shared__ __align__(16) float smem[];
+  __shared__ PortionSearch search;
   const int ld = row_stride(p.d), d4 = (p.d + 3) / 4;
   float *q_s = smem, *k_s = q_s + kRows * ld, *v_s = k_s + kKeys * ld, *p_s = v_s + kKeys * ld;
   grid_dependency_launch();
@@ -36,7 +37,7 @@ portion_fma_kernel(const PortionParams p) {
   const int part = kSplit ? unit % p.parts : 0;
   if (kSplit) unit /= p.parts;
   PortionBlock block;
-  if (!find_portion_block(p, unit, block) || part >= block.parts) return;
+  if (!find_portion_block(p, unit, block, &search) || part >= block.parts) return;
   const int head0 = hk * p.group + slice * at_once, heads = min(at_once, p.group - slice * at_once);
   const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, block.parts);
   const int tile1 = block.tile0 + portion_part_begin(block.tiles, part + 1, block.parts);
@@ -121,8 +122,9 @@ portion_fma_kernel(const PortionParams p) {
   const bool divided = kSplit && block.parts > 1;
   if (kSplit && part == 0 && at_head == 0 && sub == 0) p.row_parts[at_row] = block.parts;
   const size_t place = kSplit ? portion_place(p, part, at_row, at_head) : 0;
-  if (divided && sub == 0) p.ml[place] = make_float2(m, l);
-  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : NAN;
+  const bool some_key = max(key_begin, tile0 * kPortionKeys) < min(key_end, tile1 * kPortionKeys);
+  if (divided && sub == 0) p.ml[place] = portion_ml(m, l, some_key);
+  const float inv = portion_inverse(l, some_key);
 #pragma unroll
   for (int j = 0; j < kMaxD / 16; ++j) {
     const float x[4] = {acc[j].x, acc[j].y, acc[j].z, acc[j].w};

@@ -1,0 +1,419 @@
+// Attention of portions over a paged cache on the 5th-generation tensor cores: FLOAT16, head sizes that are multiples of 8 up to 128.
+//
+// One CTA per block - 128 virtual rows: `tokens` rows of one sequence times the query heads of one KV head, head by head within a row -
+// and part of its keys, two CTAs per SM.  Tiles of 64 keys, each in one page, whose 64 rows of a KV head are one run of memory: TMA fetches
+// them through a map of the pool (d, page_tokens, hkv, num_pages).  S = Q.K^T (128 x 64) and O += P.V are tcgen05.mma with the sums in
+// tensor memory; thread t owns virtual row t: scores from tensor memory, online softmax in registers, P as fp16 pairs over the scores,
+// from where P.V takes its A operand.  S is computed two tiles ahead.  Few rows leave most of the 128 empty: their warps stay out, and
+// the products, which take as long as full ones, keep up with memory all the same (a tile of 32 KB in 660 cycles of an SM, 12 TB/s).
+//
+// Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
+// still meet weights of zero in P.V, so rows of V behind the sequence's end, where anything may stand, are cleared in shared memory
+// before the product, and a thread whose row is not finite does it over without them (redo_row).
+#include <math.h>
+
+#include <mutex>
+
+#include "portion_attn.cuh"
+#include "tcgen05.cuh"
+
+namespace axb {
+namespace {
+
+constexpr int kM = 128, kN = kPortionKeys, kD = 128;
+constexpr int kMmaWarp = 4, kLoadWarp = 5, kThreads = 192;
+constexpr int kQBytes = kM * kD * 2, kTileBytes = kN * kD * 2;  // two swizzled boxes of 64 elements each
+constexpr int kKStages = 3, kVStages = 2;
+constexpr int kOffK = kQBytes, kOffV = kOffK + kKStages * kTileBytes, kOffBar = kOffV + kVStages * kTileBytes;
+constexpr int kOffPages = kOffBar + 160, kPageRing = 64, kOffSearch = kOffPages + kPageRing * 4;
+constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
+constexpr float kLazyLog2 = 8.0f;
+
+// One row over the keys [key0, key1) as the definition has it, with fp32 weights: for results that are not finite, which a weight of
+// zero and a value of infinity give as well.  Un-normalised into `sums` where the keys are divided, else the result.
+__device__ __noinline__ void redo_row(const PortionParams &p, int seq, int row, int head, int key0, int key1, float *sums, float2 *ml) {
+  const int hk = head / p.group, pieces = p.d / 8;
+  const __half *q = static_cast<const __half *>(p.q) + ((size_t)row * p.hq + head) * p.d;
+  const auto key_row = [&](const void *pool, int key) {
+    const int page = p.block_table[(int64_t)seq * p.max_blocks + key / p.page_tokens];
+    if (page < 0 || page >= p.num_pages) return static_cast<const uint4 *>(nullptr);  // read as zeros
+    return reinterpret_cast<const uint4 *>(static_cast<const __half *>(pool) +
+                                           (((size_t)page * p.hkv + hk) * p.page_tokens + key % p.page_tokens) * p.d);
+  };
+  const auto dot2 = [](uint32_t a, uint32_t b, float s) {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+    return fmaf(x.y, y.y, fmaf(x.x, y.x, s));
+  };
+  const auto score = [&](int key) {
+    const uint4 *k = key_row(p.k_pages, key);
+    float s = 0.f;
+    if (!k) return s;
+    for (int c = 0; c < pieces; ++c) {
+      const uint4 a = reinterpret_cast<const uint4 *>(q)[c], b = k[c];
+      s = dot2(a.w, b.w, dot2(a.z, b.z, dot2(a.y, b.y, dot2(a.x, b.x, s))));
+    }
+    return s;
+  };
+  float m = -INFINITY;
+  for (int key = key0; key < key1; ++key) m = fmaxf(m, score(key));
+  const float shift = m == -INFINITY ? 0.f : m;
+  for (int c0 = 0; c0 < pieces; c0 += 4) {
+    float acc[32], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+    for (int key = key0; key < key1; ++key) {
+      const float w = exp2f((score(key) - shift) * p.scale_log2);
+      l += w;
+      const uint4 *v = key_row(p.v_pages, key);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (v && c0 + u < pieces) {
+          const uint4 x = v[c0 + u];
+          const uint32_t part[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&part[i]));
+            acc[u * 8 + 2 * i] = fmaf(w, f.x, acc[u * 8 + 2 * i]);
+            acc[u * 8 + 2 * i + 1] = fmaf(w, f.y, acc[u * 8 + 2 * i + 1]);
+          }
+        }
+    }
+    const float inv = portion_inverse(l, key0 < key1);
+    __half *out = static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d + c0 * 8;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c0 * 8 + i < p.d) {
+        if (ml)
+          sums[c0 * 8 + i] = acc[i];
+        else
+          out[i] = __float2half_rn(acc[i] * inv);
+      }
+    if (ml) *ml = portion_ml(m * p.scale_log2, l, key0 < key1);
+  }
+}
+
+// Warps 0-3: softmax, thread = virtual row; warp 4 issues the products; warp 5 the copies.  They meet on mbarriers: full / empty per
+// stage, bar_s (S_j ready, per buffer), bar_p (P_j written, per buffer, one arrival per softmax warp that has rows), bar_o (P_j.V_j
+// done), bar_fin (the last of them: the softmax warps skip phases of bar_o, and a wait by parity there would alias).  Every wait is
+// bounded.
+__global__ void __launch_bounds__(kThreads, 2)
+portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PortionParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kOffBar);
+  uint64_t *bar_q = bars, *full_k = bars + 1, *empty_k = bars + 4, *full_v = bars + 7, *empty_v = bars + 9, *bar_s = bars + 11,
+           *bar_o = bars + 13, *bar_fin = bars + 14, *bar_p = bars + 15;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 18);
+  int *pages = reinterpret_cast<int *>(smem + kOffPages);
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it; nothing is written
+    if (threadIdx.x == 0) atomicOr(&g_error_word, AXB200_ERR_WAIT_TIMEOUT);
+    return;
+  }
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    tma_prefetch_descriptor(&tm_q);
+    tma_prefetch_descriptor(&tm_k);
+    tma_prefetch_descriptor(&tm_v);
+  }
+  grid_dependency_launch();
+  grid_dependency_wait();
+  const int hk = blockIdx.x % p.hkv, rest = blockIdx.x / p.hkv;
+  const int part = p.parts > 1 ? rest % p.parts : 0, index = p.parts > 1 ? rest / p.parts : rest;
+  PortionBlock block;
+  if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(smem + kOffSearch)) || part >= block.parts) return;
+  const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, block.parts);
+  const int nkv = block.tile0 + portion_part_begin(block.tiles, part + 1, block.parts) - tile0;
+  const int virtual_rows = block.rows * p.group, active_warps = (virtual_rows + 31) >> 5;
+  const bool two_boxes = p.d > 64;
+  const uint32_t tile_bytes = two_boxes ? kTileBytes : kTileBytes / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 15; ++i) mbar_init(&bars[i], 1);
+    // one per S buffer: a softmax warp may be a tile ahead, and its second arrival would complete a phase that others have not reached
+    mbar_init(&bar_p[0], active_warps);
+    mbar_init(&bar_p[1], active_warps);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == kLoadWarp) pages[lane] = lane < nkv ? portion_page(p, block.seq, tile0 + lane) : p.num_pages;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;  // S buffers at columns 0 and 64
+
+  if (warp == kLoadWarp) {
+    if (nkv > 0) {
+      bool ok = true;
+      int nk = 0, nv = 0;  // tiles asked for, the same in all lanes
+      if (lane == 0) {
+        const uint32_t box = (uint32_t)(p.tokens * p.group * 128);
+        mbar_arrive_expect_tx(bar_q, two_boxes ? 2 * box : box);
+        tma_load_3d(smem, &tm_q, bar_q, 0, hk * p.group, block.row0);  // rows of the next sequence come along and are not stored
+        if (two_boxes) tma_load_3d(smem + kQBytes / 2, &tm_q, bar_q, 64, hk * p.group, block.row0);
+      }
+      auto load = [&](int &n, int stages, int off, const CUtensorMap &map, uint64_t *full, uint64_t *empty) {
+        const int s = n % stages;
+        if (lane == 0) {
+          if (n >= stages) ok = mbar_wait_bounded(&empty[s], (n / stages - 1) & 1, abort_flag, p.wait_ns);
+          if (ok) {
+            uint8_t *dst = smem + off + s * kTileBytes;
+            const int page = pages[n % kPageRing], in_page = (tile0 + n) * kN % p.page_tokens;
+            mbar_arrive_expect_tx(&full[s], tile_bytes);
+            tma_load_4d(dst, &map, &full[s], 0, in_page, hk, page);
+            if (two_boxes) tma_load_4d(dst + kTileBytes / 2, &map, &full[s], 64, in_page, hk, page);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (ok) ++n;
+      };
+      auto load_k = [&] {
+        if (nk > 0 && nk % 32 == 0) {  // the next pages: K is at most four tiles ahead of V, whose pages are in the ring's other half
+          const int t = nk + lane;
+          pages[t % kPageRing] = t < nkv ? portion_page(p, block.seq, tile0 + t) : p.num_pages;
+          __syncwarp();
+        }
+        load(nk, kKStages, kOffK, tm_k, full_k, empty_k);
+      };
+      // in the order of use, S_0 S_1 (P.V_0 S_2) (P.V_1 S_3) ...: K_0 K_1 K_2 V_0 K_3 V_1 ...
+      while (nk < 2 && nk < nkv && ok) load_k();
+      while (nv < nkv && ok) {
+        if (nk < nkv) load_k();
+        if (ok) load(nv, kVStages, kOffV, tm_v, full_v, empty_v);
+      }
+      if (*abort_flag && lane == 0) {  // no copy may still be on its way when the CTA leaves
+        const unsigned long long t0 = global_timer_ns();
+        auto drain = [&](uint64_t *bar, uint32_t parity) {
+          while (!mbar_try_wait(bar, parity) && global_timer_ns() - t0 < 100000000ull) {
+          }
+        };
+        drain(bar_q, 0);
+        for (int t = max(0, nk - kKStages); t < nk; ++t) drain(&full_k[t % kKStages], (t / kKStages) & 1);
+        for (int t = max(0, nv - kVStages); t < nv; ++t) drain(&full_v[t % kVStages], (t / kVStages) & 1);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // fp32 sums, fp16 operands, M = 128.  Q.K^T: N = 64 keys, B K-major; P.V: N = the head size to a multiple of 16, B MN-major
+    const int d_steps = (p.d + 15) / 16;
+    const uint32_t idesc_qk = (1u << 4) | ((kN >> 3) << 17) | ((kM >> 4) << 24);
+    const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(d_steps * 2) << 17) | ((kM >> 4) << 24);
+    const uint64_t dq = smem_desc(smem_u32(smem), 16, 1024), dk = smem_desc(smem_u32(smem + kOffK), 16, 1024);
+    const uint64_t dv = smem_desc(smem_u32(smem + kOffV), kTileBytes / 2, 1024);
+    auto issue_s = [&](int j) -> bool {
+      const int s = j & 1, sk = j % kKStages;
+      if (!mbar_wait_warp(&full_k[sk], (j / kKStages) & 1, abort_flag, p.wait_ns)) return false;
+      tc_fence_after();
+      const uint64_t dks = dk + (uint64_t)(sk * (kTileBytes >> 4));
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          if (ks >= d_steps) break;
+          const uint32_t q_off = (ks >> 2) * (kQBytes / 2) + (ks & 3) * 32, k_off = (ks >> 2) * (kTileBytes / 2) + (ks & 3) * 32;
+          umma_f16(tmem + s * kN, dq + (q_off >> 4), dks + (k_off >> 4), idesc_qk, ks > 0);
+        }
+        umma_commit(&bar_s[s]);
+        umma_commit(&empty_k[sk]);
+      }
+      return true;
+    };
+    bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns) && issue_s(0);
+    if (ok && nkv > 1) ok = issue_s(1);
+    for (int j = 0; j < nkv && ok; ++j) {
+      const int sv = j % kVStages;
+      ok = mbar_wait_warp(&full_v[sv], (j / kVStages) & 1, abort_flag, p.wait_ns);
+      if (!ok) break;
+      const int left = block.key_limit - (tile0 + j) * kN;  // keys of this tile that the sequence has
+      if (left < kN) {
+        uint4 *v = reinterpret_cast<uint4 *>(smem + kOffV + sv * kTileBytes);
+        for (int i = left * 8 + lane; i < kN * 8; i += 32) {
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (two_boxes) v[i + kTileBytes / 32] = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      ok = mbar_wait_warp(&bar_p[j & 1], (j >> 1) & 1, abort_flag, p.wait_ns);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t dvs = dv + (uint64_t)(sv * (kTileBytes >> 4));
+      if (elect_one()) {
+#pragma unroll
+        for (int ks = 0; ks < kN / 16; ++ks)
+          umma_f16_ts(tmem_o, tmem + (j & 1) * kN + ks * 8, dvs + (uint64_t)(ks * (2048 >> 4)), idesc_pv, j > 0 || ks > 0);
+        umma_commit(bar_o);
+        umma_commit(&empty_v[sv]);
+        if (j == nkv - 1) umma_commit(bar_fin);
+      }
+      // S_{j+2} takes the place of P_j, so P_j.V_j is waited for
+      if (j + 2 < nkv) ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns) && issue_s(j + 2);
+    }
+  } else if (warp < active_warps) {
+    const int token = threadIdx.x / p.group, head = hk * p.group + threadIdx.x % p.group;
+    const bool there = token < block.rows;
+    const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0;
+    const int key_begin = there && p.window ? max(0, pos + 1 - p.window) : 0;
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nkv && ok; ++j) {
+      const int sb = j & 1;
+      ok = mbar_wait_warp(&bar_s[sb], (j >> 1) & 1, abort_flag, p.wait_ns);
+      if (!ok) break;
+      tc_fence_after();
+      const int n0 = (tile0 + j) * kN;
+      uint32_t sr[2][32];
+      tmem_ld32_async(tmem + sb * kN + lane_base, sr[0]);
+      tmem_ld32_async(tmem + sb * kN + lane_base + 32, sr[1]);
+      tmem_wait_ld();
+      if (n0 + kN > key_end || n0 < key_begin) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n0 + c * 32 + i >= key_end || n0 + c * 32 + i < key_begin) sr[c][i] = 0xff800000u;  // -inf
+      }
+      // the running maximum moves only when some row of the warp has a score more than 2^kLazyLog2 above it; P and its sum hold that
+      const float m_tile = row_max(sr) * p.scale_log2;
+      float corr = 1.f;
+      const bool moved = __any_sync(0xffffffffu, m_tile > m_run + kLazyLog2);
+      if (moved) {
+        const float m_new = fmaxf(m_run, m_tile);
+        corr = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        m_run = m_new;
+      }
+      const float m_safe = m_run == -INFINITY ? 0.f : m_run;
+      const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), shift2 = pack_f32x2(-m_safe, -m_safe);
+      uint64_t sum2[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1])), scale2, shift2));
+          const float a = fast_exp2(x.x), b = fast_exp2(x.y);
+          sum2[(i >> 1) & 3] = add_f32x2(sum2[(i >> 1) & 3], pack_f32x2(a, b));
+          packed[i >> 1] = pack_half2(a, b);
+        }
+        tmem_st16(tmem + sb * kN + lane_base + c * 16, packed);
+      }
+      const float2 sum = unpack_f32x2(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])));
+      l_run = l_run * corr + (sum.x + sum.y);
+      // O moves with the maximum once P_{j-1}.V_{j-1} is done (P_j.V_j waits for this warp, so the barrier is at most a phase ahead)
+      if (j > 0 && moved) {
+        ok = mbar_wait_warp(bar_o, (j - 1) & 1, abort_flag, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c * 32 >= p.d) break;
+          uint32_t r[32];
+          tmem_ld32(tmem_o + lane_base + c * 32, r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+          tmem_st32(tmem_o + lane_base + c * 32, r);
+        }
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_p[sb]);
+    }
+    if (ok && nkv > 0) ok = mbar_wait_warp(bar_fin, 0, abort_flag, p.wait_ns);
+    tc_fence_after();
+    const int row = block.row0 + token;
+    const bool divided = block.parts > 1;
+    const int key0 = max(key_begin, tile0 * kN), key1 = min(key_end, (tile0 + nkv) * kN);
+    const size_t place = divided ? portion_place(p, part, row, head) : 0;
+    if (ok && p.parts > 1 && part == 0 && there && head == 0) p.row_parts[row] = block.parts;
+    if (ok && nkv == 0 && there) {  // no key at all
+      uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d);
+      for (int c = 0; c < p.d / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+    }
+    if (ok && nkv > 0) {
+      const float inv = portion_inverse(l_run, key0 < key1);
+      float bad = 0.f;  // NaN once a sum is not finite
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c * 32 >= p.d) break;
+        uint32_t r[32];
+        tmem_ld32(tmem_o + lane_base + c * 32, r);
+        if (there) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (c * 32 + u * 8 >= p.d) break;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              x[i] = __uint_as_float(r[u * 8 + i]);
+              bad = fmaf(x[i], 0.f, bad);
+            }
+            if (divided) {
+              float4 *dst = reinterpret_cast<float4 *>(p.sums + place * p.d + c * 32 + u * 8);
+              dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+              dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+              uint4 w;
+              w.x = pack_half2(x[0] * inv, x[1] * inv);
+              w.y = pack_half2(x[2] * inv, x[3] * inv);
+              w.z = pack_half2(x[4] * inv, x[5] * inv);
+              w.w = pack_half2(x[6] * inv, x[7] * inv);
+              *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d + c * 32 + u * 8) = w;
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (divided && there) p.ml[place] = portion_ml(m_run, l_run, key0 < key1);
+      if (there && bad != 0.f)
+        redo_row(p, block.seq, row, head, key0, key1, p.sums + place * p.d, divided ? p.ml + place : nullptr);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+}
+
+bool encode(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+int portion_umma_tokens(int group) { return kM / group; }
+
+bool portion_umma_sizes(int group, int d, int dtype) { return dtype == AXB200_FLOAT16 && d % 8 == 0 && d <= kD && group <= kM; }
+
+int portions_umma(const PortionParams &p, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  const cuuint64_t d = p.d, row = (cuuint64_t)p.d * 2;
+  const cuuint64_t q_dims[3] = {d, (cuuint64_t)p.hq, (cuuint64_t)p.rows}, q_strides[2] = {row, row * p.hq};
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.tokens};
+  const cuuint64_t dims[4] = {d, (cuuint64_t)p.page_tokens, (cuuint64_t)p.hkv, (cuuint64_t)p.num_pages};
+  const cuuint64_t strides[3] = {row, row * p.page_tokens, row * p.page_tokens * p.hkv};
+  const cuuint32_t box[4] = {64, kN, 1, 1};
+  if (!tensor_map_encoder() || !encode(&mq, p.q, 3, q_dims, q_strides, q_box) || !encode(&mk, p.k_pages, 4, dims, strides, box) ||
+      !encode(&mv, p.v_pages, 4, dims, strides, box))
+    return AXB200_INTERNAL_ERROR;
+  static std::mutex mu;
+  static bool opted[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return AXB200_DEVICE_ERROR;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!opted[dev] && cudaFuncSetAttribute(portion_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return AXB200_DEVICE_ERROR;
+    opted[dev] = true;
+  }
+  const int64_t ctas = (int64_t)p.blocks * p.hkv * p.parts;
+  if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
+  return launch_dependent(portion_umma_kernel, dim3((unsigned)ctas), dim3(kThreads), kSmem, st, mq, mk, mv, p);
+}
+
+}  // namespace axb
