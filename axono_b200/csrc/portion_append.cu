@@ -10,12 +10,14 @@
 // before the first and behind the last sequence are left alone, in the outputs too.
 #include <math.h>
 
+#include "tcgen05.cuh"
 #include "vec.cuh"
 
 namespace axb {
 namespace {
 
-constexpr int kThreads = 256, kMaxPairs = 128;  // head sizes up to 256
+constexpr int kMaxPairs = 128;  // head sizes up to 256
+constexpr int kThreads = 256, kRowThreads = 128, kRowBlocks = 6, kStages = 4;
 
 struct TurnParams {
   const void *q, *k;  // rows of q_ld and k_ld elements; v stands behind k in the form with a cache
@@ -41,63 +43,53 @@ __device__ __forceinline__ int64_t first_slot(const TurnParams &p, int len, int 
   return first < 0 || first + count > (int64_t)p.max_blocks * p.page_tokens ? -1 : first;
 }
 
-// What the threads of a block know about one of its rows.
+// What the threads of a warp know about a row.
 struct RowPlace {
   int64_t at[3];    // its position on each axis
   int64_t element;  // of head 0's key and value in the pools; -1: not written
-  int alive;        // belongs to a sequence
+  bool alive;       // belongs to a sequence
 };
 
-// One warp finds a row's sequence, slot and position.  row_start counts up, so that the sequence is the number of entries that are
-// not above the row; a table that does not count up is noticed where the entries found do not enclose the row.
-__device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowPlace *place) {
-  const int lane = threadIdx.x & 31;
-  int count = 0;
-  for (int i = lane; i <= p.batch; i += 32) count += p.row_start[i] <= row;
-  count = __reduce_add_sync(0xffffffffu, count);
-  if (lane != 0) return;
-  const int b = count - 1;
-  place->alive = 0;
-  place->element = -1;
-  if (b < 0 || b >= p.batch) return;  // a row of no sequence
-  const int r0 = p.row_start[b], r1 = p.row_start[b + 1];
-  if (r0 < 0 || r0 > row || r1 <= row || r1 > p.rows) {
-    atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
-    return;
-  }
-  place->alive = 1;
-  const int len = p.seq_lens[b];
-  const int64_t first = first_slot(p, len, r1 - r0), slot = first + (row - r0);
-  // a position is that of the slot even where the portion does not fit
-  const int64_t here = (p.advance ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);
-  for (int a = 0; a < 3; ++a) place->at[a] = !p.pos ? here : p.mrope ? p.pos[a * p.rows + row] : p.pos[row];
-  if (first < 0) {
-    atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
-    return;
-  }
-  const int page = p.block_table[(int64_t)b * p.max_blocks + slot / p.page_tokens];
-  if (page < 0 || page >= p.num_pages) {
-    atomicOr(&g_error_word, AXB200_ERR_BAD_PAGE);
-    return;
-  }
-  place->element = ((int64_t)page * p.hkv * p.page_tokens + slot % p.page_tokens) * p.d;
-}
-
+// A warp finds a row's sequence, slot and position.  row_start counts up, so that the sequence is the number of entries that are not
+// above the row; a table that does not count up is noticed where the entries found do not enclose the row.
 template <bool kAppend>
-__device__ __forceinline__ void place_or_position(const TurnParams &p, int64_t row, RowPlace *place) {
+__device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowPlace &place) {
+  place.alive = true;
+  place.element = -1;
+  int64_t here = 0;  // the row's slot, which is its position where none is given, even where the portion does not fit
   if constexpr (kAppend) {
-    place_row(p, row, place);
-  } else if ((threadIdx.x & 31) == 0) {
-    place->alive = 1;
-    if (p.pairs)
-      for (int a = 0; a < 3; ++a) place->at[a] = p.mrope ? p.pos[a * p.rows + row] : p.pos[row];
+    const int lane = threadIdx.x & 31;
+    int count = 0;
+    for (int i = lane; i <= p.batch; i += 32) count += p.row_start[i] <= row;
+    const int b = __reduce_add_sync(0xffffffffu, count) - 1;
+    place.alive = false;
+    if (b < 0 || b >= p.batch) return;  // a row of no sequence
+    const int r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
+    if (r0 < 0 || r0 > row || r1 <= row || r1 > p.rows) {
+      if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
+      return;
+    }
+    place.alive = true;
+    here = (p.advance ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);
+    if (first_slot(p, len, r1 - r0) < 0) {
+      if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
+    } else {
+      const int slot = (int)here, block = slot / p.page_tokens;
+      const int page = p.block_table[(int64_t)b * p.max_blocks + block];
+      if (page >= 0 && page < p.num_pages)
+        place.element = ((int64_t)page * p.hkv * p.page_tokens + (slot - block * p.page_tokens)) * p.d;
+      else if (lane == 0)
+        atomicOr(&g_error_word, AXB200_ERR_BAD_PAGE);
+    }
   }
+#pragma unroll
+  for (int a = 0; a < 3; ++a) place.at[a] = !p.pos || !p.pairs ? here : p.mrope ? p.pos[a * p.rows + row] : p.pos[row];
 }
 
 // factor * (cos, sin) of pair i at a row's position.
 __device__ __forceinline__ void pair_turn(const TurnParams &p, const int64_t (&at)[3], int i, float &c, float &s) {
-  const int axis = !p.mrope ? 0 : i % 3 == 1 && i < p.h_lim ? 1 : i % 3 == 2 && i < p.w_lim ? 2 : 0;
-  const double turns = (double)at[axis] * p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
+  const int64_t pos = !p.mrope ? at[0] : i % 3 == 1 && i < p.h_lim ? at[1] : i % 3 == 2 && i < p.w_lim ? at[2] : at[0];
+  const double turns = (double)pos * p.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
   sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
   c *= p.factor;
   s *= p.factor;
@@ -127,128 +119,201 @@ struct Heads {
   __device__ __forceinline__ const T *weight(int h) const { return static_cast<const T *>(h < p.hq ? p.q_w : p.k_w); }
 };
 
-// 16 bytes at a time.  kRows rows per block: their heads are dealt out to groups of `lanes` threads, each with two vectors of a head,
-// such that both elements of a pair are one thread's; the norm's sum goes over the group by shuffles.  Cosines and sines are formed
-// once per row and pair for all heads.  Four vectors pairs per thread are under way before the first is used.
-template <typename T, bool kAppend, int kRows>
-__global__ void __launch_bounds__(kThreads)
-turn_rows_kernel(const TurnParams p, int lanes) {
-  constexpr int kVec = 16 / (int)sizeof(T), kAhead = 4;
-  __shared__ __align__(16) float s_cos[kRows][kMaxPairs], s_sin[kRows][kMaxPairs];
-  __shared__ RowPlace s_place[kRows];
-  const Heads<T, kAppend> heads{p};
-  const int64_t row0 = (int64_t)blockIdx.x * kRows;
-  const int n_rows = (int)min((int64_t)kRows, p.rows - row0), warp = threadIdx.x >> 5;
-  const int per_row = heads.count() * lanes, items = n_rows * per_row;
-  const int vectors = p.d / kVec, turned = p.interleaved ? 0 : p.pairs / kVec;  // vectors that have a partner `turned` further on
+__device__ __forceinline__ void copy_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory");
+}
+
+// 16 bytes of T as floats, and back with one rounding.
+__device__ __forceinline__ void unpack16(const uint4 &raw, float (&x)[4], const float *) {
+  x[0] = __uint_as_float(raw.x), x[1] = __uint_as_float(raw.y), x[2] = __uint_as_float(raw.z), x[3] = __uint_as_float(raw.w);
+}
+__device__ __forceinline__ void unpack16(const uint4 &raw, float (&x)[8], const __half *) {
+  const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack16(const uint4 &raw, float (&x)[8], const __nv_bfloat16 *) {
+  const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+}
+__device__ __forceinline__ uint4 pack16(const float (&x)[4], const float *) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+__device__ __forceinline__ uint4 pack16(const float (&x)[8], const __half *) {
+  return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+}
+__device__ __forceinline__ uint4 pack16(const float (&x)[8], const __nv_bfloat16 *) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+}
+
+// 16 bytes at a time.  A warp takes a row, or with `ways` > 1 a share of a row's heads, and goes through its heads in groups: kLanes
+// threads take a head, two vectors each, such that both elements of a pair are one thread's and a thread has the same pairs in every
+// head, whose cosines and sines stay in its registers.  These are formed once per row, a few pairs per thread, and handed round through
+// shared memory; the norm's sum goes over a head's threads by shuffles.  Each thread copies its own vectors into its own places of
+// shared memory, kStages groups ahead and beyond the end of a row, so that loads are under way whatever the warp waits for; no
+// barrier is wider than a warp.  kFull: every thread has both vectors (head sizes of 2 * kLanes vectors).
+template <typename T, bool kAppend, bool kInterleaved, int kLanes, bool kFull>
+__global__ void __launch_bounds__(kRowThreads, kRowBlocks)
+turn_rows_kernel(const TurnParams p, int ways) {
+  constexpr int kVec = 16 / (int)sizeof(T), kAtOnce = 32 / kLanes;
+  constexpr const T *kType = nullptr;
+  __shared__ __align__(16) float s_cos[kRowThreads / 32][kMaxPairs], s_sin[kRowThreads / 32][kMaxPairs];
+  __shared__ __align__(16) uint4 s_raw[kRowThreads / 32][kStages][2][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & (kLanes - 1), group = lane / kLanes;
+  const int vectors = p.d / kVec, turned = p.pairs / kVec;  // halves: vectors that have a partner `turned` further on
+  // this thread's two vectors of every head, whether it has them, and whether they are turned: together in halves, each by itself
+  // interleaved
+  const int va = kInterleaved || c < turned ? c : 2 * c, vb = kInterleaved ? c + kLanes : c < turned ? c + turned : 2 * c + 1;
+  const bool has_a = kFull || va < vectors, has_b = kFull || vb < vectors;
+  const bool turn_a = kInterleaved ? has_a && va * (kVec / 2) < p.pairs : c < turned;
+  const bool turn_b = kInterleaved && has_b && vb * (kVec / 2) < p.pairs;
+  const float over_d = 1.0f / (float)p.d;
+  const unsigned mates = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1) << (group * kLanes);  // the threads of this head
+  const int rotated = p.hq + p.hkv, n_heads = rotated + (kAppend ? p.hkv : 0), share = (n_heads + ways - 1) / ways;
+  const int64_t tasks = p.rows * ways, step = (int64_t)gridDim.x * (kRowThreads / 32);
+  const int64_t first_task = (int64_t)blockIdx.x * (kRowThreads / 32) + warp;
+
+  // Heads of a row stand behind one another from two bases, the queries' and - moved back by the queries - the keys'.
   grid_dependency_launch();
   grid_dependency_wait();
-
-  struct Item {
-    int row, head, va, vb;  // vectors of the head; -1: none
+  int64_t ahead_task = first_task;
+  int ahead_head, ahead_end;
+  const T *ahead_q, *ahead_k;
+  const auto begin_ahead = [&] {
+    const int64_t row = ways == 1 ? ahead_task : ahead_task / ways;
+    ahead_head = ways == 1 ? 0 : (int)(ahead_task - row * ways) * share;
+    ahead_end = min(n_heads, ahead_head + share);
+    ahead_q = static_cast<const T *>(p.q) + row * p.q_ld;
+    ahead_k = static_cast<const T *>(p.k) + row * p.k_ld - p.hq * p.d;
   };
-  const auto item = [&](int i) {
-    Item it{i / per_row, 0, -1, -1};
-    const int rest = i - it.row * per_row, c = rest & (lanes - 1);
-    it.head = rest / lanes;
-    if (p.interleaved) {
-      it.va = c, it.vb = c + lanes;
+  begin_ahead();
+  int filled = 0;  // the stage that is filled next
+  const auto fetch = [&] {
+    if (ahead_task < tasks) {
+      const int h = ahead_head + group;
+      if (h < ahead_end) {
+        const uint4 *src = reinterpret_cast<const uint4 *>((h < p.hq ? ahead_q : ahead_k) + h * p.d);
+        if (has_a) copy_async16(&s_raw[warp][filled][0][lane], src + va);
+        if (has_b) copy_async16(&s_raw[warp][filled][1][lane], src + vb);
+      }
+      ahead_head += kAtOnce;
+      if (ahead_head >= ahead_end) {
+        ahead_task += step;
+        begin_ahead();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    filled = filled + 1 == kStages ? 0 : filled + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) fetch();
+
+  int stage = 0;
+  for (int64_t task = first_task; task < tasks; task += step) {
+    const int64_t row = ways == 1 ? task : task / ways;
+    const int head0 = ways == 1 ? 0 : (int)(task - row * ways) * share, end = min(n_heads, head0 + share);
+    RowPlace place;
+    place_row<kAppend>(p, row, place);
+    float cs[kVec], sn[kVec];
+    if (p.pairs && place.alive) {
+      __syncwarp();  // the row before has been read
+      for (int i = lane; i < p.pairs; i += 32) pair_turn(p, place.at, i, s_cos[warp][i], s_sin[warp][i]);
+      __syncwarp();
+      if (kInterleaved) {
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          if (turn_a) cs[i] = s_cos[warp][va * (kVec / 2) + i], sn[i] = s_sin[warp][va * (kVec / 2) + i];
+          if (turn_b) cs[kVec / 2 + i] = s_cos[warp][vb * (kVec / 2) + i], sn[kVec / 2 + i] = s_sin[warp][vb * (kVec / 2) + i];
+        }
+      } else if (turn_a) {
+        load_vec<kVec>(&s_cos[warp][va * kVec], cs);
+        load_vec<kVec>(&s_sin[warp][va * kVec], sn);
+      }
+    }
+    T *out_q = static_cast<T *>(p.q_out) + row * p.hq * p.d, *out_k, *out_v;
+    int head_step = p.d;  // between the heads of keys
+    if constexpr (kAppend) {
+      head_step = p.page_tokens * p.d;
+      out_k = static_cast<T *>(p.k_pages) + place.element;
+      out_v = static_cast<T *>(p.v_pages) + place.element;
     } else {
-      it.va = c < turned ? c : 2 * c;  // beyond the pairs, two neighbours
-      it.vb = c < turned ? c + turned : 2 * c + 1;
+      out_k = static_cast<T *>(p.k_out) + row * p.hkv * p.d, out_v = nullptr;
     }
-    if (it.va >= vectors) it.va = -1;
-    if (it.vb >= vectors) it.vb = -1;
-    return it;
-  };
-  uint4 raw[kAhead][2];
-  const auto fetch = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int i = base + j * kThreads + (int)threadIdx.x;
-      raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
-      if (i >= items) continue;
-      const Item it = item(i);
-      const uint4 *src = reinterpret_cast<const uint4 *>(heads.source(row0 + it.row, it.head));
-      if (it.va >= 0) raw[j][0] = src[it.va];
-      if (it.vb >= 0) raw[j][1] = src[it.vb];
-    }
-  };
-  fetch(0);
-  for (int r = warp; r < n_rows; r += kThreads / 32) place_or_position<kAppend>(p, row0 + r, &s_place[r]);
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_rows * p.pairs; i += kThreads) {
-    const int r = i / p.pairs, pair = i - r * p.pairs;
-    if (s_place[r].alive) pair_turn(p, s_place[r].at, pair, s_cos[r][pair], s_sin[r][pair]);
-  }
-  __syncthreads();
-
-  for (int base = 0; base < items; base += kAhead * kThreads) {
-    if (base) fetch(base);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int i = base + j * kThreads + (int)threadIdx.x;
-      if (base + j * kThreads >= items) break;  // the same for the whole block
-      const bool there = i < items;
-      const Item it = item(there ? i : 0);
-      const int64_t row = row0 + it.row;
-      float x[2][kVec];
-      load_vec<kVec>(reinterpret_cast<const T *>(&raw[j][0]), x[0]);
-      load_vec<kVec>(reinterpret_cast<const T *>(&raw[j][1]), x[1]);
-      const T *w = heads.weight(it.head);
-      float sum = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) sum = fmaf(x[u][e], x[u][e], sum);
-      for (int off = lanes >> 1; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      if (!there || !s_place[it.row].alive) continue;
-      T *dst = heads.target(row, it.head, s_place[it.row]);
-      if (!dst) continue;
-      const int v[2] = {it.va, it.vb};
-      if (heads.is_value(it.head)) {  // the bits as they came
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (v[u] >= 0) reinterpret_cast<uint4 *>(dst)[v[u]] = raw[j][u];
+    const bool written = !kAppend || place.element >= 0;
+#pragma unroll 1
+    for (int head = head0; head < end; head += kAtOnce) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      const int h = head + group;
+      uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (has_a) raw[0] = s_raw[warp][stage][0][lane];
+      if (has_b) raw[1] = s_raw[warp][stage][1][lane];
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+      fetch();  // into the stage that was read in the round before
+      if (h >= end || !place.alive) continue;
+      const bool query = h < p.hq;
+      if (kAppend && h >= rotated) {  // a value: the bits as they came
+        uint4 *dst = reinterpret_cast<uint4 *>(out_v + (int64_t)(h - rotated) * head_step);
+        if (written && has_a) dst[va] = raw[0];
+        if (written && has_b) dst[vb] = raw[1];
         continue;
       }
-      if (w) {
-        const float inv = 1.0f / sqrtf(sum / (float)p.d + p.eps);
+      float x[2][kVec];
+      unpack16(raw[0], x[0], kType);
+      unpack16(raw[1], x[1], kType);
+      if (const uint4 *w = static_cast<const uint4 *>(query ? p.q_w : p.k_w)) {
+        uint64_t sum2 = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < kVec; e += 2) {
+            const uint64_t y = pack_f32x2(x[u][e], x[u][e + 1]);
+            sum2 = fma_f32x2(y, y, sum2);
+          }
+        float sum = unpack_f32x2(sum2).x + unpack_f32x2(sum2).y;
+#pragma unroll
+        for (int off = kLanes >> 1; off > 0; off >>= 1) sum += __shfl_xor_sync(mates, sum, off);
+        const float inv = rsqrtf(fmaf(sum, over_d, p.eps));
+        const uint64_t inv2 = pack_f32x2(inv, inv);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          if (v[u] < 0) continue;
           float weight[kVec];
-          load_vec<kVec>(w + v[u] * kVec, weight);
+          unpack16((u ? has_b : has_a) ? w[u ? vb : va] : make_uint4(0, 0, 0, 0), weight, kType);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) x[u][e] = x[u][e] * inv * weight[e];
-        }
-      }
-      if (p.interleaved) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int pair0 = v[u] * (kVec / 2);
-          if (v[u] < 0 || pair0 >= p.pairs) continue;
-#pragma unroll
-          for (int e = 0; e < kVec / 2; ++e) {
-            const float c = s_cos[it.row][pair0 + e], s = s_sin[it.row][pair0 + e], a = x[u][2 * e], b = x[u][2 * e + 1];
-            x[u][2 * e] = rope_lo(a, b, c, s);
-            x[u][2 * e + 1] = rope_hi(a, b, c, s);
+          for (int e = 0; e < kVec; e += 2) {
+            const float2 y = unpack_f32x2(mul_f32x2(mul_f32x2(pack_f32x2(x[u][e], x[u][e + 1]), inv2), pack_f32x2(weight[e], weight[e + 1])));
+            x[u][e] = y.x, x[u][e + 1] = y.y;
           }
         }
-      } else if (v[0] >= 0 && v[0] < turned) {
-        float c[kVec], s[kVec];
-        load_vec<kVec>(&s_cos[it.row][v[0] * kVec], c);
-        load_vec<kVec>(&s_sin[it.row][v[0] * kVec], s);
+      }
+      if (kInterleaved) {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float a = x[0][e], b = x[1][e];
-          x[0][e] = rope_lo(a, b, c[e], s[e]);
-          x[1][e] = rope_hi(a, b, c[e], s[e]);
+        for (int u = 0; u < 2; ++u) {
+          if (!(u ? turn_b : turn_a)) continue;
+#pragma unroll
+          for (int e = 0; e < kVec / 2; ++e) {
+            const float a = x[u][2 * e], b = x[u][2 * e + 1], cc = cs[u * (kVec / 2) + e], ss = sn[u * (kVec / 2) + e];
+            x[u][2 * e] = rope_lo(a, b, cc, ss);
+            x[u][2 * e + 1] = rope_hi(a, b, cc, ss);
+          }
+        }
+      } else if (turn_a) {
+#pragma unroll
+        for (int e = 0; e < kVec; e += 2) {  // two pairs at a time
+          const uint64_t a = pack_f32x2(x[0][e], x[0][e + 1]), b = pack_f32x2(x[1][e], x[1][e + 1]);
+          const uint64_t c2 = pack_f32x2(cs[e], cs[e + 1]), s2 = pack_f32x2(sn[e], sn[e + 1]);
+          const float2 bs = unpack_f32x2(mul_f32x2(b, s2)), hi = unpack_f32x2(fma_f32x2(b, c2, mul_f32x2(a, s2)));
+          x[0][e] = __fmaf_rn(x[0][e], cs[e], -bs.x), x[0][e + 1] = __fmaf_rn(x[0][e + 1], cs[e + 1], -bs.y);
+          x[1][e] = hi.x, x[1][e + 1] = hi.y;
         }
       }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (v[u] >= 0) store_vec<kVec>(dst + v[u] * kVec, x[u]);
+      if (!query && !written) continue;
+      uint4 *dst = reinterpret_cast<uint4 *>(query ? out_q + h * p.d : out_k + (int64_t)(h - p.hq) * head_step);
+      if (has_a) dst[va] = pack16(x[0], kType);
+      if (has_b) dst[vb] = pack16(x[1], kType);
     }
   }
 }
@@ -259,20 +324,19 @@ __global__ void __launch_bounds__(kThreads)
 turn_row_any_kernel(const TurnParams p) {
   constexpr int kWarps = kThreads / 32, kPer = 2 * kMaxPairs / 32;
   __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs], s_head[kWarps][2 * kMaxPairs];
-  __shared__ RowPlace s_place;
   const Heads<T, kAppend> heads{p};
   const int64_t row = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_launch();
   grid_dependency_wait();
-  if (warp == 0) place_or_position<kAppend>(p, row, &s_place);
-  __syncthreads();
-  if (!s_place.alive) return;
-  for (int i = threadIdx.x; i < p.pairs; i += kThreads) pair_turn(p, s_place.at, i, s_cos[i], s_sin[i]);
+  RowPlace place;
+  place_row<kAppend>(p, row, place);
+  if (!place.alive) return;  // the same for the block
+  for (int i = threadIdx.x; i < p.pairs; i += kThreads) pair_turn(p, place.at, i, s_cos[i], s_sin[i]);
   __syncthreads();
   for (int h = warp; h < heads.count(); h += kWarps) {
     const T *src = heads.source(row, h), *w = heads.weight(h);
-    T *dst = heads.target(row, h, s_place);
+    T *dst = heads.target(row, h, place);
     if (!dst) continue;
     if (heads.is_value(h)) {
       for (int i = lane; i < p.d; i += 32) dst[i] = src[i];
@@ -285,7 +349,7 @@ turn_row_any_kernel(const TurnParams p) {
       x[j] = i < p.d ? ldf(src + i) : 0.f;
       sum = fmaf(x[j], x[j], sum);
     }
-    const float inv = w ? 1.0f / sqrtf(warp_sum(sum) / (float)p.d + p.eps) : 1.f;
+    const float inv = w ? rsqrtf(warp_sum(sum) / (float)p.d + p.eps) : 1.f;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = lane + 32 * j;
@@ -332,6 +396,20 @@ advance_lengths_kernel(const TurnParams p, int32_t *seq_lens) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+template <typename T, bool kAppend, int kLanes>
+int launch_rows(const TurnParams &p, cudaStream_t st) {
+  constexpr int kVec = 16 / (int)sizeof(T), kAtOnce = 32 / kLanes;
+  const int n_heads = p.hq + (kAppend ? 2 : 1) * p.hkv;
+  int ways = 1;
+  while (p.rows * ways < 148 * 8 && ways * 2 * kAtOnce <= n_heads) ways *= 2;
+  const int64_t blocks = (p.rows * ways + kRowThreads / 32 - 1) / (kRowThreads / 32), most = 148 * kRowBlocks;
+  const bool full = p.d == 2 * kLanes * kVec;
+  auto *kernel = p.interleaved ? full ? turn_rows_kernel<T, kAppend, true, kLanes, true> : turn_rows_kernel<T, kAppend, true, kLanes, false>
+                 : full        ? turn_rows_kernel<T, kAppend, false, kLanes, true>
+                               : turn_rows_kernel<T, kAppend, false, kLanes, false>;
+  return launch_dependent(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kRowThreads), 0, st, p, ways);
+}
+
 template <typename T, bool kAppend>
 int launch_turn(const TurnParams &p, cudaStream_t st) {
   constexpr int kVec = 16 / (int)sizeof(T);
@@ -340,9 +418,12 @@ int launch_turn(const TurnParams &p, cudaStream_t st) {
                        aligned16(p.v_pages) && aligned16(p.q_w) && aligned16(p.k_w);
   if (!whole || !aligned)
     return launch_dependent(turn_row_any_kernel<T, kAppend>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p);
-  int lanes = 1;
-  while (2 * lanes * kVec < p.d) lanes *= 2;
-  return launch_dependent(turn_rows_kernel<T, kAppend, 1>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p, lanes);
+  const int vectors = p.d / kVec;
+  if (vectors <= 4 || vectors > 64) return launch_dependent(turn_row_any_kernel<T, kAppend>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p);
+  return vectors <= 8    ? launch_rows<T, kAppend, 4>(p, st)
+         : vectors <= 16 ? launch_rows<T, kAppend, 8>(p, st)
+         : vectors <= 32 ? launch_rows<T, kAppend, 16>(p, st)
+                         : launch_rows<T, kAppend, 32>(p, st);
 }
 
 bool turn_sizes_ok(const TurnParams &p) {
