@@ -93,14 +93,14 @@ bool portion_sizes_ok(int64_t rows, int batch, int hq, int hkv, int d, int page_
          (int64_t)max_blocks * page_tokens <= 0x7fffffff - 4096 && window >= 0;
 }
 
-// Everything but addresses.  The plan of the tensor-core kernel where that takes the sizes.
+// Everything but addresses, with the plan of the tensor-core kernel or of the other.
 PortionParams portion_params(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks, int num_pages,
-                             int64_t max_seq_len, int window, bool umma) {
+                             int64_t max_seq_len, int window, int dtype, bool tensor) {
   PortionParams p{};
   p.rows = (int)rows, p.batch = batch, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.d = d;
   p.page_tokens = page_tokens, p.max_blocks = max_blocks, p.num_pages = num_pages, p.window = window;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
-  plan_portions(p, max_seq_len, umma ? portion_umma_tokens(p.group) : portion_fma_tokens(p.group), 2 * kSms);
+  plan_portions(p, max_seq_len, tensor ? kPortionRows / p.group : portion_fma_tokens(p.group), tensor && dtype == AXB200_FLOAT32 ? kSms : 2 * kSms);
   return p;
 }
 
@@ -114,14 +114,14 @@ extern "C" {
 size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
                                                      int64_t max_seq_len, int window, int dtype) {
   if (!axb::portion_sizes_ok(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window) || rows == 0 || hq % hkv) return 0;
-  const auto need = [&](bool umma) {
-    axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, umma);
+  const auto need = [&](bool tensor) {
+    axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, dtype, tensor);
     return axb::portion_scratch(p, nullptr);
   };
   const size_t fma = need(false);
-  if (!axb::portion_umma_sizes(hq / hkv, d, dtype)) return fma;
-  const size_t umma = need(true);
-  return umma > fma ? umma : fma;  // which kernel serves a call depends on its addresses too
+  if (!axb::portion_tensor_sizes(hq / hkv, d, dtype)) return fma;
+  const size_t tensor = need(true);
+  return tensor > fma ? tensor : fma;  // which kernel serves a call depends on its addresses too
 }
 
 int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,
@@ -134,10 +134,10 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
   if (hq % hkv) return AXB200_SHAPE_MISMATCH;
   if (rows == 0) return AXB200_OK;
   if (!q || !out || !k_pages || !v_pages || !block_table || !seq_lens || !row_start) return AXB200_INVALID_PTR;
-  const bool umma = axb::portion_umma_sizes(hq / hkv, d, dtype) && axb::aligned16(q) && axb::aligned16(out) && axb::aligned16(k_pages) &&
-                    axb::aligned16(v_pages);
+  const bool tensor = axb::portion_tensor_sizes(hq / hkv, d, dtype) && axb::aligned16(q) && axb::aligned16(out) &&
+                      axb::aligned16(k_pages) && axb::aligned16(v_pages);
   axb::PortionParams p =
-      axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, num_pages, max_seq_len, window, umma);
+      axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, num_pages, max_seq_len, window, dtype, tensor);
   const size_t need = axb::portion_scratch(p, workspace);
   if (need && (!workspace || workspace_bytes < need)) return AXB200_OUT_OF_MEMORY;
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return AXB200_INVALID_PTR;
@@ -145,7 +145,9 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
   p.block_table = block_table, p.seq_lens = seq_lens, p.row_start = row_start;
   p.wait_ns = axb::wait_limit_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = umma ? axb::portions_umma(p, st) : axb::portions_fma(p, dtype, st);
+  const int rc = !tensor                    ? axb::portions_fma(p, dtype, st)
+                 : dtype == AXB200_FLOAT32 ? axb::portions_f32(p, st)
+                                           : axb::portions_umma(p, st);
   if (rc != AXB200_OK || p.parts <= 1) return rc;
   const unsigned ctas = (unsigned)((rows * hq + 7) / 8);
   return dtype == AXB200_FLOAT32 ? axb::launch_dependent(axb::join_portions_kernel<float>, dim3(ctas), dim3(256), 0, st, p)

@@ -129,11 +129,80 @@ __device__ __forceinline__ float portion_inverse(float l, bool some_key) { retur
 // (maximum in powers of two, denominator) of a part; -1 as denominator: keys, but scores of -inf alone.
 __device__ __forceinline__ float2 portion_ml(float m, float l, bool some_key) { return make_float2(m, l == 0.f && some_key ? -1.f : l); }
 
-// What serves a call: FLOAT16 on the tensor cores (portion_attn_umma.cu), all else on the FMA pipe (portion_attn_fma.cu).  Each gives its
-// rows per block, and with p.parts > 1 partial results.
-bool portion_umma_sizes(int group, int d, int dtype);
-int portion_umma_tokens(int group);
+// Four consecutive elements as floats.
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const __half *p) {
+  const uint2 raw = *reinterpret_cast<const uint2 *>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// A warp does one row of a block over - its keys from key0 to key1 - as the definition has it, with fp32 multiplications and only the keys
+// that the row sees: what the tensor-core kernels cannot finish (a weight of zero times an infinite value, values without exact parts).
+// Scores with lane = key, sums with lane = four columns.  d: a multiple of 4 up to 128.
+template <typename T>
+__device__ __noinline__ void redo_portion_row(const PortionParams &p, const PortionBlock &block, int part, int token, int head, int key0,
+                                              int key1) {
+  const int lane = threadIdx.x & 31, hk = head / p.group, row = block.row0 + token, pos = block.first_pos + token;
+  key1 = min(key1, min(pos + 1, block.key_limit));
+  if (p.window) key0 = max(key0, pos + 1 - p.window);
+  const T *q = static_cast<const T *>(p.q) + ((size_t)row * p.hq + head) * p.d;
+  const auto key_row = [&](const void *pool, int key) {  // null: a page outside the pool, read as zeros
+    const int page = p.block_table[(int64_t)block.seq * p.max_blocks + key / p.page_tokens];
+    if (page < 0 || page >= p.num_pages) return static_cast<const T *>(nullptr);
+    return static_cast<const T *>(pool) + (((size_t)page * p.hkv + hk) * p.page_tokens + key % p.page_tokens) * p.d;
+  };
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int first = key0; first < key1; first += 32) {
+    const int key = first + lane;
+    float s = -INFINITY;
+    if (key < key1) {
+      const T *k = key_row(p.k_pages, key);
+      s = 0.f;
+      for (int c = 0; k && c < p.d; c += 4) {
+        const float4 a = load4(q + c), b = load4(k + c);
+        s = fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, s))));
+      }
+      s *= p.scale_log2;
+    }
+    float m_new = fmaxf(m, s);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, off));
+    const float shift = m_new == -INFINITY ? 0.f : m_new, corr = exp2f(m - shift), w = key < key1 ? exp2f(s - shift) : 0.f;
+    m = m_new;
+    l = l * corr + warp_sum(w);
+    acc.x *= corr, acc.y *= corr, acc.z *= corr, acc.w *= corr;
+    for (int i = 0; i < min(32, key1 - first); ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const T *v = key_row(p.v_pages, first + i);
+      if (!v || lane * 4 >= p.d) continue;
+      const float4 x = load4(v + lane * 4);
+      acc.x = fmaf(wi, x.x, acc.x), acc.y = fmaf(wi, x.y, acc.y), acc.z = fmaf(wi, x.z, acc.z), acc.w = fmaf(wi, x.w, acc.w);
+    }
+  }
+  const bool divided = block.parts > 1;
+  const size_t place = divided ? portion_place(p, part, row, head) : 0;
+  if (divided && lane == 0) p.ml[place] = portion_ml(m, l, key0 < key1);
+  if (lane * 4 >= p.d) return;
+  const float inv = divided ? 1.f : portion_inverse(l, key0 < key1), x[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (divided)
+      p.sums[place * p.d + lane * 4 + e] = x[e];
+    else
+      stf(static_cast<T *>(p.out) + ((size_t)row * p.hq + head) * p.d + lane * 4 + e, x[e] * inv);
+  }
+}
+
+// What serves a call: the tensor cores in FLOAT16 (portion_attn_umma.cu) and FLOAT32 (portion_attn_f32.cu), all else the FMA pipe
+// (portion_attn_fma.cu).  Each gives its rows per block, and with p.parts > 1 partial results.
+constexpr int kPortionRows = 128;  // virtual rows of a block on the tensor cores
+inline bool portion_tensor_sizes(int group, int d, int dtype) {
+  return d % (dtype == AXB200_FLOAT16 ? 8 : 4) == 0 && d <= 128 && group <= kPortionRows;
+}
 int portions_umma(const PortionParams &p, cudaStream_t st);
+int portions_f32(const PortionParams &p, cudaStream_t st);
 int portion_fma_tokens(int group);
 int portions_fma(const PortionParams &p, int dtype, cudaStream_t st);
 

@@ -9,7 +9,7 @@
 //
 // Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
 // still meet weights of zero in P.V, so rows of V behind the sequence's end, where anything may stand, are cleared in shared memory
-// before the product, and a thread whose row is not finite does it over without them (redo_row).
+// before the product, and rows that are not finite are done over without them (redo_portion_row).
 #include <math.h>
 
 #include <mutex>
@@ -20,7 +20,7 @@
 namespace axb {
 namespace {
 
-constexpr int kM = 128, kN = kPortionKeys, kD = 128;
+constexpr int kM = kPortionRows, kN = kPortionKeys, kD = 128;
 constexpr int kMmaWarp = 4, kLoadWarp = 5, kThreads = 192;
 constexpr int kQBytes = kM * kD * 2, kTileBytes = kN * kD * 2;  // two swizzled boxes of 64 elements each
 constexpr int kKStages = 3, kVStages = 2;
@@ -28,69 +28,6 @@ constexpr int kOffK = kQBytes, kOffV = kOffK + kKStages * kTileBytes, kOffBar = 
 constexpr int kOffPages = kOffBar + 160, kPageRing = 64, kOffSearch = kOffPages + kPageRing * 4;
 constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
 constexpr float kLazyLog2 = 8.0f;
-
-// One row over the keys [key0, key1) as the definition has it, with fp32 weights: for results that are not finite, which a weight of
-// zero and a value of infinity give as well.  Un-normalised into `sums` where the keys are divided, else the result.
-__device__ __noinline__ void redo_row(const PortionParams &p, int seq, int row, int head, int key0, int key1, float *sums, float2 *ml) {
-  const int hk = head / p.group, pieces = p.d / 8;
-  const __half *q = static_cast<const __half *>(p.q) + ((size_t)row * p.hq + head) * p.d;
-  const auto key_row = [&](const void *pool, int key) {
-    const int page = p.block_table[(int64_t)seq * p.max_blocks + key / p.page_tokens];
-    if (page < 0 || page >= p.num_pages) return static_cast<const uint4 *>(nullptr);  // read as zeros
-    return reinterpret_cast<const uint4 *>(static_cast<const __half *>(pool) +
-                                           (((size_t)page * p.hkv + hk) * p.page_tokens + key % p.page_tokens) * p.d);
-  };
-  const auto dot2 = [](uint32_t a, uint32_t b, float s) {
-    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&a)), y = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-    return fmaf(x.y, y.y, fmaf(x.x, y.x, s));
-  };
-  const auto score = [&](int key) {
-    const uint4 *k = key_row(p.k_pages, key);
-    float s = 0.f;
-    if (!k) return s;
-    for (int c = 0; c < pieces; ++c) {
-      const uint4 a = reinterpret_cast<const uint4 *>(q)[c], b = k[c];
-      s = dot2(a.w, b.w, dot2(a.z, b.z, dot2(a.y, b.y, dot2(a.x, b.x, s))));
-    }
-    return s;
-  };
-  float m = -INFINITY;
-  for (int key = key0; key < key1; ++key) m = fmaxf(m, score(key));
-  const float shift = m == -INFINITY ? 0.f : m;
-  for (int c0 = 0; c0 < pieces; c0 += 4) {
-    float acc[32], l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-    for (int key = key0; key < key1; ++key) {
-      const float w = exp2f((score(key) - shift) * p.scale_log2);
-      l += w;
-      const uint4 *v = key_row(p.v_pages, key);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (v && c0 + u < pieces) {
-          const uint4 x = v[c0 + u];
-          const uint32_t part[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&part[i]));
-            acc[u * 8 + 2 * i] = fmaf(w, f.x, acc[u * 8 + 2 * i]);
-            acc[u * 8 + 2 * i + 1] = fmaf(w, f.y, acc[u * 8 + 2 * i + 1]);
-          }
-        }
-    }
-    const float inv = portion_inverse(l, key0 < key1);
-    __half *out = static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d + c0 * 8;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (c0 * 8 + i < p.d) {
-        if (ml)
-          sums[c0 * 8 + i] = acc[i];
-        else
-          out[i] = __float2half_rn(acc[i] * inv);
-      }
-    if (ml) *ml = portion_ml(m * p.scale_log2, l, key0 < key1);
-  }
-}
 
 // Warps 0-3: softmax, thread = virtual row; warp 4 issues the products; warp 5 the copies.  They meet on mbarriers: full / empty per
 // stage, bar_s (S_j ready, per buffer), bar_p (P_j written, per buffer, one arrival per softmax warp that has rows), bar_o (P_j.V_j
@@ -368,8 +305,12 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         __syncwarp();
       }
       if (divided && there) p.ml[place] = portion_ml(m_run, l_run, key0 < key1);
-      if (there && bad != 0.f)
-        redo_row(p, block.seq, row, head, key0, key1, p.sums + place * p.d, divided ? p.ml + place : nullptr);
+      __syncwarp();  // other lanes write such a row anew
+      const unsigned again = __ballot_sync(0xffffffffu, there && bad != 0.f);
+      for (unsigned left = again; left; left &= left - 1) {
+        const int r = warp * 32 + __ffs(left) - 1;
+        redo_portion_row<__half>(p, block, part, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
+      }
     }
   }
   tc_fence_before();
@@ -385,10 +326,6 @@ bool encode(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims
 }
 
 }  // namespace
-
-int portion_umma_tokens(int group) { return kM / group; }
-
-bool portion_umma_sizes(int group, int d, int dtype) { return dtype == AXB200_FLOAT16 && d % 8 == 0 && d <= kD && group <= kM; }
 
 int portions_umma(const PortionParams &p, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
