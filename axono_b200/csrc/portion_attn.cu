@@ -7,71 +7,109 @@ namespace {
 
 constexpr int kSms = 148;
 
-// out = sum_i 2^(m_i - m) sums_i / sum_i 2^(m_i - m) l_i over the parts of a row's keys; a warp per row and head.  Rows whose keys were
-// not divided have their result already.
-template <typename T>
-__global__ void __launch_bounds__(256)
+// out = sum_i 2^(m_i - m) sums_i / sum_i 2^(m_i - m) l_i over the parts of a row's keys; a warp per row and head, four columns per lane.
+// Rows whose keys were not divided have their result already.  Bound by the way to L2: the sums of eight parts are under way at once.
+template <typename T, int kVecs>
+__global__ void __launch_bounds__(128)
 join_portions_kernel(const PortionParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  constexpr int kAhead = 8 / kVecs;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, row = (int)(i / p.hq), head = (int)(i - (int64_t)row * p.hq);
   grid_dependency_launch();
   grid_dependency_wait();
-  if (row >= p.rows || row < p.row_start[0] || row >= p.row_start[p.batch]) return;
-  const int parts = min(p.row_parts[row], p.parts);
-  if (parts <= 1) return;
+  if (row >= p.rows) return;
+  const int first_row = p.row_start[0], end_row = p.row_start[p.batch], parts = min(p.row_parts[row], p.parts);
+  if (row < first_row || row >= end_row || parts <= 1) return;
   float m = -INFINITY;
   for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.ml[portion_place(p, k, row, head)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
   const float shift = m == -INFINITY ? 0.f : m;
+  const size_t step = (size_t)p.rows * p.hq * p.d;
+  const float *sums = p.sums + portion_place(p, 0, row, head) * p.d;
+  const bool whole = p.d % 4 == 0;
   bool some = false;
-  float l = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < parts; ++k) {
-    const size_t place = portion_place(p, k, row, head);
-    const float2 ml = p.ml[place];
-    some = some || ml.y != 0.f;
-    if (ml.x == -INFINITY && ml.y <= 0.f) continue;  // no key, or no score above -inf
-    const float w = exp2f(ml.x - shift);
-    l = fmaf(w, ml.y, l);
+  float l = 0.f, acc[kVecs][4] = {};
+  for (int base = 0; base < parts; base += 32) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (base + lane < parts) mine = p.ml[portion_place(p, base + lane, row, head)];
+    const bool there = !(mine.x == -INFINITY && mine.y <= 0.f);  // else no key, or no score above -inf
+    const float weight = there ? exp2f(mine.x - shift) : 0.f;
+    some = some || mine.y != 0.f;
+    l += there ? weight * mine.y : 0.f;
+    const unsigned use = __ballot_sync(0xffffffffu, there);
+    for (int k0 = 0; k0 < 32 && base + k0 < parts; k0 += kAhead) {
+      float x[kAhead][kVecs][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (lane + 32 * j < p.d) acc[j] = fmaf(w, p.sums[place * p.d + lane + 32 * j], acc[j]);
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) {
+          const int c = (lane + 32 * v) * 4;
+          const float *src = sums + (base + k0 + k) * step + c;
+          if (!((use >> (k0 + k)) & 1)) continue;
+          if (whole) {
+            if (c < p.d) *reinterpret_cast<float4 *>(x[k][v]) = *reinterpret_cast<const float4 *>(src);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < p.d) x[k][v][e] = src[e];
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const float w = __shfl_sync(0xffffffffu, weight, k0 + k);
+        if (!((use >> (k0 + k)) & 1)) continue;
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((lane + 32 * v) * 4 + e < p.d) acc[v][e] = fmaf(w, x[k][v][e], acc[v][e]);
+      }
+    }
   }
-  const float inv = portion_inverse(l, some);
+  l = warp_sum(l);
+  const float inv = portion_inverse(l, __any_sync(0xffffffffu, some));
+  T *dst = static_cast<T *>(p.out) + ((size_t)row * p.hq + head) * p.d;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (lane + 32 * j < p.d) stf(static_cast<T *>(p.out) + ((size_t)row * p.hq + head) * p.d + lane + 32 * j, acc[j] * inv);
+  for (int v = 0; v < kVecs; ++v)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = (lane + 32 * v) * 4 + e;
+      if (c < p.d) stf(dst + c, acc[v][e] * inv);
+    }
+}
+
+template <typename T>
+int join_portions(const PortionParams &p, cudaStream_t st) {
+  const dim3 ctas((unsigned)(((int64_t)p.rows * p.hq + 3) / 4));
+  return launch_dependent(p.d <= 128 ? join_portions_kernel<T, 1> : join_portions_kernel<T, 2>, ctas, dim3(128), 0, st, p);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Rows per block and how the keys are divided, from sizes and bounds alone.  In units of a tile's time: blocks that all run at once take
-// their longest part, else an even share of all and half of the last; a block or part costs kPartCost tiles beside its own, joining
-// kJoinCost and the way of the partial results to memory and back.  A part has 512 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 32768 keys are
-// 2048 products.
-constexpr double kPartCost = 6, kJoinCost = 8, kJoinBytes = 1.4e6;  // bytes moved in a tile's time
-void plan_portions(PortionParams &p, int64_t max_seq_len, int tokens, int places) {
-  p.tokens = tokens;
-  const int some = p.rows < p.batch ? p.rows : p.batch;  // sequences with rows: each may add a block that is not full
-  p.blocks = some + (p.rows - some) / tokens;
+// Rows per block, and the bounds within which the kernels divide the keys: where all blocks run at once, into as many parts as do.
+// A part has 1024 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 65536 keys are 4096 products.
+void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32) {
+  p.tokens = tensor ? kPortionRows / p.group : portion_fma_tokens(p.group);
+  const int places = tensor && f32 ? kSms : 2 * kSms;
   const int64_t pages = (int64_t)p.max_blocks * p.page_tokens;
   p.max_keys = (int)(max_seq_len < pages ? max_seq_len : pages);
   int64_t tiles = ((int64_t)p.max_keys + kPortionKeys - 1) / kPortionKeys;
   if (p.window) {
-    const int64_t seen = ((int64_t)p.window + tokens + kPortionKeys - 3) / kPortionKeys + 1;  // keys of a block, wherever they begin
+    const int64_t seen = ((int64_t)p.window + p.tokens + kPortionKeys - 3) / kPortionKeys + 1;  // keys of a block, wherever they begin
     tiles = seen < tiles ? seen : tiles;
   }
   tiles = tiles < 1 ? 1 : tiles;
-  const double units = (double)p.blocks * p.hkv, per_part = (double)p.rows * p.hq * (p.d + 2) * sizeof(float);
-  double best = INFINITY;
-  p.parts = 1, p.tiles_per_part = (int)tiles;
-  for (int parts = (int)((tiles + 511) / 512); parts <= 128 && (parts == 1 || parts <= tiles / 2); ++parts) {
-    if (parts > 1 && parts * per_part > (double)((size_t)2 << 30) && best < INFINITY) break;
-    const int each = (int)((tiles + parts - 1) / parts);
-    double time = units * parts <= places ? each + kPartCost : units * parts / places * (each + kPartCost) + 0.5 * each;
-    if (parts > 1) time += kJoinCost + 2 * parts * per_part / kJoinBytes;
-    if (time < best) best = time, p.parts = (int)((tiles + each - 1) / each), p.tiles_per_part = each;
-  }
+  const int some = p.rows < p.batch ? p.rows : p.batch;  // sequences with rows: each may add a block that is not full
+  const int64_t blocks = some + (p.rows - some) / p.tokens;
+  const int64_t needed = (tiles + kPortionMostTiles - 1) / kPortionMostTiles, at_once = places / p.hkv;
+  const size_t per_part = (size_t)p.rows * p.hq * (p.d + 2) * sizeof(float);
+  int64_t parts = blocks < at_once ? (tiles / 2 < 128 ? tiles / 2 : 128) : 1;
+  while (parts > 1 && parts * per_part > ((size_t)1 << 30)) --parts;
+  p.parts = (int)(parts > needed ? parts : needed);
+  p.units = (int)(p.parts > 1 && at_once > blocks * needed ? at_once : blocks * needed);
+  p.least_gain = f32 ? 3.f : 6.f;
+  p.part_gain = (float)(2. * per_part / (f32 ? 8e6 : 3e6));
 }
 
 size_t portion_scratch(PortionParams &p, void *base) {
@@ -100,7 +138,7 @@ PortionParams portion_params(int64_t rows, int batch, int hq, int hkv, int d, in
   p.rows = (int)rows, p.batch = batch, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.d = d;
   p.page_tokens = page_tokens, p.max_blocks = max_blocks, p.num_pages = num_pages, p.window = window;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)d));
-  plan_portions(p, max_seq_len, tensor ? kPortionRows / p.group : portion_fma_tokens(p.group), tensor && dtype == AXB200_FLOAT32 ? kSms : 2 * kSms);
+  plan_portions(p, max_seq_len, tensor, dtype == AXB200_FLOAT32);
   return p;
 }
 
@@ -149,9 +187,7 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
                  : dtype == AXB200_FLOAT32 ? axb::portions_f32(p, st)
                                            : axb::portions_umma(p, st);
   if (rc != AXB200_OK || p.parts <= 1) return rc;
-  const unsigned ctas = (unsigned)((rows * hq + 7) / 8);
-  return dtype == AXB200_FLOAT32 ? axb::launch_dependent(axb::join_portions_kernel<float>, dim3(ctas), dim3(256), 0, st, p)
-                                 : axb::launch_dependent(axb::join_portions_kernel<__half>, dim3(ctas), dim3(256), 0, st, p);
+  return dtype == AXB200_FLOAT32 ? axb::join_portions<float>(p, st) : axb::join_portions<__half>(p, st);
 }
 
 }  // extern "C"

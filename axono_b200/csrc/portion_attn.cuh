@@ -13,7 +13,9 @@
 
 namespace axb {
 
-constexpr int kPortionKeys = 64;  // keys of a tile, which lies in one page
+constexpr int kPortionKeys = 64;   // keys of a tile, which lies in one page
+constexpr int kPortionWarps = 14;  // of a CTA at most
+constexpr int kPortionMostTiles = 1024;  // of a part
 
 struct PortionParams {
   const void *q;
@@ -21,10 +23,11 @@ struct PortionParams {
   const void *k_pages, *v_pages;
   const int32_t *block_table, *seq_lens, *row_start;
   int rows, batch, hq, hkv, group, d, page_tokens, max_blocks, num_pages, window;
-  int max_keys;                  // keys of a sequence that the grid is made for
-  int tokens, blocks;            // rows of a block; blocks that the rows can need at most
-  int parts, tiles_per_part;     // parts that a block's tiles can need at most
-  float scale_log2;              // of scores, in powers of two
+  int max_keys;       // keys of a sequence that the grid is made for
+  int tokens, units;  // rows of a block; blocks and parts of blocks that the grid has for a KV head
+  int parts;          // the most parts that a block's keys are divided into; 1: not at all
+  float least_gain, part_gain;  // tiles in a row that dividing has to save, and that each further part has to
+  float scale_log2;  // of scores, in powers of two
   unsigned long long wait_ns;
   // with parts > 1, results of blocks with divided keys: un-normalised sums (part, row, head, d), their (maximum, denominator), and of
   // every row the number of its parts
@@ -34,31 +37,27 @@ struct PortionParams {
 };
 
 struct PortionBlock {
-  int seq, row0, rows;     // its first row and how many
-  int first_pos;           // position of the first row
-  int key_limit;           // keys of the sequence that may be read
-  int tile0, tiles, parts; // tiles of all its keys, and into how many parts they are divided (at least one)
+  int seq, row0, rows;  // its first row and how many
+  int first_pos;        // position of the first row
+  int key_limit;        // keys of the sequence that may be read
+  int tile0, tiles;     // tiles of all its keys
+  int part, parts;      // the part of them that this CTA takes; at least one, and a CTA whose part is not below leaves
 };
 
 // What find_portion_block needs of shared memory.  An argument: static shared memory in front of tiles on 1024-byte boundaries would
 // take as much as that.
 struct PortionSearch {
   PortionBlock block;
-  int found, sums[32];
+  int found, sums[kPortionWarps];
+  float totals[3][kPortionWarps];
 };
 
-// Finds block `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a CTA;
-// false beyond the last block.
-__device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block, PortionSearch *search) {
-  PortionBlock &s_block = search->block;
-  int *s_sums = search->sums;
-  volatile int &s_found = search->found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
-  if (threadIdx.x == 0) s_found = 0;
-  int before = 0;  // blocks of the sequences before this round's
-  for (int base = 0; base < p.batch; base += blockDim.x) {
-    const int b = base + threadIdx.x;
-    int r0 = 0, r1 = 0, len = 0;
+// One sequence of a launch.
+struct PortionSpan {
+  int r0, count, len, blocks;
+  __device__ __forceinline__ PortionSpan(const PortionParams &p, int b) {
+    r0 = 0, len = 0;
+    int r1 = 0;
     if (b < p.batch) {
       r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
       if (r0 < 0 || r1 < r0 || r1 > p.rows) {
@@ -66,7 +65,67 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
         r0 = r1 = 0;
       }
     }
-    const int mine = (r1 - r0 + p.tokens - 1) / p.tokens;
+    count = r1 - r0;
+    blocks = (count + p.tokens - 1) / p.tokens;
+  }
+  // the tiles of the keys of rows [first, first + rows) of it
+  __device__ __forceinline__ void tiles(const PortionParams &p, int first, int rows, int &tile0, int &n) const {
+    const int pos = len - count + first, end = min(pos + rows, min(max(len, 0), p.max_keys));
+    const int begin = p.window ? max(0, pos + 1 - p.window) : 0;
+    tile0 = begin / kPortionKeys;
+    n = end > begin ? (end + kPortionKeys - 1) / kPortionKeys - tile0 : 0;
+  }
+};
+
+// Finds block and part `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a
+// CTA; false beyond the last.
+//
+// Where blocks may be too few to fill the GPU, every CTA first makes the same plan from the lengths: the blocks of a sequence get
+// ceil(t / L) parts, t the tiles at its end.  With N blocks and V = sum of blocks x t these are at most V / L + N, so that L = V / (units -
+// N) fits the grid, whose units run at once.
+__device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block, PortionSearch *search) {
+  volatile int &s_found = search->found;
+  int *s_sums = search->sums;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+  if (threadIdx.x == 0) s_found = 0;
+  float part_tiles = (float)kPortionMostTiles;  // L
+  if (p.parts > 1) {
+    float n = 0.f, v = 0.f, most = 0.f;
+    for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
+      const PortionSpan s(p, b);
+      if (s.blocks == 0) continue;
+      int tile0, last;
+      s.tiles(p, (s.blocks - 1) * p.tokens, s.count - (s.blocks - 1) * p.tokens, tile0, last);
+      n += s.blocks;
+      v += (float)s.blocks * last;
+      most = fmaxf(most, last);
+    }
+    n = warp_sum(n);
+    v = warp_sum(v);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+    if (lane == 0) search->totals[0][warp] = n, search->totals[1][warp] = v, search->totals[2][warp] = most;
+    __syncthreads();
+    n = v = most = 0.f;
+    for (int w = 0; w < warps; ++w) {
+      n += search->totals[0][w];
+      v += search->totals[1][w];
+      most = fmaxf(most, search->totals[2][w]);
+    }
+    if (n < p.units) {
+      const float length = ceilf(fmaxf(v * 1.001f / (p.units - n), sqrtf(most * 0.12f)));  // joining a part takes 0.12 tiles
+      if (length >= 1.f && most - length > p.least_gain + p.part_gain * most / length) part_tiles = fminf(part_tiles, length);
+    }
+  }
+  int before = 0;  // blocks and parts of the sequences before this round's
+  for (int base = 0; base < p.batch; base += blockDim.x) {
+    const PortionSpan s(p, base + (int)threadIdx.x);
+    int tile0, tiles, parts = 1;
+    if (p.parts > 1 && s.blocks) {
+      s.tiles(p, (s.blocks - 1) * p.tokens, s.count - (s.blocks - 1) * p.tokens, tile0, tiles);
+      parts = min(p.parts, max(1, (int)ceilf((float)tiles / part_tiles)));
+    }
+    const int at_end = p.parts > 1 ? tiles : 0, mine = s.blocks * parts;
     int upto = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -81,30 +140,28 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
       if (w < warp) upto += n;
       total += n;
     }
-    const int at = index - before - (upto - mine);  // among this sequence's blocks
+    const int at = index - before - (upto - mine);  // among this sequence's
     if (at >= 0 && at < mine) {
-      const int first = (mine - 1 - at) * p.tokens, count = r1 - r0;
       PortionBlock f;
-      f.seq = b;
-      f.row0 = r0 + first;
-      f.rows = min(p.tokens, count - first);
-      f.first_pos = len - count + first;
-      f.key_limit = min(max(len, 0), p.max_keys);
-      if (len > p.max_keys) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
-      const int end = min(f.first_pos + f.rows, f.key_limit);
-      const int begin = p.window ? max(0, f.first_pos + 1 - p.window) : 0;
-      f.tile0 = begin / kPortionKeys;
-      f.tiles = end > begin ? (end + kPortionKeys - 1) / kPortionKeys - f.tile0 : 0;
-      f.parts = max(1, (f.tiles + p.tiles_per_part - 1) / p.tiles_per_part);
-      s_block = f;
+      const int i = at / parts, first = (s.blocks - 1 - i) * p.tokens;
+      f.seq = base + threadIdx.x;
+      f.row0 = s.r0 + first;
+      f.rows = min(p.tokens, s.count - first);
+      f.first_pos = s.len - s.count + first;
+      f.key_limit = min(max(s.len, 0), p.max_keys);
+      if (s.len > p.max_keys) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
+      s.tiles(p, first, f.rows, f.tile0, f.tiles);
+      f.part = at - i * parts;
+      f.parts = parts == 1 ? 1 : min(parts, max(1, (int)(((int64_t)f.tiles * parts + at_end - 1) / max(at_end, 1))));
+      search->block = f;
       s_found = 1;
     }
     before += total;
     __syncthreads();
     if (s_found || before > index) break;
   }
-  block = s_block;
-  return s_found;
+  block = search->block;
+  return s_found && block.part < block.parts;
 }
 
 __host__ __device__ inline int portion_part_begin(int tiles, int part, int parts) { return (int)((int64_t)tiles * part / parts); }
@@ -141,8 +198,7 @@ __device__ __forceinline__ float4 load4(const __half *p) {
 // that the row sees: what the tensor-core kernels cannot finish (a weight of zero times an infinite value, values without exact parts).
 // Scores with lane = key, sums with lane = four columns.  d: a multiple of 4 up to 128.
 template <typename T>
-__device__ __noinline__ void redo_portion_row(const PortionParams &p, const PortionBlock &block, int part, int token, int head, int key0,
-                                              int key1) {
+__device__ __noinline__ void redo_portion_row(const PortionParams &p, const PortionBlock &block, int token, int head, int key0, int key1) {
   const int lane = threadIdx.x & 31, hk = head / p.group, row = block.row0 + token, pos = block.first_pos + token;
   key1 = min(key1, min(pos + 1, block.key_limit));
   if (p.window) key0 = max(key0, pos + 1 - p.window);
@@ -182,7 +238,7 @@ __device__ __noinline__ void redo_portion_row(const PortionParams &p, const Port
     }
   }
   const bool divided = block.parts > 1;
-  const size_t place = divided ? portion_place(p, part, row, head) : 0;
+  const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
   if (divided && lane == 0) p.ml[place] = portion_ml(m, l, key0 < key1);
   if (lane * 4 >= p.d) return;
   const float inv = divided ? 1.f : portion_inverse(l, key0 < key1), x[4] = {acc.x, acc.y, acc.z, acc.w};

@@ -32,11 +32,12 @@ template <int kB>
 struct Layout {
   static constexpr int kRawTile = kN * 64 * kB * 4, kPart = kB * kBox, kTile = 3 * kPart;
   static constexpr int kOffK = kRaw * kRawTile, kOffV = kOffK + kTile, kOffCorr = kOffV + kTile, kOffL = kOffCorr + 2 * kM * 4;
-  static constexpr int kOffBar = kOffL + 2 * kM * 4, kOffPages = kOffBar + 256, kOffSearch = kOffPages + kPageRing * 4;
-  static constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
+  static constexpr int kOffBar = kOffL + 2 * kM * 4, kOffPages = kOffBar + 256;
+  static constexpr int kSmem = kOffPages + kPageRing * 4;
   static constexpr int kQCols = 96 * kB, kSpCols = 96, kColO = kQCols + 2 * kSpCols;
 };
 static_assert(Layout<2>::kSmem <= 232448, "shared memory of a CTA");
+static_assert(sizeof(PortionSearch) <= 2 * kM * 4, "the search is over before rescale factors stand in its place");
 
 // Three bf16 parts of each of two floats; their sum is exact.
 __device__ __forceinline__ void split3(float a, float b, uint32_t &h, uint32_t &m, uint32_t &l) {
@@ -60,7 +61,7 @@ struct Range {
 // The order in which tiles are used, and copied: K_0 K_1 V_0, then K_{j+2} V_{j+1}.
 struct TileOrder {
   int k = 0, v = 0;
-  __device__ __forceinline__ bool next_is_k(int tiles) const { return k < tiles && k < v + 2; }
+  __device__ __forceinline__ bool next_is_k(int tiles) const { return k < tiles && k < v + 2; }  // else V, the last of them one too far
 };
 
 template <int kB>
@@ -94,12 +95,11 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   }
   grid_dependency_launch();
   grid_dependency_wait();
-  const int hk = blockIdx.x % p.hkv, rest = blockIdx.x / p.hkv;
-  const int part = p.parts > 1 ? rest % p.parts : 0, index = p.parts > 1 ? rest / p.parts : rest;
+  const int hk = blockIdx.x % p.hkv, index = blockIdx.x / p.hkv;
   PortionBlock block;
-  if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(smem + L::kOffSearch)) || part >= block.parts) return;
-  const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, block.parts);
-  const int nkv = block.tile0 + portion_part_begin(block.tiles, part + 1, block.parts) - tile0;
+  if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(corr_s))) return;
+  const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
+  const int nkv = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts) - tile0;
   const int active = (block.rows * p.group + 31) >> 5;  // warps' worth of rows: tensor memory's quarters that matter
 
   if (threadIdx.x == 0) {
@@ -127,7 +127,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const uint32_t tmem_sp = tmem + L::kQCols, tmem_o = tmem + L::kColO;
   const int vrow = threadIdx.x & (kM - 1), token = vrow / p.group, head = hk * p.group + vrow % p.group;  // of warps 0 to 11
   const bool there = token < block.rows;
-  const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0;
+  // rows that are none are left unmasked, as in portion_attn_umma.cu
+  const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0x7fffffff;
   const int key_begin = there && p.window ? max(0, pos + 1 - p.window) : 0;
   const int row = block.row0 + token;
 
@@ -168,43 +169,46 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t idesc_qk = bf16 | ((kN >> 3) << 17), idesc_pv = bf16 | (1u << 16) | ((uint32_t)(d_steps * 2) << 17);
     const uint64_t dk = smem_desc(smem_u32(smem + L::kOffK), 16, 1024), dv = smem_desc(smem_u32(smem + L::kOffV), kBox, 1024);
     constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kC[6] = {2, 0, 1, 1, 0, 0};  // parts of A and B, smallest products first
-    auto issue_s = [&](int j) -> bool {
-      const int s = j & 1;
-      if (!mbar_wait_warp(full_k, j & 1, abort_flag, p.wait_ns)) return false;
-      tc_fence_after();
-      if (elect_one()) {
+    // round i: P_{i-2}.V_{i-2}, then S_i in its place, with one copy of each in the instruction cache
+    bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns);
+#pragma unroll 1
+    for (int i = 0; i < nkv + 2 && ok; ++i) {
+      const int s = i & 1;
+      if (i >= 2) {
+        const int j = i - 2;
+        ok = mbar_wait_warp(&bar_p[s], (j >> 1) & 1, abort_flag, p.wait_ns) && mbar_wait_warp(full_v, j & 1, abort_flag, p.wait_ns) &&
+             (j == 0 || mbar_wait_warp(&bar_c[s ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.wait_ns));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < 6; ++i)
+          for (int c = 0; c < 6; ++c)
 #pragma unroll
-          for (int ks = 0; ks < 4 * kB; ++ks) {
-            if (ks >= d_steps) break;
-            umma_f16_ts(tmem_sp + s * L::kSpCols, tmem + kA[i] * 32 * kB + ks * 8,
-                        dk + (uint64_t)((kC[i] * L::kPart + (ks >> 2) * kBox + (ks & 3) * 32) >> 4), idesc_qk, i > 0 || ks > 0);
-          }
-        umma_commit(&bar_s[s]);
-        umma_commit(empty_k);
+            for (int ks = 0; ks < kN / 16; ++ks)
+              umma_f16_ts(tmem_o, tmem_sp + s * L::kSpCols + kA[c] * 32 + ks * 8, dv + (uint64_t)((kC[c] * L::kPart + ks * 2048) >> 4),
+                          idesc_pv, c > 0 || ks > 0);
+          umma_commit(bar_o);
+        }
+        if (i >= nkv) continue;
+        ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns);  // S_i takes the place of P_{i-2}
+        if (!ok) break;
       }
-      return true;
-    };
-    bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns) && issue_s(0);
-    if (ok && nkv > 1) ok = issue_s(1);
-    for (int j = 0; j < nkv && ok; ++j) {
-      const int s = j & 1;
-      ok = mbar_wait_warp(&bar_p[s], (j >> 1) & 1, abort_flag, p.wait_ns) && mbar_wait_warp(full_v, j & 1, abort_flag, p.wait_ns) &&
-           (j == 0 || mbar_wait_warp(&bar_c[s ^ 1], ((j - 1) >> 1) & 1, abort_flag, p.wait_ns));
+      if (i >= nkv) continue;
+      ok = mbar_wait_warp(full_k, i & 1, abort_flag, p.wait_ns);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int i = 0; i < 6; ++i)
+        for (int c = 0; c < 6; ++c)
 #pragma unroll
-          for (int ks = 0; ks < kN / 16; ++ks)
-            umma_f16_ts(tmem_o, tmem_sp + s * L::kSpCols + kA[i] * 32 + ks * 8, dv + (uint64_t)((kC[i] * L::kPart + ks * 2048) >> 4),
-                        idesc_pv, i > 0 || ks > 0);
-        umma_commit(bar_o);
+          for (int ks = 0; ks < 4 * kB; ++ks) {
+            if (ks >= d_steps) break;
+            umma_f16_ts(tmem_sp + s * L::kSpCols, tmem + kA[c] * 32 * kB + ks * 8,
+                        dk + (uint64_t)((kC[c] * L::kPart + (ks >> 2) * kBox + (ks & 3) * 32) >> 4), idesc_qk, c > 0 || ks > 0);
+          }
+        umma_commit(&bar_s[s]);
+        umma_commit(empty_k);
       }
-      // S_{j+2} takes the place of P_j, so P_j.V_j is waited for
-      if (j + 2 < nkv) ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns) && issue_s(j + 2);
     }
   } else if (warp < 4) {
     if (warp < active) {
@@ -296,13 +300,47 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int i = 0; i < 16 * kB; ++i) acc[i] = 0;
     bool ok = nkv > 0;
     int n = 0;  // tiles of floats used
-    const auto split_tile = [&](int j, int off, uint64_t *full) {
+    // tiles of floats in the order of their use; O_{j-1} is added up before V_j takes the place of V_{j-1}
+    TileOrder at;
+#pragma unroll 1
+    while (ok) {
+      const bool is_k = at.next_is_k(nkv);
+      const int j = is_k ? at.k++ : at.v++;
+      if (is_k) {
+        if (j > 0) ok = mbar_wait_warp(empty_k, (j - 1) & 1, abort_flag, p.wait_ns);
+      } else if (j > 0) {
+        const int s = (j - 1) & 1;
+        if (mine) ok = mbar_wait_warp(&bar_p[s], ((j - 1) >> 1) & 1, abort_flag, p.wait_ns);
+        if (!ok) break;
+        const float corr = mine ? corr_s[s * kM + vrow] : 0.f;
+        ok = mbar_wait_warp(bar_o, (j - 1) & 1, abort_flag, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        if (mine) {
+          const uint64_t corr2 = pack_f32x2(corr, corr);
+#pragma unroll
+          for (int c = 0; c < kB; ++c) {
+            if (half * 32 * kB + c * 32 >= p.d) break;
+            uint32_t r[32];
+            tmem_ld32(tmem_o + lane_base + half * 32 * kB + c * 32, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              acc[c * 16 + i] = fma_f32x2(acc[c * 16 + i], corr2, pack_f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])));
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_c[s]);
+        }
+        if (j == nkv) break;
+      }
+      if (!ok) break;
       const int s = n % kRaw;
       ok = mbar_wait_warp(&raw_full[s], (n / kRaw) & 1, abort_flag, p.wait_ns);
-      if (!ok) return;
+      if (!ok) break;
       const int left = block.key_limit - (tile0 + j) * kN;  // keys that the sequence has; behind them anything may stand
       const float4 *src = reinterpret_cast<const float4 *>(smem + s * L::kRawTile);
-#pragma unroll
+      uint8_t *parts_at = smem + (is_k ? L::kOffK : L::kOffV);
+#pragma unroll 2
       for (int i = 0; i < 4 * kB; ++i) {
         const int id = (helper * 4 * kB + i) * 32 + lane, key = id / (16 * kB), c = id % (16 * kB);
         float4 x = src[id];
@@ -311,7 +349,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         uint2 h, m, l;
         split3(x.x, x.y, h.x, m.x, l.x);
         split3(x.z, x.w, h.y, m.y, l.y);
-        uint8_t *dst = smem + off + (c >> 4) * kBox + key * 128 + ((((c & 15) >> 1) ^ (key & 7)) << 4) + (c & 1) * 8;
+        uint8_t *dst = parts_at + (c >> 4) * kBox + key * 128 + ((((c & 15) >> 1) ^ (key & 7)) << 4) + (c & 1) * 8;
         *reinterpret_cast<uint2 *>(dst) = h;
         *reinterpret_cast<uint2 *>(dst + L::kPart) = m;
         *reinterpret_cast<uint2 *>(dst + 2 * L::kPart) = l;
@@ -320,50 +358,17 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&raw_empty[s]);
-        mbar_arrive(full);
+        mbar_arrive(is_k ? full_k : full_v);
       }
       ++n;
-    };
-    const auto split_k = [&](int j) {
-      if (j > 0) ok = mbar_wait_warp(empty_k, (j - 1) & 1, abort_flag, p.wait_ns);
-      if (ok) split_tile(j, L::kOffK, full_k);
-    };
-    if (ok) split_k(0);
-    if (ok && nkv > 1) split_k(1);
-    if (ok) split_tile(0, L::kOffV, full_v);
-    for (int j = 0; j < nkv && ok; ++j) {
-      const int s = j & 1;
-      if (j + 2 < nkv) split_k(j + 2);
-      if (ok && mine) ok = mbar_wait_warp(&bar_p[s], (j >> 1) & 1, abort_flag, p.wait_ns);
-      if (!ok) break;
-      const float corr = mine ? corr_s[s * kM + vrow] : 0.f;
-      ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns);
-      if (!ok) break;
-      tc_fence_after();
-      if (mine) {
-        const uint64_t corr2 = pack_f32x2(corr, corr);
-#pragma unroll
-        for (int c = 0; c < kB; ++c) {
-          if (half * 32 * kB + c * 32 >= p.d) break;
-          uint32_t r[32];
-          tmem_ld32(tmem_o + lane_base + half * 32 * kB + c * 32, r);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            acc[c * 16 + i] = fma_f32x2(acc[c * 16 + i], corr2, pack_f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])));
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_c[s]);
-      }
-      if (j + 1 < nkv) split_tile(j + 1, L::kOffV, full_v);
     }
     if (range.unsplittable()) *bad_flag = 1;
     if (ok && mine) ok = mbar_wait_warp(bar_l, 0, abort_flag, p.wait_ns);
     if ((ok || nkv == 0) && mine && there) {
       const bool some_key = max(key_begin, tile0 * kN) < min(key_end, (tile0 + nkv) * kN), divided = block.parts > 1;
       const float l = nkv > 0 ? l_s[vrow] : 0.f;
-      const size_t place = divided ? portion_place(p, part, row, head) : 0;
-      if (p.parts > 1 && part == 0 && head == 0 && half == 0) p.row_parts[row] = block.parts;
+      const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
+      if (p.parts > 1 && block.part == 0 && head == 0 && half == 0) p.row_parts[row] = block.parts;
       if (divided && half == 0) p.ml[place] = portion_ml(l_s[kM + vrow], l, some_key);
       const float inv = divided ? 1.f : portion_inverse(l, some_key);
       float *dst = divided ? p.sums + place * p.d : static_cast<float *>(p.out) + ((size_t)row * p.hq + head) * p.d;
@@ -381,7 +386,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   if (*bad_flag && !*abort_flag)
     for (int r = warp; r < block.rows * p.group; r += kThreads / 32)
-      redo_portion_row<float>(p, block, part, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
+      redo_portion_row<float>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
 }
 
 template <int kB>
@@ -396,7 +401,7 @@ int launch(const PortionParams &p, const CUtensorMap &mk, const CUtensorMap &mv,
       return AXB200_DEVICE_ERROR;
     opted[dev] = true;
   }
-  const int64_t ctas = (int64_t)p.blocks * p.hkv * p.parts;
+  const int64_t ctas = (int64_t)p.units * p.hkv;
   if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
   return launch_dependent(portion_f32_kernel<kB>, dim3((unsigned)ctas), dim3(kThreads), Layout<kB>::kSmem, st, mk, mv, p);
 }

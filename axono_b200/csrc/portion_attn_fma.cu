@@ -34,13 +34,11 @@ portion_fma_kernel(const PortionParams p) {
   unit /= slices;
   const int hk = unit % p.hkv;
   unit /= p.hkv;
-  const int part = kSplit ? unit % p.parts : 0;
-  if (kSplit) unit /= p.parts;
   PortionBlock block;
-  if (!find_portion_block(p, unit, block, &search) || part >= block.parts) return;
+  if (!find_portion_block(p, unit, block, &search)) return;
   const int head0 = hk * p.group + slice * at_once, heads = min(at_once, p.group - slice * at_once);
-  const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, block.parts);
-  const int tile1 = block.tile0 + portion_part_begin(block.tiles, part + 1, block.parts);
+  const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
+  const int tile1 = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts);
 
   const T *q = static_cast<const T *>(p.q);
   for (int i = threadIdx.x; i < kRows * 4 * d4; i += kThreads) {
@@ -120,8 +118,8 @@ portion_fma_kernel(const PortionParams p) {
   if (!there) return;
   const int at_row = block.row0 + token, at_head = head0 + head;
   const bool divided = kSplit && block.parts > 1;
-  if (kSplit && part == 0 && at_head == 0 && sub == 0) p.row_parts[at_row] = block.parts;
-  const size_t place = kSplit ? portion_place(p, part, at_row, at_head) : 0;
+  if (kSplit && block.part == 0 && at_head == 0 && sub == 0) p.row_parts[at_row] = block.parts;
+  const size_t place = kSplit ? portion_place(p, block.part, at_row, at_head) : 0;
   const bool some_key = max(key_begin, tile0 * kPortionKeys) < min(key_end, tile1 * kPortionKeys);
   if (divided && sub == 0) p.ml[place] = portion_ml(m, l, some_key);
   const float inv = portion_inverse(l, some_key);
@@ -156,7 +154,7 @@ int launch(const PortionParams &p, cudaStream_t st) {
     }
   }
   const int at_once = heads_at_once(p.group), slices = (p.group + at_once - 1) / at_once;
-  const int64_t ctas = (int64_t)p.blocks * p.hkv * slices * (kSplit ? p.parts : 1);
+  const int64_t ctas = (int64_t)p.units * p.hkv * slices;
   if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
   return launch_dependent(portion_fma_kernel<T, kSplit>, dim3((unsigned)ctas), dim3(kThreads), smem, st, p);
 }

@@ -55,12 +55,11 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
   grid_dependency_launch();
   grid_dependency_wait();
-  const int hk = blockIdx.x % p.hkv, rest = blockIdx.x / p.hkv;
-  const int part = p.parts > 1 ? rest % p.parts : 0, index = p.parts > 1 ? rest / p.parts : rest;
+  const int hk = blockIdx.x % p.hkv, index = blockIdx.x / p.hkv;
   PortionBlock block;
-  if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(smem + kOffSearch)) || part >= block.parts) return;
-  const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, block.parts);
-  const int nkv = block.tile0 + portion_part_begin(block.tiles, part + 1, block.parts) - tile0;
+  if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(smem + kOffSearch))) return;
+  const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
+  const int nkv = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts) - tile0;
   const int virtual_rows = block.rows * p.group, active_warps = (virtual_rows + 31) >> 5;
   const bool two_boxes = p.d > 64;
   const uint32_t tile_bytes = two_boxes ? kTileBytes : kTileBytes / 2;
@@ -140,9 +139,45 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const uint32_t idesc_pv = (1u << 4) | (1u << 16) | ((uint32_t)(d_steps * 2) << 17) | ((kM >> 4) << 24);
     const uint64_t dq = smem_desc(smem_u32(smem), 16, 1024), dk = smem_desc(smem_u32(smem + kOffK), 16, 1024);
     const uint64_t dv = smem_desc(smem_u32(smem + kOffV), kTileBytes / 2, 1024);
-    auto issue_s = [&](int j) -> bool {
-      const int s = j & 1, sk = j % kKStages;
-      if (!mbar_wait_warp(&full_k[sk], (j / kKStages) & 1, abort_flag, p.wait_ns)) return false;
+    // round i: P_{i-2}.V_{i-2}, then S_i in its place - S_0 S_1 (P.V_0 S_2) (P.V_1 S_3) ..., with one copy of each in the instruction cache
+    bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns);
+#pragma unroll 1
+    for (int i = 0; i < nkv + 2 && ok; ++i) {
+      const int s = i & 1;
+      if (i >= 2) {
+        const int j = i - 2, sv = j % kVStages;
+        ok = mbar_wait_warp(&full_v[sv], (j / kVStages) & 1, abort_flag, p.wait_ns);
+        if (!ok) break;
+        const int left = block.key_limit - (tile0 + j) * kN;  // keys of this tile that the sequence has
+        if (left < kN) {
+          uint4 *v = reinterpret_cast<uint4 *>(smem + kOffV + sv * kTileBytes);
+          for (int c = left * 8 + lane; c < kN * 8; c += 32) {
+            v[c] = make_uint4(0, 0, 0, 0);
+            if (two_boxes) v[c + kTileBytes / 32] = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        ok = mbar_wait_warp(&bar_p[s], (j >> 1) & 1, abort_flag, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dvs = dv + (uint64_t)(sv * (kTileBytes >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < kN / 16; ++ks)
+            umma_f16_ts(tmem_o, tmem + s * kN + ks * 8, dvs + (uint64_t)(ks * (2048 >> 4)), idesc_pv, j > 0 || ks > 0);
+          umma_commit(bar_o);
+          umma_commit(&empty_v[sv]);
+          if (j == nkv - 1) umma_commit(bar_fin);
+        }
+        if (i >= nkv) continue;
+        ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns);  // S_i takes the place of P_{i-2}
+        if (!ok) break;
+      }
+      if (i >= nkv) continue;
+      const int sk = i % kKStages;
+      ok = mbar_wait_warp(&full_k[sk], (i / kKStages) & 1, abort_flag, p.wait_ns);
+      if (!ok) break;
       tc_fence_after();
       const uint64_t dks = dk + (uint64_t)(sk * (kTileBytes >> 4));
       if (elect_one()) {
@@ -155,43 +190,13 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         umma_commit(&bar_s[s]);
         umma_commit(&empty_k[sk]);
       }
-      return true;
-    };
-    bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns) && issue_s(0);
-    if (ok && nkv > 1) ok = issue_s(1);
-    for (int j = 0; j < nkv && ok; ++j) {
-      const int sv = j % kVStages;
-      ok = mbar_wait_warp(&full_v[sv], (j / kVStages) & 1, abort_flag, p.wait_ns);
-      if (!ok) break;
-      const int left = block.key_limit - (tile0 + j) * kN;  // keys of this tile that the sequence has
-      if (left < kN) {
-        uint4 *v = reinterpret_cast<uint4 *>(smem + kOffV + sv * kTileBytes);
-        for (int i = left * 8 + lane; i < kN * 8; i += 32) {
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (two_boxes) v[i + kTileBytes / 32] = make_uint4(0, 0, 0, 0);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
-      ok = mbar_wait_warp(&bar_p[j & 1], (j >> 1) & 1, abort_flag, p.wait_ns);
-      if (!ok) break;
-      tc_fence_after();
-      const uint64_t dvs = dv + (uint64_t)(sv * (kTileBytes >> 4));
-      if (elect_one()) {
-#pragma unroll
-        for (int ks = 0; ks < kN / 16; ++ks)
-          umma_f16_ts(tmem_o, tmem + (j & 1) * kN + ks * 8, dvs + (uint64_t)(ks * (2048 >> 4)), idesc_pv, j > 0 || ks > 0);
-        umma_commit(bar_o);
-        umma_commit(&empty_v[sv]);
-        if (j == nkv - 1) umma_commit(bar_fin);
-      }
-      // S_{j+2} takes the place of P_j, so P_j.V_j is waited for
-      if (j + 2 < nkv) ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns) && issue_s(j + 2);
     }
   } else if (warp < active_warps) {
     const int token = threadIdx.x / p.group, head = hk * p.group + threadIdx.x % p.group;
     const bool there = token < block.rows;
-    const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0;
+    // Rows that are none (a group that does not divide 128, the last block of a sequence) are left unmasked: what they compute is stored
+    // nowhere and moves no maximum, and a mask for one row costs its warp 200 instructions with every tile (heads of 64, three to a KV head: 538 us and FILL).
+    const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0x7fffffff;
     const int key_begin = there && p.window ? max(0, pos + 1 - p.window) : 0;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     float m_run = -INFINITY, l_run = 0.f;
@@ -216,7 +221,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       // the running maximum moves only when some row of the warp has a score more than 2^kLazyLog2 above it; P and its sum hold that
       const float m_tile = row_max(sr) * p.scale_log2;
       float corr = 1.f;
-      const bool moved = __any_sync(0xffffffffu, m_tile > m_run + kLazyLog2);
+      const bool moved = __any_sync(0xffffffffu, there && m_tile > m_run + kLazyLog2);
       if (moved) {
         const float m_new = fmaxf(m_run, m_tile);
         corr = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
@@ -264,8 +269,8 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int row = block.row0 + token;
     const bool divided = block.parts > 1;
     const int key0 = max(key_begin, tile0 * kN), key1 = min(key_end, (tile0 + nkv) * kN);
-    const size_t place = divided ? portion_place(p, part, row, head) : 0;
-    if (ok && p.parts > 1 && part == 0 && there && head == 0) p.row_parts[row] = block.parts;
+    const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
+    if (ok && p.parts > 1 && block.part == 0 && there && head == 0) p.row_parts[row] = block.parts;
     if (ok && nkv == 0 && there) {  // no key at all
       uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d);
       for (int c = 0; c < p.d / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
@@ -309,7 +314,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const unsigned again = __ballot_sync(0xffffffffu, there && bad != 0.f);
       for (unsigned left = again; left; left &= left - 1) {
         const int r = warp * 32 + __ffs(left) - 1;
-        redo_portion_row<__half>(p, block, part, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
+        redo_portion_row<__half>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
       }
     }
   }
@@ -348,7 +353,7 @@ int portions_umma(const PortionParams &p, cudaStream_t st) {
       return AXB200_DEVICE_ERROR;
     opted[dev] = true;
   }
-  const int64_t ctas = (int64_t)p.blocks * p.hkv * p.parts;
+  const int64_t ctas = (int64_t)p.units * p.hkv;
   if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
   return launch_dependent(portion_umma_kernel, dim3((unsigned)ctas), dim3(kThreads), kSmem, st, mq, mk, mv, p);
 }

@@ -650,52 +650,58 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling=None, device=
     return freq.to(device), factor
 
 
-def _on_device(ref, op, *tensors):
+def _one_device(op, device, tensors):
     for t in tensors:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != device:
             raise RuntimeError(f"{op}: tensors on different devices")
 
 
-def _launch_on(t, call, *args):
-    """The call with t's device as the current one (a launch goes to the current device whatever its stream)."""
-    if t.device.index == torch.cuda.current_device():
-        return call(*args)
-    with torch.cuda.device(t.device):
-        return call(*args)
+def _launch_on(device, op, call, *args):
+    """The call on the device's current stream, with the device as the current one (a launch goes to the current device whatever its
+    stream).  torch.cuda.current_stream and current_device take 5 us of the 15 that a call of these operators has."""
+    global _launches
+    if device == torch._C._cuda_getDevice():
+        status = call(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        _capi.check(status, op)
+    _launches += 1
 
 
 def _rotation(op, d, inv_freq, pos, rows, mrope_section, pos_needed):
-    """(rot_dim, mrope, h, w, pos) of the operators below."""
+    """(pos, its address, inv_freq's address, rot_dim, mrope, h, w) of the operators below."""
     if inv_freq is None:
-        return 0, 0, 0, 0, None
-    if inv_freq.dtype != torch.float64:
+        return None, None, None, 0, 0, 0, 0
+    if inv_freq.dtype is not torch.float64:
         _capi.check(3, op)
-    if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= d or not inv_freq.is_contiguous():
+    pairs = inv_freq.numel()
+    if inv_freq.dim() != 1 or not 0 < 2 * pairs <= d or not inv_freq.is_contiguous():
         _capi.check(4, op)
-    mrope = mrope_section is not None
     if pos is None:
         if pos_needed:
             raise RuntimeError(f"{op}: a rotation needs positions")
-    elif pos.dtype != torch.int64:
+        return None, None, inv_freq.data_ptr(), 2 * pairs, 0, 0, 0
+    if pos.dtype is not torch.int64:
         _capi.check(3, op)
-    elif tuple(pos.shape) != ((3, rows) if mrope else (rows,)):
+    if pos.shape != ((rows,) if mrope_section is None else (3, rows)):
         _capi.check(4, op)
-    _, h, w = mrope_section if mrope and pos is not None else (0, 0, 0)
-    return 2 * inv_freq.numel(), int(mrope and pos is not None), int(h), int(w), None if pos is None else _c(pos)
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
+    if mrope_section is None:
+        return pos, pos.data_ptr(), inv_freq.data_ptr(), 2 * pairs, 0, 0, 0
+    _, h, w = mrope_section
+    return pos, pos.data_ptr(), inv_freq.data_ptr(), 2 * pairs, 1, h, w
 
 
-def _head_rows(x, op):
-    """x (rows, heads, d) as it is where each row is contiguous, else a contiguous copy; and its row stride."""
-    if x.dim() != 3:
+def _norm_weight(w, dtype, d, op):
+    """The address of a norm's weight."""
+    if w is None:
+        return None
+    if w.dtype is not dtype or w.shape != (d,) or not w.is_contiguous():
         _capi.check(4, op)
-    if not (x.stride(2) == 1 and x.stride(1) == x.shape[2] and x.stride(0) >= x.shape[1] * x.shape[2]) and not x.is_contiguous():
-        x = x.contiguous()
-    return x, x.stride(0) if x.shape[0] > 1 else x.shape[1] * x.shape[2]
-
-
-def _norm_weight(w, x, d, op):
-    if w is not None and (w.dtype != x.dtype or tuple(w.shape) != (d,) or not w.is_contiguous()):
-        _capi.check(4, op)
+    return w.data_ptr()
 
 
 def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False, factor: float = 1.0,
@@ -711,48 +717,56 @@ def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float =
         _capi.check(7, op)
     if not x.is_cuda:
         raise RuntimeError(f"{op}: expected CUDA tensors (this package has no CPU path)")
-    dt = _TURN_DTYPES.get(x.dtype)
+    dtype, device = x.dtype, x.get_device()
+    dt = _TURN_DTYPES.get(dtype)
     if dt is None:
         _capi.check(3, op)
-    rows, _, d = x.shape if x.dim() == 3 else _capi.check(4, op)
+    if x.dim() != 3:
+        _capi.check(4, op)
+    rows, _, d = x.shape
     args, outs = [], []
-    for t, w in ((q, q_weight), (k, k_weight)):
+    for t in (q, k):
         if t is None:
             args.append((None, 0, 0))
             outs.append(None)
             continue
-        t, ld = _head_rows(t, op)
-        if t.dtype != x.dtype:
+        if t.dtype is not dtype:
             _capi.check(3, op)
-        if t.shape[0] != rows or t.shape[2] != d:
+        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d:
             _capi.check(4, op)
-        _norm_weight(w, x, d, op)
-        args.append((t, ld, t.shape[1]))
-        outs.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
-    rot_dim, mrope, h, w, pos = _rotation(op, d, inv_freq, pos, rows, mrope_section, True)
-    _on_device(x, op, q, k, pos, inv_freq, q_weight, k_weight)
+        heads = t.shape[1]
+        ld, head_ld, element = t.stride()
+        if element != 1 or head_ld != d or ld < heads * d:  # rows that are not one run each
+            t = t.contiguous() if not t.is_contiguous() else t
+            ld = heads * d
+        args.append((t, ld, heads))
+        outs.append(torch.empty((rows, heads, d), dtype=dtype, device=x.device))
     (tq, q_ld, hq), (tk, k_ld, hkv) = args
-    _call(_launch_on(x, _capi.lib().axb200_qk_norm_rope, _ptr(tq), q_ld, _ptr(tk), k_ld, _ptr(q_weight), _ptr(k_weight), float(eps),
-                     _ptr(pos), _ptr(inv_freq), rot_dim, int(interleaved), float(factor), mrope, h, w, _ptr(outs[0]), _ptr(outs[1]),
-                     rows, hq, hkv, d, dt, _stream(x)), op)
-    return tuple(outs)
+    wq, wk = _norm_weight(q_weight, dtype, d, op), _norm_weight(k_weight, dtype, d, op)
+    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, True)
+    _one_device(op, device, (q, k, pos, inv_freq, q_weight, k_weight))
+    _launch_on(device, op, _capi.lib().axb200_qk_norm_rope, tq.data_ptr() if tq is not None else None, q_ld,
+               tk.data_ptr() if tk is not None else None, k_ld, wq, wk, eps, at, freq, rot_dim, bool(interleaved), factor, mrope, h, w,
+               outs[0].data_ptr() if tq is not None else None, outs[1].data_ptr() if tk is not None else None, rows, hq, hkv, d, dt)
+    return outs[0], outs[1]
 
 
-def _portion_tables(op, ref, k_pages, v_pages, block_table, seq_lens, row_start):
-    """batch of the operators below; everything that a kernel would follow blindly is checked here."""
+def _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start):
+    """The batch of the operators below, and the addresses of pages and tables, after what a kernel would follow blindly was checked."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or block_table.dim() != 2 or seq_lens.dim() != 1 or row_start.dim() != 1:
         _capi.check(4, op)
-    if k_pages.dtype != ref.dtype or v_pages.dtype != ref.dtype or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
-            or row_start.dtype != torch.int32:
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype or block_table.dtype is not torch.int32 or \
+            seq_lens.dtype is not torch.int32 or row_start.dtype is not torch.int32:
         _capi.check(3, op)
-    batch = row_start.numel() - 1
-    if batch < 1 or seq_lens.numel() < batch or block_table.shape[0] < batch:
+    batch = row_start.shape[0] - 1
+    if batch < 1 or seq_lens.shape[0] < batch or block_table.shape[0] < batch:
         _capi.check(4, op)
-    for t in (k_pages, v_pages, block_table, seq_lens, row_start):
+    tables = (k_pages, v_pages, block_table, seq_lens, row_start)
+    for t in tables:
         if not t.is_contiguous():
             raise RuntimeError(f"{op}: pages and tables must be contiguous")
-    _on_device(ref, op, k_pages, v_pages, block_table, seq_lens, row_start)
-    return batch
+    _one_device(op, device, tables)
+    return batch, [t.data_ptr() for t in tables]
 
 
 def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens, row_start,
@@ -764,26 +778,27 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
     the turned q (rows, hq, d); rows of no sequence are left as they are in `out`."""
     op = "qkv_norm_rope_append_portions"
     dt = _dt(qkv, op)
-    if qkv.dim() != 2 or (qkv.shape[1] > 1 and qkv.stride(1) != 1):
+    dtype, device = qkv.dtype, qkv.get_device()
+    if qkv.dim() != 2:
         _capi.check(4, op)
-    batch = _portion_tables(op, qkv, k_pages, v_pages, block_table, seq_lens, row_start)
+    batch, pages = _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start)
     num_pages, hkv, page_tokens, d = k_pages.shape
-    rows = qkv.shape[0]
-    ld = qkv.stride(0) if rows > 1 else qkv.shape[1]
-    if qkv.shape[1] != (n_q_heads + 2 * hkv) * d or ld < qkv.shape[1]:
+    rows, columns = qkv.shape
+    ld, element = qkv.stride()
+    if rows <= 1:
+        ld = columns
+    if columns != (n_q_heads + 2 * hkv) * d or ld < columns or (element != 1 and columns > 1):
         _capi.check(4, op)
-    for w in (q_norm_weight, k_norm_weight):
-        _norm_weight(w, qkv, d, op)
-    rot_dim, mrope, h, w, pos = _rotation(op, d, inv_freq, pos, rows, mrope_section, False)
+    wq, wk = _norm_weight(q_norm_weight, dtype, d, op), _norm_weight(k_norm_weight, dtype, d, op)
+    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, False)
     if out is None:
-        out = torch.empty((rows, n_q_heads, d), dtype=qkv.dtype, device=qkv.device)
-    elif tuple(out.shape) != (rows, n_q_heads, d) or out.dtype != qkv.dtype or not out.is_contiguous():
+        out = torch.empty((rows, n_q_heads, d), dtype=dtype, device=qkv.device)
+    elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous():
         _capi.check(4, op)
-    _on_device(qkv, op, pos, inv_freq, q_norm_weight, k_norm_weight, out)
-    _call(_launch_on(qkv, _capi.lib().axb200_qkv_norm_rope_append_portions, qkv.data_ptr(), ld, _ptr(q_norm_weight), _ptr(k_norm_weight),
-                     float(eps), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-                     row_start.data_ptr(), _ptr(pos), _ptr(inv_freq), rot_dim, int(interleaved), float(factor), mrope, h, w, rows, batch,
-                     n_q_heads, hkv, d, page_tokens, block_table.shape[1], num_pages, dt, int(advance), _stream(qkv)), op)
+    _one_device(op, device, (pos, inv_freq, q_norm_weight, k_norm_weight, out))
+    _launch_on(device, op, _capi.lib().axb200_qkv_norm_rope_append_portions, qkv.data_ptr(), ld, wq, wk, eps, out.data_ptr(), *pages, at,
+               freq, rot_dim, bool(interleaved), factor, mrope, h, w, rows, batch, n_q_heads, hkv, d, page_tokens, block_table.shape[1],
+               num_pages, dt, bool(advance))
     return out
 
 
@@ -796,24 +811,23 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
     dt = _dt(q, op)
     if q.dim() != 3:
         _capi.check(4, op)
-    batch = _portion_tables(op, q, k_pages, v_pages, block_table, seq_lens, row_start)
+    dtype, device = q.dtype, q.get_device()
+    batch, pages = _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start)
     rows, hq, d = q.shape
     num_pages, hkv, page_tokens, dk = k_pages.shape
     if dk != d or hkv == 0 or hq % hkv:
         _capi.check(4, op)
-    q = _c(q)
+    if not q.is_contiguous():
+        q = q.contiguous()
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+    elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
-    _on_device(q, op, out)
-    lib = _capi.lib()
-    sizes = (hq, hkv, d, page_tokens, block_table.shape[1])
-    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, *sizes, int(max_seq_len), int(window), dt)
+    lib, blocks = _capi.lib(), block_table.shape[1]
+    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, max_seq_len, window, dt)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone: streams may overlap
-    _call(_launch_on(q, lib.axb200_gqa_attention_portions_paged, q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                     block_table.data_ptr(), seq_lens.data_ptr(), row_start.data_ptr(), rows, batch, *sizes, num_pages, int(max_seq_len),
-                     int(window), dt, _ptr(ws), need, _stream(q)), op)
+    _launch_on(device, op, lib.axb200_gqa_attention_portions_paged, q.data_ptr(), out.data_ptr(), *pages, rows, batch, hq, hkv, d,
+               page_tokens, blocks, num_pages, max_seq_len, window, dt, ws.data_ptr() if need else None, need)
     return out
 
 
