@@ -7,10 +7,9 @@
 //   warps 4-11  make the operands and add up: they split tiles of K and V, which TMA brings as floats, into parts in shared memory, and
 //               take the finished tiles of O (thread = virtual row and half of the columns)
 //   warp 12     issues the products: parts of Q and P in tensor memory are operand A
-//   warp 13     the copies, four tiles ahead
+//   warp 13     the copies
 // Splitting in the kernel needs no scratch for a cache whose lengths the host does not know, and hides behind the products: a tile's
-// scores take 2400 cycles and its sums 1600, and while the one runs the operand of the other is made, so that one buffer for K's parts
-// and one for V's do.
+// scores take 2400 cycles and its sums 1600.  K's parts have two buffers, V's one: V is split while the next scores are formed.
 //
 // Values that have no exact parts (infinities, NaN, values that round to infinity in bf16, below 2^-100) are noticed while splitting,
 // and the CTA does its rows over with plain multiplications (redo_portion_row).
@@ -25,13 +24,13 @@ namespace axb {
 namespace {
 
 constexpr int kM = 128, kN = kPortionKeys, kBox = kN * 64 * 2;
-constexpr int kHelpers = 8, kMmaWarp = 12, kLoadWarp = 13, kThreads = 448, kRaw = 4, kPageRing = 64;
+constexpr int kHelpers = 8, kMmaWarp = 12, kLoadWarp = 13, kThreads = 448, kRaw = 2, kKBufs = 2, kPageRing = 64;
 
 // kB: 64-wide blocks of the head size
 template <int kB>
 struct Layout {
   static constexpr int kRawTile = kN * 64 * kB * 4, kPart = kB * kBox, kTile = 3 * kPart;
-  static constexpr int kOffK = kRaw * kRawTile, kOffV = kOffK + kTile, kOffCorr = kOffV + kTile, kOffL = kOffCorr + 2 * kM * 4;
+  static constexpr int kOffK = kRaw * kRawTile, kOffV = kOffK + kKBufs * kTile, kOffCorr = kOffV + kTile, kOffL = kOffCorr + 2 * kM * 4;
   static constexpr int kOffBar = kOffL + 2 * kM * 4, kOffPages = kOffBar + 256;
   static constexpr int kSmem = kOffPages + kPageRing * 4;
   static constexpr int kQCols = 96 * kB, kSpCols = 96, kColO = kQCols + 2 * kSpCols;
@@ -39,23 +38,29 @@ struct Layout {
 static_assert(Layout<2>::kSmem <= 232448, "shared memory of a CTA");
 static_assert(sizeof(PortionSearch) <= 2 * kM * 4, "the search is over before rescale factors stand in its place");
 
-// Three bf16 parts of each of two floats; their sum is exact.
-__device__ __forceinline__ void split3(float a, float b, uint32_t &h, uint32_t &m, uint32_t &l) {
+// Three bf16 parts of each of two floats; their sum is exact.  Infinities, NaN and what rounds to infinity make `check` NaN.
+__device__ __forceinline__ void split3(float a, float b, uint32_t &h, uint32_t &m, uint32_t &l, uint64_t &check) {
+  const uint64_t minus = pack_f32x2(-1.f, -1.f), zero = pack_f32x2(0.f, 0.f);
   h = pack_bf16x2(a, b);
-  const float ra = a - __uint_as_float(h << 16), rb = b - __uint_as_float(h & 0xffff0000u);
-  m = pack_bf16x2(ra, rb);
-  l = pack_bf16x2(ra - __uint_as_float(m << 16), rb - __uint_as_float(m & 0xffff0000u));
+  const uint64_t h2 = pack_f32x2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+  check = fma_f32x2(h2, zero, check);
+  const uint64_t r = fma_f32x2(h2, minus, pack_f32x2(a, b));
+  m = pack_bf16x2(unpack_f32x2(r).x, unpack_f32x2(r).y);
+  const uint64_t m2 = pack_f32x2(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  const float2 s = unpack_f32x2(fma_f32x2(m2, minus, r));
+  l = pack_bf16x2(s.x, s.y);
 }
 
-// Largest and smallest (zero aside) magnitude seen, as bits.
+// What has no three parts among the values seen: not finite ones by `check` above, and by the smallest magnitude, zero aside, those
+// below 2^-100.
 struct Range {
-  uint32_t most = 0, least = 0xffffffffu;
-  __device__ __forceinline__ void see(float x) {
-    const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-    most = max(most, u);
-    least = min(least, u - 1u);
+  uint64_t check = 0;
+  uint32_t least = 0xffffffffu;  // of twice the bits of a magnitude, less one
+  __device__ __forceinline__ void see(float x) { least = __viaddmin_u32(__float_as_uint(x) << 1, 0xffffffffu, least); }
+  __device__ __forceinline__ bool unsplittable() const {
+    const float2 c = unpack_f32x2(check);
+    return !(c.x == 0.f && c.y == 0.f) || least < (27u << 24) - 1u;
   }
-  __device__ __forceinline__ bool unsplittable() const { return most >= 0x7f7f8000u || least < (27u << 23) - 1u; }
 };
 
 // The order in which tiles are used, and copied: K_0 K_1 V_0, then K_{j+2} V_{j+1}.
@@ -71,17 +76,16 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   using L = Layout<kB>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kOffBar);
-  uint64_t *raw_full = bars, *raw_empty = bars + 4;    // per stage of floats
-  uint64_t *full_k = bars + 8, *full_v = bars + 9;     // parts written; one arrival per helper warp
-  uint64_t *empty_k = bars + 10;                       // S that read K's parts done
-  uint64_t *bar_s = bars + 11;                         // S_j ready, per buffer
-  uint64_t *bar_o = bars + 13;                         // P_j . V_j done
-  uint64_t *bar_p = bars + 14;                         // P_j and its rescale factor written, per buffer
-  uint64_t *bar_c = bars + 16;                         // O_j added up, per parity of j
-  uint64_t *bar_q = bars + 18, *bar_l = bars + 19;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 20);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 21);
-  volatile int *bad_flag = reinterpret_cast<volatile int *>(bars + 22);
+  uint64_t *raw_full = bars, *raw_empty = bars + 2;    // per stage of floats
+  uint64_t *full_k = bars + 4, *full_v = bars + 6;     // parts written (K: per buffer); one arrival per helper warp
+  uint64_t *bar_s = bars + 7;                          // S_j ready, and the buffer of K_j free: per parity of j
+  uint64_t *bar_o = bars + 9;                          // P_j . V_j done
+  uint64_t *bar_p = bars + 10;                         // P_j and its rescale factor written, per parity
+  uint64_t *bar_c = bars + 12;                         // O_j added up, per parity
+  uint64_t *bar_q = bars + 14, *bar_l = bars + 15;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 17);
+  volatile int *bad_flag = reinterpret_cast<volatile int *>(bars + 18);
   int *pages = reinterpret_cast<int *>(smem + L::kOffPages);
   float *corr_s = reinterpret_cast<float *>(smem + L::kOffCorr), *l_s = reinterpret_cast<float *>(smem + L::kOffL);
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -104,9 +108,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRaw; ++i) mbar_init(&raw_full[i], 1), mbar_init(&raw_empty[i], kHelpers);
-    mbar_init(full_k, kHelpers);
+    for (int i = 0; i < kKBufs; ++i) mbar_init(&full_k[i], kHelpers);
     mbar_init(full_v, kHelpers);
-    mbar_init(empty_k, 1);
     mbar_init(bar_o, 1);
     for (int i = 0; i < 2; ++i) mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], active), mbar_init(&bar_c[i], 2 * active);
     mbar_init(bar_q, 2 * active);
@@ -194,9 +197,10 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         if (!ok) break;
       }
       if (i >= nkv) continue;
-      ok = mbar_wait_warp(full_k, i & 1, abort_flag, p.wait_ns);
+      ok = mbar_wait_warp(&full_k[s], (i >> 1) & 1, abort_flag, p.wait_ns);
       if (!ok) break;
       tc_fence_after();
+      const uint64_t dks = dk + (uint64_t)(s * (L::kTile >> 4));
       if (elect_one()) {
 #pragma unroll
         for (int c = 0; c < 6; ++c)
@@ -204,10 +208,9 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           for (int ks = 0; ks < 4 * kB; ++ks) {
             if (ks >= d_steps) break;
             umma_f16_ts(tmem_sp + s * L::kSpCols, tmem + kA[c] * 32 * kB + ks * 8,
-                        dk + (uint64_t)((kC[c] * L::kPart + (ks >> 2) * kBox + (ks & 3) * 32) >> 4), idesc_qk, c > 0 || ks > 0);
+                        dks + (uint64_t)((kC[c] * L::kPart + (ks >> 2) * kBox + (ks & 3) * 32) >> 4), idesc_qk, c > 0 || ks > 0);
           }
         umma_commit(&bar_s[s]);
-        umma_commit(empty_k);
       }
     }
   } else if (warp < 4) {
@@ -237,7 +240,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const float corr = fast_exp2((m_run - m_safe) * p.scale_log2);  // 0 at the first tile
         m_run = m_new;
         const uint64_t shift2 = pack_f32x2(-m_safe, -m_safe);
-        uint64_t sum2[4] = {0, 0, 0, 0};
+        uint64_t sum2[4] = {0, 0, 0, 0}, unused = 0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t parts[3][16];
@@ -247,7 +250,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             const float2 x = unpack_f32x2(mul_f32x2(x2, scale2));
             const float a = fast_exp2(x.x), b = fast_exp2(x.y);
             sum2[(i >> 1) & 3] = add_f32x2(sum2[(i >> 1) & 3], pack_f32x2(a, b));
-            split3(a, b, parts[0][i >> 1], parts[1][i >> 1], parts[2][i >> 1]);
+            split3(a, b, parts[0][i >> 1], parts[1][i >> 1], parts[2][i >> 1], unused);
           }
 #pragma unroll
           for (int i = 0; i < 3; ++i) tmem_st16(sp + i * 32 + c * 16, parts[i]);
@@ -284,8 +287,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (there && half * 32 * kB + c * 32 + u * 4 < p.d) x = *reinterpret_cast<const float4 *>(src + c * 32 + u * 4);
           range.see(x.x), range.see(x.y), range.see(x.z), range.see(x.w);
-          split3(x.x, x.y, parts[0][2 * u], parts[1][2 * u], parts[2][2 * u]);
-          split3(x.z, x.w, parts[0][2 * u + 1], parts[1][2 * u + 1], parts[2][2 * u + 1]);
+          split3(x.x, x.y, parts[0][2 * u], parts[1][2 * u], parts[2][2 * u], range.check);
+          split3(x.z, x.w, parts[0][2 * u + 1], parts[1][2 * u + 1], parts[2][2 * u + 1], range.check);
         }
 #pragma unroll
         for (int i = 0; i < 3; ++i) tmem_st16(tmem + lane_base + i * 32 * kB + half * 16 * kB + c * 16, parts[i]);
@@ -307,7 +310,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const bool is_k = at.next_is_k(nkv);
       const int j = is_k ? at.k++ : at.v++;
       if (is_k) {
-        if (j > 0) ok = mbar_wait_warp(empty_k, (j - 1) & 1, abort_flag, p.wait_ns);
+        if (j >= kKBufs) ok = mbar_wait_warp(&bar_s[j & 1], ((j - 2) >> 1) & 1, abort_flag, p.wait_ns);
       } else if (j > 0) {
         const int s = (j - 1) & 1;
         if (mine) ok = mbar_wait_warp(&bar_p[s], ((j - 1) >> 1) & 1, abort_flag, p.wait_ns);
@@ -338,18 +341,23 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       ok = mbar_wait_warp(&raw_full[s], (n / kRaw) & 1, abort_flag, p.wait_ns);
       if (!ok) break;
       const int left = block.key_limit - (tile0 + j) * kN;  // keys that the sequence has; behind them anything may stand
-      const float4 *src = reinterpret_cast<const float4 *>(smem + s * L::kRawTile);
-      uint8_t *parts_at = smem + (is_k ? L::kOffK : L::kOffV);
-#pragma unroll 2
+      const bool whole = left >= kN;
+      const float4 *src = reinterpret_cast<const float4 *>(smem + s * L::kRawTile) + helper * 128 * kB + lane;
+      uint8_t *parts_at = smem + (is_k ? L::kOffK + (j & 1) * L::kTile : L::kOffV);
+      // a warp's rows of the tile are helper * 8 .. + 7, whose places in the swizzle are 0 .. 7
+      const int c = lane % (16 * kB), row0 = kB == 1 ? lane >> 4 : 0;
+      uint8_t *dst0 = parts_at + (c >> 4) * kBox + (helper * 8 + row0) * 128 + (c & 1) * 8;
+      const int chunk = (c & 15) >> 1;
+#pragma unroll 4
       for (int i = 0; i < 4 * kB; ++i) {
-        const int id = (helper * 4 * kB + i) * 32 + lane, key = id / (16 * kB), c = id % (16 * kB);
-        float4 x = src[id];
-        if (key >= left) x = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int r = i * (2 / kB);  // row0 + r is the row among the warp's eight
+        float4 x = src[i * 32];
+        if (!whole && helper * 8 + row0 + r >= left) x = make_float4(0.f, 0.f, 0.f, 0.f);
         range.see(x.x), range.see(x.y), range.see(x.z), range.see(x.w);
         uint2 h, m, l;
-        split3(x.x, x.y, h.x, m.x, l.x);
-        split3(x.z, x.w, h.y, m.y, l.y);
-        uint8_t *dst = parts_at + (c >> 4) * kBox + key * 128 + ((((c & 15) >> 1) ^ (key & 7)) << 4) + (c & 1) * 8;
+        split3(x.x, x.y, h.x, m.x, l.x, range.check);
+        split3(x.z, x.w, h.y, m.y, l.y, range.check);
+        uint8_t *dst = dst0 + r * 128 + ((chunk ^ (row0 + r)) << 4);
         *reinterpret_cast<uint2 *>(dst) = h;
         *reinterpret_cast<uint2 *>(dst + L::kPart) = m;
         *reinterpret_cast<uint2 *>(dst + 2 * L::kPart) = l;
@@ -358,7 +366,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&raw_empty[s]);
-        mbar_arrive(is_k ? full_k : full_v);
+        mbar_arrive(is_k ? &full_k[j & 1] : full_v);
       }
       ++n;
     }
