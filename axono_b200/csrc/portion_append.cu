@@ -10,6 +10,8 @@
 // before the first and behind the last sequence are left alone, in the outputs too.
 #include <math.h>
 
+#include <mutex>
+
 #include "tcgen05.cuh"
 #include "vec.cuh"
 
@@ -17,7 +19,8 @@ namespace axb {
 namespace {
 
 constexpr int kMaxPairs = 128;  // head sizes up to 256
-constexpr int kThreads = 256, kRowThreads = 128, kRowBlocks = 6, kStages = 4;
+constexpr int kThreads = 256, kRowThreads = 128, kRowBlocks = 6, kRowStages = 4, kSoloThreads = 512, kSoloStages = 5;
+constexpr int kSoloGroups = 64;  // groups of heads that one block takes at most, four per warp
 
 struct TurnParams {
   const void *q, *k;  // rows of q_ld and k_ld elements; v stands behind k in the form with a cache
@@ -119,6 +122,23 @@ struct Heads {
   __device__ __forceinline__ const T *weight(int h) const { return static_cast<const T *>(h < p.hq ? p.q_w : p.k_w); }
 };
 
+// A sequence's length with its portion added, found by a warp; -1 where it stays: nothing new, no room, or a page outside the pool.
+__device__ __forceinline__ int advanced_length(const TurnParams &p, int b) {
+  const int lane = threadIdx.x & 31, r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
+  if (r0 < 0 || r1 < r0 || r1 > p.rows) {
+    if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
+    return -1;
+  }
+  const int64_t first = first_slot(p, len, r1 - r0);
+  if (r1 == r0 || first < 0) return -1;
+  bool ok = true;
+  for (int64_t i = first / p.page_tokens + lane; i <= (first + r1 - r0 - 1) / p.page_tokens; i += 32) {
+    const int page = p.block_table[(int64_t)b * p.max_blocks + i];
+    ok = ok && page >= 0 && page < p.num_pages;
+  }
+  return __all_sync(0xffffffffu, ok) ? len + (r1 - r0) : -1;
+}
+
 __device__ __forceinline__ void copy_async16(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)) : "memory");
 }
@@ -156,13 +176,16 @@ __device__ __forceinline__ uint4 pack16(const float (&x)[8], const __nv_bfloat16
 // shared memory; the norm's sum goes over a head's threads by shuffles.  Each thread copies its own vectors into its own places of
 // shared memory, kStages groups ahead and beyond the end of a row, so that loads are under way whatever the warp waits for; no
 // barrier is wider than a warp.  kFull: every thread has both vectors (head sizes of 2 * kLanes vectors).
-template <typename T, bool kAppend, bool kInterleaved, int kLanes, bool kFull>
-__global__ void __launch_bounds__(kRowThreads, kRowBlocks)
-turn_rows_kernel(const TurnParams p, int ways) {
+// kSolo: one block does it all and, behind a barrier, advances the lengths (p.advance).
+template <typename T, bool kAppend, bool kInterleaved, int kLanes, bool kFull, bool kSolo>
+__global__ void __launch_bounds__(kSolo ? kSoloThreads : kRowThreads, kSolo ? 1 : kRowBlocks)
+turn_rows_kernel(const TurnParams p, int ways, int32_t *seq_lens) {
   constexpr int kVec = 16 / (int)sizeof(T), kAtOnce = 32 / kLanes;
   constexpr const T *kType = nullptr;
-  __shared__ __align__(16) float s_cos[kRowThreads / 32][kMaxPairs], s_sin[kRowThreads / 32][kMaxPairs];
-  __shared__ __align__(16) uint4 s_raw[kRowThreads / 32][kStages][2][32];
+  constexpr int kWarps = (kSolo ? kSoloThreads : kRowThreads) / 32, kStages = kSolo ? kSoloStages : kRowStages;
+  __shared__ __align__(16) float s_cos[kWarps][kMaxPairs], s_sin[kWarps][kMaxPairs];
+  extern __shared__ __align__(16) uint8_t s_dynamic[];
+  uint4(*s_raw)[kStages][2][32] = reinterpret_cast<uint4(*)[kStages][2][32]>(s_dynamic);  // per warp
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & (kLanes - 1), group = lane / kLanes;
   const int vectors = p.d / kVec, turned = p.pairs / kVec;  // halves: vectors that have a partner `turned` further on
   // this thread's two vectors of every head, whether it has them, and whether they are turned: together in halves, each by itself
@@ -174,8 +197,8 @@ turn_rows_kernel(const TurnParams p, int ways) {
   const float over_d = 1.0f / (float)p.d;
   const unsigned mates = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1) << (group * kLanes);  // the threads of this head
   const int rotated = p.hq + p.hkv, n_heads = rotated + (kAppend ? p.hkv : 0), share = (n_heads + ways - 1) / ways;
-  const int64_t tasks = p.rows * ways, step = (int64_t)gridDim.x * (kRowThreads / 32);
-  const int64_t first_task = (int64_t)blockIdx.x * (kRowThreads / 32) + warp;
+  const int64_t tasks = p.rows * ways, step = (int64_t)gridDim.x * (blockDim.x >> 5);
+  const int64_t first_task = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
 
   // Heads of a row stand behind one another from two bases, the queries' and - moved back by the queries - the keys'.
   grid_dependency_launch();
@@ -211,6 +234,8 @@ turn_rows_kernel(const TurnParams p, int ways) {
   };
 #pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) fetch();
+  int advanced = -1;
+  if (kSolo && warp < p.batch) advanced = advanced_length(p, warp);
 
   int stage = 0;
   for (int64_t task = first_task; task < tasks; task += step) {
@@ -316,6 +341,13 @@ turn_rows_kernel(const TurnParams p, int ways) {
       if (has_b) dst[vb] = pack16(x[1], kType);
     }
   }
+  if constexpr (kSolo) {
+    __syncthreads();  // every warp has read the lengths
+    for (int b = warp; b < p.batch; b += blockDim.x >> 5) {
+      if (b != warp) advanced = advanced_length(p, b);
+      if (lane == 0 && advanced >= 0) seq_lens[b] = advanced;
+    }
+  }
 }
 
 // Any head size up to 256, any alignment: a block per row, a warp per head, the normed head in shared memory.
@@ -370,60 +402,79 @@ turn_row_any_kernel(const TurnParams p) {
   }
 }
 
-// The lengths after a step's first append: a kernel of its own, since any block of the append may still read them.  A sequence whose
-// portion does not fit, or has a page outside the pool, keeps its length.  One warp per sequence.
+// The lengths after a step's first append, as a kernel of its own: any block of the append may still read them.
 __global__ void __launch_bounds__(kThreads)
 advance_lengths_kernel(const TurnParams p, int32_t *seq_lens) {
-  const int b = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int b = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   grid_dependency_launch();
   grid_dependency_wait();
   if (b >= p.batch) return;
-  const int r0 = p.row_start[b], r1 = p.row_start[b + 1];
-  if (r0 < 0 || r1 < r0 || r1 > p.rows) {
-    if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
-    return;
-  }
-  const int len = seq_lens[b];
-  const int64_t first = first_slot(p, len, r1 - r0);
-  if (r1 == r0 || first < 0) return;
-  bool ok = true;
-  for (int64_t i = first / p.page_tokens + lane; i <= (first + r1 - r0 - 1) / p.page_tokens; i += 32) {
-    const int page = p.block_table[(int64_t)b * p.max_blocks + i];
-    ok = ok && page >= 0 && page < p.num_pages;
-  }
-  if (__all_sync(0xffffffffu, ok) && lane == 0) seq_lens[b] = len + (r1 - r0);
+  const int advanced = advanced_length(p, b);
+  if ((threadIdx.x & 31) == 0 && advanced >= 0) seq_lens[b] = advanced;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename T, bool kAppend, int kLanes>
-int launch_rows(const TurnParams &p, cudaStream_t st) {
-  constexpr int kVec = 16 / (int)sizeof(T), kAtOnce = 32 / kLanes;
-  const int n_heads = p.hq + (kAppend ? 2 : 1) * p.hkv;
-  int ways = 1;
-  while (p.rows * ways < 148 * 8 && ways * 2 * kAtOnce <= n_heads) ways *= 2;
-  const int64_t blocks = (p.rows * ways + kRowThreads / 32 - 1) / (kRowThreads / 32), most = 148 * kRowBlocks;
+template <typename T, bool kAppend, int kLanes, bool kSolo>
+int launch_rows(const TurnParams &p, int ways, int blocks, int warps, int32_t *seq_lens, cudaStream_t st) {
+  constexpr int kVec = 16 / (int)sizeof(T);
   const bool full = p.d == 2 * kLanes * kVec;
-  auto *kernel = p.interleaved ? full ? turn_rows_kernel<T, kAppend, true, kLanes, true> : turn_rows_kernel<T, kAppend, true, kLanes, false>
-                 : full        ? turn_rows_kernel<T, kAppend, false, kLanes, true>
-                               : turn_rows_kernel<T, kAppend, false, kLanes, false>;
-  return launch_dependent(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kRowThreads), 0, st, p, ways);
+  using Kernel = void (*)(const TurnParams, int, int32_t *);
+  static const Kernel kernels[4] = {
+      turn_rows_kernel<T, kAppend, false, kLanes, false, kSolo>, turn_rows_kernel<T, kAppend, false, kLanes, true, kSolo>,
+      turn_rows_kernel<T, kAppend, true, kLanes, false, kSolo>, turn_rows_kernel<T, kAppend, true, kLanes, true, kSolo>};
+  if constexpr (kSolo) {
+    static std::mutex mu;
+    static bool opted[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return AXB200_DEVICE_ERROR;
+    std::lock_guard<std::mutex> lock(mu);
+    for (int k = 0; k < 4 && !opted[dev]; ++k)
+      if (cudaFuncSetAttribute(kernels[k], cudaFuncAttributeMaxDynamicSharedMemorySize, kSoloThreads / 32 * kSoloStages * 1024) != cudaSuccess)
+        return AXB200_DEVICE_ERROR;
+    opted[dev] = true;
+  }
+  const size_t smem = (size_t)warps * (kSolo ? kSoloStages : kRowStages) * 2 * 32 * sizeof(uint4);
+  return launch_dependent(kernels[2 * p.interleaved + full], dim3((unsigned)blocks), dim3(warps * 32), smem, st, p, ways, seq_lens);
 }
 
+// Few rows are shared among warps, down to a group of heads each.  `done`: the lengths are advanced too.
+template <typename T, bool kAppend, int kLanes>
+int launch_lanes(const TurnParams &p, int32_t *seq_lens, bool &done, cudaStream_t st) {
+  constexpr int kAtOnce = 32 / kLanes, kSoloWarps = kSoloThreads / 32;
+  const int n_heads = p.hq + (kAppend ? 2 : 1) * p.hkv, groups = (n_heads + kAtOnce - 1) / kAtOnce;
+  int ways = 1;
+  if constexpr (kAppend) {
+    if (seq_lens && p.rows * groups <= kSoloGroups && p.batch <= kSoloGroups) {
+      while (p.rows * ways * 2 <= kSoloWarps && ways * 2 <= groups) ways *= 2;
+      const int64_t tasks = p.rows * ways;
+      done = true;
+      return launch_rows<T, kAppend, kLanes, true>(p, ways, 1, (int)(tasks < kSoloWarps ? tasks : kSoloWarps), seq_lens, st);
+    }
+  }
+  while (p.rows * ways < 148 * 8 && ways * 2 <= groups) ways *= 2;
+  const int64_t blocks = (p.rows * ways + kRowThreads / 32 - 1) / (kRowThreads / 32), most = 148 * kRowBlocks;
+  return launch_rows<T, kAppend, kLanes, false>(p, ways, (int)(blocks < most ? blocks : most), kRowThreads / 32, nullptr, st);
+}
+
+// seq_lens: the lengths to be advanced, or null.
 template <typename T, bool kAppend>
-int launch_turn(const TurnParams &p, cudaStream_t st) {
+int launch_turn(const TurnParams &p, int32_t *seq_lens, cudaStream_t st) {
   constexpr int kVec = 16 / (int)sizeof(T);
   const bool whole = p.d % kVec == 0 && (p.interleaved ? 2 * p.pairs : p.pairs) % kVec == 0 && p.q_ld % kVec == 0 && p.k_ld % kVec == 0;
   const bool aligned = aligned16(p.q) && aligned16(p.k) && aligned16(p.q_out) && aligned16(p.k_out) && aligned16(p.k_pages) &&
                        aligned16(p.v_pages) && aligned16(p.q_w) && aligned16(p.k_w);
-  if (!whole || !aligned)
-    return launch_dependent(turn_row_any_kernel<T, kAppend>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p);
   const int vectors = p.d / kVec;
-  if (vectors <= 4 || vectors > 64) return launch_dependent(turn_row_any_kernel<T, kAppend>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p);
-  return vectors <= 8    ? launch_rows<T, kAppend, 4>(p, st)
-         : vectors <= 16 ? launch_rows<T, kAppend, 8>(p, st)
-         : vectors <= 32 ? launch_rows<T, kAppend, 16>(p, st)
-                         : launch_rows<T, kAppend, 32>(p, st);
+  bool done = false;
+  const int rc = !whole || !aligned || vectors <= 4 || vectors > 64
+                     ? launch_dependent(turn_row_any_kernel<T, kAppend>, dim3((unsigned)p.rows), dim3(kThreads), 0, st, p)
+                 : vectors <= 8  ? launch_lanes<T, kAppend, 4>(p, seq_lens, done, st)
+                 : vectors <= 16 ? launch_lanes<T, kAppend, 8>(p, seq_lens, done, st)
+                 : vectors <= 32 ? launch_lanes<T, kAppend, 16>(p, seq_lens, done, st)
+                                 : launch_lanes<T, kAppend, 32>(p, seq_lens, done, st);
+  if (rc != AXB200_OK || !seq_lens || done) return rc;
+  const unsigned blocks = (unsigned)((p.batch + kThreads / 32 - 1) / (kThreads / 32));
+  return launch_dependent(advance_lengths_kernel, dim3(blocks), dim3(kThreads), 0, st, p, seq_lens);
 }
 
 bool turn_sizes_ok(const TurnParams &p) {
@@ -447,9 +498,9 @@ int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld
   if ((hq > 0 && (!q || !q_out)) || (hkv > 0 && (!k || !k_out)) || (rot_dim > 0 && (!pos || !inv_freq))) return AXB200_INVALID_PTR;
   if ((hq > 0 && q_ld < (int64_t)hq * d) || (hkv > 0 && k_ld < (int64_t)hkv * d)) return AXB200_SHAPE_MISMATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, false>(p, st)
-         : dtype == AXB200_FLOAT16 ? axb::launch_turn<__half, false>(p, st)
-                                   : axb::launch_turn<__nv_bfloat16, false>(p, st);
+  return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, false>(p, nullptr, st)
+         : dtype == AXB200_FLOAT16 ? axb::launch_turn<__half, false>(p, nullptr, st)
+                                   : axb::launch_turn<__nv_bfloat16, false>(p, nullptr, st);
 }
 
 int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
@@ -472,10 +523,8 @@ int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void
     return AXB200_INVALID_PTR;
   if (ld < (int64_t)(hq + 2 * hkv) * d) return AXB200_SHAPE_MISMATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = dtype == AXB200_FLOAT32 ? axb::launch_turn<float, true>(p, st) : axb::launch_turn<__half, true>(p, st);
-  if (rc != AXB200_OK || !advance) return rc;
-  const unsigned blocks = (unsigned)((batch + axb::kThreads / 32 - 1) / (axb::kThreads / 32));
-  return axb::launch_dependent(axb::advance_lengths_kernel, dim3(blocks), dim3(axb::kThreads), 0, st, p, seq_lens);
+  int32_t *advanced = advance ? seq_lens : nullptr;
+  return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, true>(p, advanced, st) : axb::launch_turn<__half, true>(p, advanced, st);
 }
 
 }  // extern "C"

@@ -740,7 +740,7 @@ def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float =
             t = t.contiguous() if not t.is_contiguous() else t
             ld = heads * d
         args.append((t, ld, heads))
-        outs.append(torch.empty((rows, heads, d), dtype=dtype, device=x.device))
+        outs.append(torch.empty_like(t))  # rows apart or not, the copy is contiguous
     (tq, q_ld, hq), (tk, k_ld, hkv) = args
     wq, wk = _norm_weight(q_weight, dtype, d, op), _norm_weight(k_weight, dtype, d, op)
     pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, True)
@@ -792,7 +792,7 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
     wq, wk = _norm_weight(q_norm_weight, dtype, d, op), _norm_weight(k_norm_weight, dtype, d, op)
     pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, False)
     if out is None:
-        out = torch.empty((rows, n_q_heads, d), dtype=dtype, device=qkv.device)
+        out = qkv.new_empty((rows, n_q_heads, d))
     elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous():
         _capi.check(4, op)
     _one_device(op, device, (pos, inv_freq, q_norm_weight, k_norm_weight, out))
@@ -825,7 +825,7 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
         _capi.check(4, op)
     lib, blocks = _capi.lib(), block_table.shape[1]
     need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, max_seq_len, window, dt)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # of this call alone: streams may overlap
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None  # of this call alone: streams may overlap
     _launch_on(device, op, lib.axb200_gqa_attention_portions_paged, q.data_ptr(), out.data_ptr(), *pages, rows, batch, hq, hkv, d,
                page_tokens, blocks, num_pages, max_seq_len, window, dt, ws.data_ptr() if need else None, need)
     return out
