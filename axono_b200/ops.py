@@ -650,10 +650,8 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling=None, device=
     return freq.to(device), factor
 
 
-def _one_device(op, device, tensors):
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise RuntimeError(f"{op}: tensors on different devices")
+def _elsewhere(op):
+    raise RuntimeError(f"{op}: tensors on different devices")
 
 
 def _launch_on(device, op, call, *args):
@@ -670,38 +668,58 @@ def _launch_on(device, op, call, *args):
     _launches += 1
 
 
-def _rotation(op, d, inv_freq, pos, rows, mrope_section, pos_needed):
+def _rotation(op, x, d, inv_freq, pos, rows, mrope_section, pos_needed):
     """(pos, its address, inv_freq's address, rot_dim, mrope, h, w) of the operators below."""
     if inv_freq is None:
         return None, None, None, 0, 0, 0, 0
     if inv_freq.dtype is not torch.float64:
         _capi.check(3, op)
-    pairs = inv_freq.numel()
-    if inv_freq.dim() != 1 or not 0 < 2 * pairs <= d or not inv_freq.is_contiguous():
+    rot_dim, device = 2 * inv_freq.numel(), x.get_device()
+    if inv_freq.dim() != 1 or not 0 < rot_dim <= d or not inv_freq.is_contiguous():
         _capi.check(4, op)
+    if inv_freq.get_device() != device:
+        _elsewhere(op)
     if pos is None:
         if pos_needed:
             raise RuntimeError(f"{op}: a rotation needs positions")
-        return None, None, inv_freq.data_ptr(), 2 * pairs, 0, 0, 0
+        return None, None, inv_freq.data_ptr(), rot_dim, 0, 0, 0
     if pos.dtype is not torch.int64:
         _capi.check(3, op)
     if pos.shape != ((rows,) if mrope_section is None else (3, rows)):
         _capi.check(4, op)
+    if pos.get_device() != device:
+        _elsewhere(op)
     if not pos.is_contiguous():
         pos = pos.contiguous()
     if mrope_section is None:
-        return pos, pos.data_ptr(), inv_freq.data_ptr(), 2 * pairs, 0, 0, 0
+        return pos, pos.data_ptr(), inv_freq.data_ptr(), rot_dim, 0, 0, 0
     _, h, w = mrope_section
-    return pos, pos.data_ptr(), inv_freq.data_ptr(), 2 * pairs, 1, h, w
+    return pos, pos.data_ptr(), inv_freq.data_ptr(), rot_dim, 1, h, w
 
 
-def _norm_weight(w, dtype, d, op):
+def _norm_weight(w, x, d, op):
     """The address of a norm's weight."""
-    if w is None:
-        return None
-    if w.dtype is not dtype or w.shape != (d,) or not w.is_contiguous():
+    if w.dtype is not x.dtype or w.dim() != 1 or w.shape[0] != d or not w.is_contiguous():
         _capi.check(4, op)
+    if w.get_device() != x.get_device():
+        _elsewhere(op)
     return w.data_ptr()
+
+
+def _head_rows(t, op, x, rows, d):
+    """t (rows, heads, d), a contiguous copy where a row is not one run; the rows' stride; heads."""
+    if t is not x:
+        if t.dtype is not x.dtype:
+            _capi.check(3, op)
+        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d:
+            _capi.check(4, op)
+        if t.get_device() != x.get_device():
+            _elsewhere(op)
+    heads = t.shape[1]
+    ld, head_ld, element = t.stride()
+    if element != 1 or head_ld != d or ld < heads * d:
+        return t.contiguous(), heads * d, heads
+    return t, ld, heads
 
 
 def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False, factor: float = 1.0,
@@ -717,56 +735,52 @@ def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float =
         _capi.check(7, op)
     if not x.is_cuda:
         raise RuntimeError(f"{op}: expected CUDA tensors (this package has no CPU path)")
-    dtype, device = x.dtype, x.get_device()
+    dtype, device, shape = x.dtype, x.get_device(), x.shape
     dt = _TURN_DTYPES.get(dtype)
     if dt is None:
         _capi.check(3, op)
-    if x.dim() != 3:
+    if len(shape) != 3:
         _capi.check(4, op)
-    rows, _, d = x.shape
-    args, outs = [], []
-    for t in (q, k):
-        if t is None:
-            args.append((None, 0, 0))
-            outs.append(None)
-            continue
-        if t.dtype is not dtype:
-            _capi.check(3, op)
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != d:
-            _capi.check(4, op)
-        heads = t.shape[1]
-        ld, head_ld, element = t.stride()
-        if element != 1 or head_ld != d or ld < heads * d:  # rows that are not one run each
-            t = t.contiguous() if not t.is_contiguous() else t
-            ld = heads * d
-        args.append((t, ld, heads))
-        outs.append(torch.empty_like(t))  # rows apart or not, the copy is contiguous
-    (tq, q_ld, hq), (tk, k_ld, hkv) = args
-    wq, wk = _norm_weight(q_weight, dtype, d, op), _norm_weight(k_weight, dtype, d, op)
-    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, True)
-    _one_device(op, device, (q, k, pos, inv_freq, q_weight, k_weight))
-    _launch_on(device, op, _capi.lib().axb200_qk_norm_rope, tq.data_ptr() if tq is not None else None, q_ld,
-               tk.data_ptr() if tk is not None else None, k_ld, wq, wk, eps, at, freq, rot_dim, bool(interleaved), factor, mrope, h, w,
-               outs[0].data_ptr() if tq is not None else None, outs[1].data_ptr() if tk is not None else None, rows, hq, hkv, d, dt)
-    return outs[0], outs[1]
+    rows, _, d = shape
+    q_out = k_out = q_at = k_at = qo_at = ko_at = wq = wk = None
+    q_ld = k_ld = hq = hkv = 0
+    if q is not None:
+        q, q_ld, hq = _head_rows(q, op, x, rows, d)
+        q_out = torch.empty_like(q)  # rows apart or not, the copy is contiguous
+        q_at, qo_at = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        k, k_ld, hkv = _head_rows(k, op, x, rows, d)
+        k_out = torch.empty_like(k)
+        k_at, ko_at = k.data_ptr(), k_out.data_ptr()
+    if q_weight is not None:
+        wq = _norm_weight(q_weight, x, d, op)
+    if k_weight is not None:
+        wk = _norm_weight(k_weight, x, d, op)
+    # `pos` is held until the launch: it may be a copy
+    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, x, d, inv_freq, pos, rows, mrope_section, True)
+    _launch_on(device, op, _capi.lib().axb200_qk_norm_rope, q_at, q_ld, k_at, k_ld, wq, wk, eps, at, freq, rot_dim, interleaved, factor,
+               mrope, h, w, qo_at, ko_at, rows, hq, hkv, d, dt)
+    return q_out, k_out
 
 
-def _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start):
+def _portion_tables(op, x, k_pages, v_pages, block_table, seq_lens, row_start):
     """The batch of the operators below, and the addresses of pages and tables, after what a kernel would follow blindly was checked."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or block_table.dim() != 2 or seq_lens.dim() != 1 or row_start.dim() != 1:
         _capi.check(4, op)
-    if k_pages.dtype is not dtype or v_pages.dtype is not dtype or block_table.dtype is not torch.int32 or \
-            seq_lens.dtype is not torch.int32 or row_start.dtype is not torch.int32:
+    i32, dtype, device = torch.int32, x.dtype, x.get_device()
+    if k_pages.dtype is not dtype or v_pages.dtype is not dtype or block_table.dtype is not i32 or seq_lens.dtype is not i32 or \
+            row_start.dtype is not i32:
         _capi.check(3, op)
     batch = row_start.shape[0] - 1
     if batch < 1 or seq_lens.shape[0] < batch or block_table.shape[0] < batch:
         _capi.check(4, op)
-    tables = (k_pages, v_pages, block_table, seq_lens, row_start)
-    for t in tables:
-        if not t.is_contiguous():
-            raise RuntimeError(f"{op}: pages and tables must be contiguous")
-    _one_device(op, device, tables)
-    return batch, [t.data_ptr() for t in tables]
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous() and block_table.is_contiguous() and seq_lens.is_contiguous() and
+            row_start.is_contiguous()):
+        raise RuntimeError(f"{op}: pages and tables must be contiguous")
+    if k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device or \
+            seq_lens.get_device() != device or row_start.get_device() != device:
+        _elsewhere(op)
+    return batch, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), row_start.data_ptr()
 
 
 def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens, row_start,
@@ -781,7 +795,7 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
     dtype, device = qkv.dtype, qkv.get_device()
     if qkv.dim() != 2:
         _capi.check(4, op)
-    batch, pages = _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start)
+    batch, *pages = _portion_tables(op, qkv, k_pages, v_pages, block_table, seq_lens, row_start)
     num_pages, hkv, page_tokens, d = k_pages.shape
     rows, columns = qkv.shape
     ld, element = qkv.stride()
@@ -789,16 +803,16 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
         ld = columns
     if columns != (n_q_heads + 2 * hkv) * d or ld < columns or (element != 1 and columns > 1):
         _capi.check(4, op)
-    wq, wk = _norm_weight(q_norm_weight, dtype, d, op), _norm_weight(k_norm_weight, dtype, d, op)
-    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, d, inv_freq, pos, rows, mrope_section, False)
+    wq = None if q_norm_weight is None else _norm_weight(q_norm_weight, qkv, d, op)
+    wk = None if k_norm_weight is None else _norm_weight(k_norm_weight, qkv, d, op)
+    pos, at, freq, rot_dim, mrope, h, w = _rotation(op, qkv, d, inv_freq, pos, rows, mrope_section, False)
     if out is None:
         out = qkv.new_empty((rows, n_q_heads, d))
-    elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous():
+    elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
-    _one_device(op, device, (pos, inv_freq, q_norm_weight, k_norm_weight, out))
     _launch_on(device, op, _capi.lib().axb200_qkv_norm_rope_append_portions, qkv.data_ptr(), ld, wq, wk, eps, out.data_ptr(), *pages, at,
-               freq, rot_dim, bool(interleaved), factor, mrope, h, w, rows, batch, n_q_heads, hkv, d, page_tokens, block_table.shape[1],
-               num_pages, dt, bool(advance))
+               freq, rot_dim, interleaved, factor, mrope, h, w, rows, batch, n_q_heads, hkv, d, page_tokens, block_table.shape[1],
+               num_pages, dt, advance)
     return out
 
 
@@ -812,7 +826,7 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
     if q.dim() != 3:
         _capi.check(4, op)
     dtype, device = q.dtype, q.get_device()
-    batch, pages = _portion_tables(op, dtype, device, k_pages, v_pages, block_table, seq_lens, row_start)
+    batch, *pages = _portion_tables(op, q, k_pages, v_pages, block_table, seq_lens, row_start)
     rows, hq, d = q.shape
     num_pages, hkv, page_tokens, dk = k_pages.shape
     if dk != d or hkv == 0 or hq % hkv:
