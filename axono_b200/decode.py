@@ -10,7 +10,8 @@ projections are library GEMMs (one cuBLASLt call each through `ops.linear_nobias
 timed per shape on first use; `lt_gemm=False` takes torch.matmul), which stay outside the rewritten path;
 everything between them is this package's kernels.  Two fusions the reference's layer does not have:
 the residual add that ends a layer is folded into the next layer's input norm (one add_rms_norm),
-and rope + append is one launch.  With few rows on one rank a layer is two launches: the attention's step and
+and rope + append is one launch.  `extend` brings prompts and portions of them to the same cache (`append_portions`,
+`attend_portions`).  With few rows on one rank a layer is two launches: the attention's step and
 everything up to the next one (`ops.row_chain`).  KV heads shard across ranks (`world`, `rank`): each rank projects
 and attends its own heads and the per-head outputs are all-gathered before o_proj - the only
 collective of the step.
@@ -120,6 +121,8 @@ class TextTower:
             self.layers.append(lw)
         self.final_ln = ones(cfg.hidden)
         self.inv_freq = (1.0 / (cfg.rope_theta ** (torch.arange(0, d, 2, dtype=torch.float32) / d))).to(self.device)
+        # the frequencies of `decode_step`, as the operators for portions take them
+        self.portion_freq = self.inv_freq.double() if cfg.use_mrope else ops.reference_frequencies(d, cfg.rope_theta, self.device)
         self.cache = PagedKVCache(cfg.n_layers, batch, self.local_kv, d, max_seq_len, dtype=dtype,
                                   device=self.device, page_tokens=page_tokens)
         # static step state (graph inputs/outputs)
@@ -175,6 +178,43 @@ class TextTower:
                 h, xn = ops.add_rms_norm(mlp_out, h, lw["input_ln"], cfg.eps)
             h, mlp_out = self._feed_forward(lw, self._attention(li, xn), h)
         return self._finish_step(self._logits(mlp_out, h))
+
+    def extend(self, token_ids, counts) -> torch.Tensor:
+        """The next tokens of the batch's sequences at once: counts[b] (host) tokens of sequence b, 0 for none - whole prompts, portions
+        of them, single tokens - whose ids stand one sequence after the other in token_ids.  Appends them to every layer's cache and
+        leaves every sequence that brought some ready for `decode_step`: the greedy next token of its last one in `token_ids`, its
+        position in `pos3`.  Returns those tokens, and their logits are `last_logits` (one row per such sequence)."""
+        cfg, d = self.cfg, self.cfg.head_dim
+        counts = torch.as_tensor(counts, dtype=torch.int64).cpu()
+        ids = torch.as_tensor(token_ids, dtype=torch.int64).reshape(-1)
+        rows = int(counts.sum())
+        if counts.shape != (self.batch,) or int(counts.min()) < 0 or rows != ids.numel() or rows == 0:
+            raise RuntimeError("extend: a count for every sequence, and as many tokens as they add up to (at least one)")
+        starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+        seq = torch.repeat_interleave(torch.arange(self.batch), counts)
+        offset = (torch.arange(rows) - starts[seq]).to(self.device)
+        brought = counts.nonzero()[:, 0]
+        last = (starts[1:][brought] - 1).to(self.device)
+        row_start, seq, brought = starts.to(torch.int32).to(self.device), seq.to(self.device), brought.to(self.device)
+        pos = self.pos3[:, seq] + offset if cfg.use_mrope else self.pos3[0, seq] + offset
+        h, mlp_out = ops.embedding(ids.to(self.device), self.embed), None
+        for li, lw in enumerate(self.layers):
+            if mlp_out is None:
+                xn = ops.rms_norm(h, lw["input_ln"], cfg.eps)
+            else:
+                h, xn = ops.add_rms_norm(mlp_out, h, lw["input_ln"], cfg.eps)
+            q = self.cache.append_portions(li, self._linear(xn, lw["qkv"]), self.local_q, row_start, int(counts.max()),
+                                           lw["q_norm"] if cfg.qk_norm else None, lw["k_norm"] if cfg.qk_norm else None, cfg.eps, pos=pos,
+                                           inv_freq=self.portion_freq, mrope_section=cfg.mrope_section if cfg.use_mrope else None)
+            attn = self.cache.attend_portions(li, q, row_start)
+            if self.world > 1:
+                attn = sharding.all_gather_heads(attn)
+            h, mlp_out = self._feed_forward(lw, self._linear(attn.reshape(rows, cfg.n_q_heads * d), lw["o"]), h)
+        self.last_logits = self._logits(mlp_out[last], h[last])
+        nxt = ops.argmax_last_dim(self.last_logits)
+        self.token_ids[brought] = nxt
+        self.pos3 += counts.to(self.device)
+        return nxt
 
     def _feed_forward(self, lw, attn_out, h):
         """The second half of a layer as single operators: (h, what is still to be added to it)."""

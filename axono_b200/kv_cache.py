@@ -147,6 +147,27 @@ class PagedKVCache(KVCache):
         self._host_len_bound += 1
         return out
 
+    def append_portions(self, layer_idx: int, qkv, n_q_heads, row_start, longest=None, q_norm_weight=None, k_norm_weight=None, eps=1e-6,
+                        pos=None, inv_freq=None, interleaved=False, factor=1.0, mrope_section=None, out=None):
+        """The next tokens of several sequences - whole prompts, portions, single tokens - straight from the QKV projection: sequence
+        b's are the rows row_start[b] .. row_start[b + 1] - 1 of qkv.  Per-head norm and rotation (`ops.qkv_norm_rope_append_portions`),
+        keys and values behind the cached ones; returns q (rows, hq, d).  longest: host bound of the tokens one sequence brings
+        (default: all rows)."""
+        first = layer_idx == 0
+        q = ops.qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, self.k_pages[layer_idx],
+                                              self.v_pages[layer_idx], self.block_table, self.seq_lens, row_start, pos=pos,
+                                              inv_freq=inv_freq, interleaved=interleaved, factor=factor, mrope_section=mrope_section,
+                                              advance=first, out=out)
+        if first:
+            self._host_len_bound = min(self.max_seq_len, self._host_len_bound + (qkv.shape[0] if longest is None else int(longest)))
+        return q
+
+    def attend_portions(self, layer_idx: int, q, row_start, out=None):
+        """Causal attention of the rows that `append_portions` has appended, over the layer's cache (and its window)."""
+        bound = self.max_seq_len if torch.cuda.is_current_stream_capturing() else min(self.max_seq_len, self._host_len_bound)
+        return ops.gqa_attention_portions_paged(q, self.k_pages[layer_idx], self.v_pages[layer_idx], self.block_table, self.seq_lens,
+                                                row_start, max(bound, 1), window=getattr(self, "window", 0), out=out)
+
     def get(self, layer_idx: int):
         """(k_pages, v_pages, block_table, seq_lens) of the layer - the paged equivalent of the
         reference's (k_full, v_full)."""

@@ -650,6 +650,19 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling=None, device=
     return freq.to(device), factor
 
 
+def reference_frequencies(dim: int, theta: float, device="cuda"):
+    """theta^(-2i / dim) as the single-token operators have it where no frequencies are given - the C library's powf
+    (src/ops/cpu/sequence.cpp:83-84) - in the form of `rope_frequencies`: keys that come in portions and one by one stand at the same
+    angles, but for the rounding of position times frequency."""
+    import ctypes
+    import ctypes.util
+
+    powf = ctypes.CDLL(ctypes.util.find_library("m") or "libm.so.6").powf
+    powf.restype, powf.argtypes = ctypes.c_float, [ctypes.c_float, ctypes.c_float]
+    exponents = -2.0 * torch.arange(dim // 2, dtype=torch.float32) / float(dim)
+    return torch.tensor([powf(theta, e) for e in exponents.tolist()], dtype=torch.float64, device=device)
+
+
 def _elsewhere(op):
     raise RuntimeError(f"{op}: tensors on different devices")
 

@@ -434,3 +434,91 @@ def test_other_streams_graphs_and_two_calls_at_once():
     torch.cuda.synchronize()
     assert torch.equal(outs[0], first) and torch.equal(outs[1], second)
     assert ops.last_error() == 0
+
+
+# ---- in the tower ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("use_mrope,qk_norm,dtype", [(True, True, torch.float16), (False, False, torch.float16), (False, True, torch.float32)])
+def test_tower_extends_in_any_portions_as_it_decodes(use_mrope, qk_norm, dtype):
+    """Prompts at once, in portions (some sequences pausing), and token by token through `decode_step` leave the same cache and logits
+    but for roundings, and decoding goes on from any of them."""
+    from axono_b200 import ops
+    from axono_b200.decode import TextTower, TextTowerConfig
+
+    cfg = TextTowerConfig(hidden=256, intermediate=512, n_q_heads=8, n_kv_heads=4, head_dim=64, vocab=1000, n_layers=3, use_mrope=use_mrope,
+                          mrope_section=(12, 10, 10), qk_norm=qk_norm)
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (70, 3, 129)]
+    tower = lambda batch=3: TextTower(cfg, batch, 320, dtype=dtype, seed=3)  # noqa: E731
+
+    whole = tower()
+    whole.extend(torch.cat(prompts), [70, 3, 129])
+    parts = tower()
+    done = [0, 0, 0]
+    for counts in ([64, 1, 0], [0, 2, 100], [5, 0, 28], [1, 0, 1]):
+        ids = torch.cat([p[a:a + n] for p, a, n in zip(prompts, done, counts)])
+        parts.extend(ids, counts)
+        done = [a + n for a, n in zip(done, counts)]
+    assert parts.cache.seq_lens.tolist() == whole.cache.seq_lens.tolist() == [70, 3, 129]
+    assert torch.equal(parts.pos3, whole.pos3) and whole.pos3[0].tolist() == [70, 3, 129]
+    tol = 3e-2 if dtype == torch.float16 else 1e-3
+    close = lambda a, b: (a.double() - b.double()).abs().max() <= tol * b.abs().max()  # noqa: E731
+    for layer in range(cfg.n_layers):
+        for b in range(3):
+            for a, c in zip(parts.cache.gather(layer, b), whole.cache.gather(layer, b)):
+                assert close(a, c)
+    logits = []
+    for b, prompt in enumerate(prompts):  # the single-token path, one sequence at a time
+        one = tower(1)
+        one.set_state([int(prompt[0])], [0])
+        for i in range(len(prompt)):
+            one.token_ids.fill_(int(prompt[i]))
+            one.decode_step()
+        logits.append(one.last_logits[0])
+        for layer in range(cfg.n_layers):
+            for a, c in zip(one.cache.gather(layer, 0), whole.cache.gather(layer, b)):
+                assert close(a, c)
+        assert close(whole.last_logits[b], one.last_logits[0])
+    for t in (whole, parts):
+        t.token_ids.copy_(torch.tensor([5, 6, 7]))
+        t.decode_step()
+    assert close(parts.last_logits, whole.last_logits)
+    with pytest.raises(RuntimeError):
+        whole.extend(torch.zeros(3, dtype=torch.int64), [1, 1])
+    with pytest.raises(RuntimeError):
+        whole.extend(torch.zeros(3, dtype=torch.int64), [1, 1, 0])
+    assert ops.last_error() == 0
+
+
+def test_windowed_cache_takes_portions():
+    """A cache with a window: portions attend the last tokens only, as its decoding does."""
+    from axono_b200 import ops
+    from axono_b200.kv_cache import PagedKVCache, SlidingWindowKVCache
+
+    hq, hkv, d, window = 4, 2, 128, 40
+    caches = [SlidingWindowKVCache(window, 1, 2, hkv, d, 256), PagedKVCache(1, 2, hkv, d, 256)]
+    starts = row_table([90, 60])
+    qkv = rnd((150, (hq + 2 * hkv) * d), torch.float16, 3)
+    outs = []
+    for cache in caches:
+        q = cache.append_portions(0, qkv, hq, starts, 90, inv_freq=freqs(d))
+        outs.append(cache.attend_portions(0, q, starts))
+    assert not torch.equal(outs[0], outs[1]) and torch.equal(outs[0][:window], outs[1][:window])
+    ref = Cache([90, 60], hkv, d, torch.float16)
+    ref.k, ref.v = zip(*[caches[0].gather(0, b) for b in range(2)])
+    check_attention(q, ref, (90, 60), starts.tolist(), outs[0], window)
+    one = rnd((2, (hq + 2 * hkv) * d), torch.float16, 9)
+    q1 = caches[0].append_portions(0, one, hq, row_table([1, 1]), 1, inv_freq=freqs(d))
+    a, b = caches[0].attend_portions(0, q1, row_table([1, 1])), caches[0].attend(0, q1)
+    assert (a.double() - b.double()).abs().max() <= 2.0 ** -9 * b.abs().max()
+    assert ops.last_error() == 0
+
+
+def test_frequencies_of_the_single_token_operators():
+    from axono_b200 import ops
+
+    x = rnd((4, 2, 128), torch.float32)
+    pos = torch.arange(4, device="cuda")
+    a = ops.rope(x, pos, 5e5)
+    b, _ = ops.qk_norm_rope(x, None, pos, ops.reference_frequencies(128, 5e5))
+    assert (a - b).abs().max() <= 2.0 ** -20 * x.abs().max()
