@@ -87,7 +87,10 @@ int join_portions(const PortionParams &p, cudaStream_t st) {
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Rows per block, and the bounds within which the kernels divide the keys: where all blocks run at once, into as many parts as do.
+// Rows per block, and the bounds within which the kernels divide the keys: nothing to divide among many times the blocks that run at once;
+// blocks that do not fill the GPU are divided into as many parts as run at once; blocks of few rows, which are bound by memory and cheap to
+// join, into parts that take some rounds.  Room in the grid that the lengths do not use costs time: three rounds of CTAs that find no work 18
+// us (8192 rows of a prompt 255 and 298 us), while 64 sequences of 16 K to 32 K tokens with a row each take 1087 us whole and 963 in parts.
 // A part has 1024 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 65536 keys are 4096 products.
 void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32) {
   p.tokens = tensor ? kPortionRows / p.group : portion_fma_tokens(p.group);
@@ -102,14 +105,22 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32)
   tiles = tiles < 1 ? 1 : tiles;
   const int some = p.rows < p.batch ? p.rows : p.batch;  // sequences with rows: each may add a block that is not full
   const int64_t blocks = some + (p.rows - some) / p.tokens;
-  const int64_t needed = (tiles + kPortionMostTiles - 1) / kPortionMostTiles, at_once = places / p.hkv;
+  const int64_t needed = (tiles + kPortionMostTiles - 1) / kPortionMostTiles, at_once = places / p.hkv > 0 ? places / p.hkv : 1;
   const size_t per_part = (size_t)p.rows * p.hq * (p.d + 2) * sizeof(float);
-  int64_t parts = blocks < at_once ? (tiles / 2 < 128 ? tiles / 2 : 128) : 1;
+  const float fill = (float)p.rows / ((float)blocks * p.tokens);  // of the blocks' rows
+  int64_t room = 0;  // units beside the blocks
+  if (blocks < at_once && (2 * blocks < at_once || (fill > 0.5f && !f32)))
+    room = at_once - blocks;
+  else if (blocks < 4 * at_once && tiles >= 32 && (fill <= 0.5f || f32))
+    room = 3 * at_once < blocks * (tiles / 16) ? 3 * at_once : blocks * (tiles / 16);
+  int64_t parts = room ? (tiles / 2 < 128 ? tiles / 2 : 128) : 1;
   while (parts > 1 && parts * per_part > ((size_t)1 << 30)) --parts;
-  p.parts = (int)(parts > needed ? parts : needed);
-  p.units = (int)(p.parts > 1 && at_once > blocks * needed ? at_once : blocks * needed);
-  p.least_gain = f32 ? 3.f : 6.f;
-  p.part_gain = (float)(2. * per_part / (f32 ? 8e6 : 3e6));
+  p.parts = (int)(parts > needed ? parts : needed > 1 ? needed : 1);
+  p.units = (int)(p.parts > 1 && blocks + room > blocks * needed ? blocks + room : blocks * needed);
+  p.at_once = (int)at_once;
+  // what a part's sums cost, to memory and back, grows with the rows of a block
+  p.part_cost = f32 ? 2.f + 2.f * fill : 4.f + 4.f * fill;
+  p.join_cost = f32 ? 2.f : 4.f;
 }
 
 size_t portion_scratch(PortionParams &p, void *base) {

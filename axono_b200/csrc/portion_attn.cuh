@@ -26,7 +26,8 @@ struct PortionParams {
   int max_keys;       // keys of a sequence that the grid is made for
   int tokens, units;  // rows of a block; blocks and parts of blocks that the grid has for a KV head
   int parts;          // the most parts that a block's keys are divided into; 1: not at all
-  float least_gain, part_gain;  // tiles in a row that dividing has to save, and that each further part has to
+  int at_once;        // units of a KV head that run at once
+  float part_cost, join_cost;  // of a part and of joining, in the time of a tile
   float scale_log2;  // of scores, in powers of two
   unsigned long long wait_ns;
   // with parts > 1, results of blocks with divided keys: un-normalised sums (part, row, head, d), their (maximum, denominator), and of
@@ -80,9 +81,11 @@ struct PortionSpan {
 // Finds block and part `index` of the launch, the last rows of a sequence first (they have the most keys).  Called by all threads of a
 // CTA; false beyond the last.
 //
-// Where blocks may be too few to fill the GPU, every CTA first makes the same plan from the lengths: the blocks of a sequence get
-// ceil(t / L) parts, t the tiles at its end.  With N blocks and V = sum of blocks x t these are at most V / L + N, so that L = V / (units -
-// N) fits the grid, whose units run at once.
+// Where blocks may be too few to fill the GPU, or too unequal, every CTA first makes the same plan from the lengths: the blocks of a
+// sequence get ceil(t / L) parts, t the tiles at its end.  With N blocks and V = sum of blocks x t these are at most V / L + N, so that
+// L = V / (units - N) fits the grid.  Times of a tile: blocks that all run at once take the longest, else an even share and half of the
+// longest; parts that run at once (L from V / (at_once - N) on) take L; parts in several rounds are best with L = sqrt(2 V part_cost /
+// at_once), which takes an even share and half of L.
 __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int index, PortionBlock &block, PortionSearch *search) {
   volatile int &s_found = search->found;
   int *s_sums = search->sums;
@@ -112,10 +115,16 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
       v += search->totals[1][w];
       most = fmaxf(most, search->totals[2][w]);
     }
-    if (n < p.units) {
-      const float length = ceilf(fmaxf(v * 1.001f / (p.units - n), sqrtf(most * 0.12f)));  // joining a part takes 0.12 tiles
-      if (length >= 1.f && most - length > p.least_gain + p.part_gain * most / length) part_tiles = fminf(part_tiles, length);
-    }
+    const float share = v / p.at_once, joining = p.join_cost + 0.12f;
+    float best = n <= p.at_once ? most + p.part_cost : share + n / p.at_once * p.part_cost + 0.5f * most;
+    const auto consider = [&](float length, bool rounds) {
+      length = fmaxf(ceilf(fmaxf(length, v * 1.001f / (p.units - n))), 1.f);
+      const float parts = v / length + n;
+      const float time = (rounds ? share + parts / p.at_once * p.part_cost + 0.5f * length : length + p.part_cost) + joining + 0.12f * most / length;
+      if (length < most && time < best) best = time, part_tiles = fminf((float)kPortionMostTiles, length);
+    };
+    if (n < p.units && n < p.at_once) consider(fmaxf(v * 1.001f / (p.at_once - n), sqrtf(0.12f * most)), false);
+    if (n < p.units && p.units > p.at_once) consider(sqrtf(2.f * share * p.part_cost), true);
   }
   int before = 0;  // blocks and parts of the sequences before this round's
   for (int base = 0; base < p.batch; base += blockDim.x) {
