@@ -438,7 +438,9 @@ int launch_rows(const TurnParams &p, int ways, int blocks, int warps, int32_t *s
   return launch_dependent(kernels[2 * p.interleaved + full], dim3((unsigned)blocks), dim3(warps * 32), smem, st, p, ways, seq_lens);
 }
 
-// Few rows are shared among warps, down to a group of heads each.  `done`: the lengths are advanced too.
+// Few rows are shared among warps, down to a group of heads each: up to 16 warps per SM, since every share forms the row's cosines and
+// sines again (fp32, 1435 rows of 16 heads of 80: 7.8 us undivided, 5.5 in two shares, 6.5 in four; 8192 rows of 24 heads of 128: 24.5, 28.5
+// and 38.8).  `done`: the lengths are advanced too.
 template <typename T, bool kAppend, int kLanes>
 int launch_lanes(const TurnParams &p, int32_t *seq_lens, bool &done, cudaStream_t st) {
   constexpr int kAtOnce = 32 / kLanes, kSoloWarps = kSoloThreads / 32;
@@ -452,7 +454,7 @@ int launch_lanes(const TurnParams &p, int32_t *seq_lens, bool &done, cudaStream_
       return launch_rows<T, kAppend, kLanes, true>(p, ways, 1, (int)(tasks < kSoloWarps ? tasks : kSoloWarps), seq_lens, st);
     }
   }
-  while (p.rows * ways < 148 * 8 && ways * 2 <= groups) ways *= 2;
+  while (p.rows * ways < 148 * 16 && ways * 2 <= groups) ways *= 2;
   const int64_t blocks = (p.rows * ways + kRowThreads / 32 - 1) / (kRowThreads / 32), most = 148 * kRowBlocks;
   return launch_rows<T, kAppend, kLanes, false>(p, ways, (int)(blocks < most ? blocks : most), kRowThreads / 32, nullptr, st);
 }
