@@ -91,7 +91,9 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // blocks that do not fill the GPU are divided into as many parts as run at once; blocks of few rows, which are bound by memory and cheap to
 // join, into parts that take some rounds.  Room in the grid that the lengths do not use costs time: three rounds of CTAs that find no work 18
 // us (8192 rows of a prompt 255 and 298 us), while 64 sequences of 16 K to 32 K tokens with a row each take 1087 us whole and 963 in parts.
+// Few blocks of few tiles are clusters (FILL).
 // A part has 1024 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 65536 keys are 4096 products.
+constexpr int kMostClusterTiles = 48;
 void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32) {
   p.tokens = tensor ? kPortionRows / p.group : portion_fma_tokens(p.group);
   const int places = tensor && f32 ? kSms : 2 * kSms;
@@ -108,15 +110,20 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32)
   const int64_t needed = (tiles + kPortionMostTiles - 1) / kPortionMostTiles, at_once = places / p.hkv > 0 ? places / p.hkv : 1;
   const size_t per_part = (size_t)p.rows * p.hq * (p.d + 2) * sizeof(float);
   const float fill = (float)p.rows / ((float)blocks * p.tokens);  // of the blocks' rows
+  p.cluster = 1;
+  if (tensor && !f32 && tiles <= kMostClusterTiles)
+    while (p.cluster < kMostCluster && p.cluster * 2 <= tiles && blocks * p.hkv * p.cluster * 2 <= places) p.cluster *= 2;
   int64_t room = 0;  // units beside the blocks
-  if (blocks < at_once && (2 * blocks < at_once || (fill > 0.5f && !f32)))
+  if (p.cluster > 1) {
+  } else if (blocks < at_once && (2 * blocks < at_once || (fill > 0.5f && !f32)))
     room = at_once - blocks;
   else if (blocks < 4 * at_once && tiles >= 32 && (fill <= 0.5f || f32))
     room = 3 * at_once < blocks * (tiles / 16) ? 3 * at_once : blocks * (tiles / 16);
   int64_t parts = room ? (tiles / 2 < 128 ? tiles / 2 : 128) : 1;
   while (parts > 1 && parts * per_part > ((size_t)1 << 30)) --parts;
   p.parts = (int)(parts > needed ? parts : needed > 1 ? needed : 1);
-  p.units = (int)(p.parts > 1 && blocks + room > blocks * needed ? blocks + room : blocks * needed);
+  const int64_t units = p.parts > 1 && blocks + room > blocks * needed ? blocks + room : blocks * needed;
+  p.units = units * p.hkv * p.cluster <= 0x7fffffff / 2 ? (int)units : 0;  // 0: more than a grid holds
   p.at_once = (int)at_once;
   // what a part's sums cost, to memory and back, grows with the rows of a block
   p.part_cost = f32 ? 2.f + 2.f * fill : 4.f + 4.f * fill;
@@ -187,6 +194,7 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
                       axb::aligned16(k_pages) && axb::aligned16(v_pages);
   axb::PortionParams p =
       axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, num_pages, max_seq_len, window, dtype, tensor);
+  if (p.units == 0) return AXB200_INVALID_ARGUMENT;
   const size_t need = axb::portion_scratch(p, workspace);
   if (need && (!workspace || workspace_bytes < need)) return AXB200_OUT_OF_MEMORY;
   if (need && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return AXB200_INVALID_PTR;

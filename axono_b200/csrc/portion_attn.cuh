@@ -16,6 +16,7 @@ namespace axb {
 constexpr int kPortionKeys = 64;   // keys of a tile, which lies in one page
 constexpr int kPortionWarps = 14;  // of a CTA at most
 constexpr int kPortionMostTiles = 1024;  // of a part
+constexpr int kMostCluster = 8;
 
 struct PortionParams {
   const void *q;
@@ -27,6 +28,7 @@ struct PortionParams {
   int tokens, units;  // rows of a block; blocks and parts of blocks that the grid has for a KV head
   int parts;          // the most parts that a block's keys are divided into; 1: not at all
   int at_once;        // units of a KV head that run at once
+  int cluster;        // CTAs that share a block by themselves (parts == 1 then); 1: one
   float part_cost, join_cost;  // of a part and of joining, in the time of a tile
   float scale_log2;  // of scores, in powers of two
   unsigned long long wait_ns;

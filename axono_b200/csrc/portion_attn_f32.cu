@@ -409,9 +409,7 @@ int launch(const PortionParams &p, const CUtensorMap &mk, const CUtensorMap &mv,
       return AXB200_DEVICE_ERROR;
     opted[dev] = true;
   }
-  const int64_t ctas = (int64_t)p.units * p.hkv;
-  if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
-  return launch_dependent(portion_f32_kernel<kB>, dim3((unsigned)ctas), dim3(kThreads), Layout<kB>::kSmem, st, mk, mv, p);
+  return launch_dependent(portion_f32_kernel<kB>, dim3((unsigned)(p.units * p.hkv)), dim3(kThreads), Layout<kB>::kSmem, st, mk, mv, p);
 }
 
 }  // namespace

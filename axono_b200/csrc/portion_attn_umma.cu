@@ -4,7 +4,8 @@
 // and part of its keys, two CTAs per SM.  Tiles of 64 keys, each in one page, whose 64 rows of a KV head are one run of memory: TMA fetches
 // them through a map of the pool (d, page_tokens, hkv, num_pages).  S = Q.K^T (128 x 64) and O += P.V are tcgen05.mma with the sums in
 // tensor memory; thread t owns virtual row t: scores from tensor memory, online softmax in registers, P as fp16 pairs over the scores,
-// from where P.V takes its A operand.  S is computed two tiles ahead.  Few rows leave most of the 128 empty: their warps stay out, and
+// from where P.V takes its A operand.  S is computed two tiles ahead.  A short call's few blocks are clusters of up to eight CTAs that
+// divide a block's keys and join their sums through each other's shared memory: one launch, and no scratch.  Few rows leave most of the 128 empty: their warps stay out, and
 // the products, which take as long as full ones, keep up with memory all the same (a tile of 32 KB in 660 cycles of an SM, 12 TB/s).
 //
 // Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
@@ -28,6 +29,67 @@ constexpr int kOffK = kQBytes, kOffV = kOffK + kKStages * kTileBytes, kOffBar = 
 constexpr int kOffPages = kOffBar + 160, kPageRing = 64, kOffSearch = kOffPages + kPageRing * 4;
 constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
 constexpr float kLazyLog2 = 8.0f;
+constexpr int kOffMl = kM * (kD + 4) * 4;  // of a cluster's part: (maximum, denominator) behind its sums, both where tiles were
+
+// A peer's shared memory in the cluster.
+__device__ __forceinline__ uint32_t peer_address(uint32_t address, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 load_peer4(uint32_t address) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address));
+  return v;
+}
+__device__ __forceinline__ float2 load_peer2(uint32_t address) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(address));
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The parts of a cluster's block joined: CTA `rank` takes every size-th virtual row, a warp per row, four columns per lane.
+__device__ __forceinline__ void join_cluster(const PortionParams &p, const PortionBlock &block, const uint8_t *smem, int hk, int rank) {
+  const int lane = threadIdx.x & 31, size = p.cluster;
+  const uint32_t sums = smem_u32(smem), ml = sums + kOffMl;
+  for (int v = rank + size * (threadIdx.x >> 5); v < block.rows * p.group; v += size * (kThreads / 32)) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (lane < size) mine = load_peer2(peer_address(ml + v * 8, lane));
+    float4 x[kMostCluster];
+#pragma unroll
+    for (int k = 0; k < kMostCluster; ++k) {
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < size && lane * 4 < p.d) x[k] = load_peer4(peer_address(sums + (v * (p.d + 4) + lane * 4) * 4, k));
+    }
+    float m = mine.x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const bool there = !(mine.x == -INFINITY && mine.y <= 0.f);  // else no key, or no score above -inf
+    const float weight = there ? exp2f(mine.x - (m == -INFINITY ? 0.f : m)) : 0.f;
+    const unsigned use = __ballot_sync(0xffffffffu, there);
+    const float l = warp_sum(there ? weight * mine.y : 0.f);
+    const float inv = portion_inverse(l, __any_sync(0xffffffffu, mine.y != 0.f));
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMostCluster; ++k) {
+      const float w = __shfl_sync(0xffffffffu, weight, k);
+      if (!((use >> k) & 1)) continue;
+      o.x = fmaf(w, x[k].x, o.x), o.y = fmaf(w, x[k].y, o.y), o.z = fmaf(w, x[k].z, o.z), o.w = fmaf(w, x[k].w, o.w);
+    }
+    const int token = v / p.group, head = hk * p.group + v % p.group;
+    const float bad = fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f)));
+    if (lane * 4 < p.d)
+      *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + ((size_t)(block.row0 + token) * p.hq + head) * p.d + lane * 4) =
+          make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+    __syncwarp();  // other lanes write such a row anew
+    if (__any_sync(0xffffffffu, bad != 0.f && lane * 4 < p.d))
+      redo_portion_row<__half>(p, block, token, head, block.tile0 * kN, (block.tile0 + block.tiles) * kN);
+  }
+}
 
 // Warps 0-3: softmax, thread = virtual row; warp 4 issues the products; warp 5 the copies.  They meet on mbarriers: full / empty per
 // stage, bar_s (S_j ready, per buffer), bar_p (P_j written, per buffer, one arrival per softmax warp that has rows), bar_o (P_j.V_j
@@ -55,11 +117,13 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
   grid_dependency_launch();
   grid_dependency_wait();
-  const int hk = blockIdx.x % p.hkv, index = blockIdx.x / p.hkv;
+  // in a cluster: one block, and each CTA a part of its keys
+  const int rank = blockIdx.x % p.cluster, unit = blockIdx.x / p.cluster, hk = unit % p.hkv, index = unit / p.hkv;
   PortionBlock block;
   if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(smem + kOffSearch))) return;
-  const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
-  const int nkv = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts) - tile0;
+  const int part = p.cluster > 1 ? rank : block.part, parts = p.cluster > 1 ? p.cluster : block.parts;
+  const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, parts);
+  const int nkv = block.tile0 + portion_part_begin(block.tiles, part + 1, parts) - tile0;
   const int virtual_rows = block.rows * p.group, active_warps = (virtual_rows + 31) >> 5;
   const bool two_boxes = p.d > 64;
   const uint32_t tile_bytes = two_boxes ? kTileBytes : kTileBytes / 2;
@@ -271,11 +335,26 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int key0 = max(key_begin, tile0 * kN), key1 = min(key_end, (tile0 + nkv) * kN);
     const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
     if (ok && p.parts > 1 && block.part == 0 && there && head == 0) p.row_parts[row] = block.parts;
-    if (ok && nkv == 0 && there) {  // no key at all
+    if (p.cluster > 1) {
+      if (ok) {
+        float *sums = reinterpret_cast<float *>(smem) + threadIdx.x * (p.d + 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c * 32 >= p.d || nkv == 0) break;
+          uint32_t r[32];
+          tmem_ld32(tmem_o + lane_base + c * 32, r);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c * 32 + u * 4 < p.d)
+              *reinterpret_cast<uint4 *>(sums + c * 32 + u * 4) = make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
+        }
+        reinterpret_cast<float2 *>(smem + kOffMl)[threadIdx.x] = portion_ml(m_run, l_run, nkv > 0 && key0 < key1);
+      }
+    } else if (ok && nkv == 0 && there) {  // no key at all
       uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d);
       for (int c = 0; c < p.d / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
     }
-    if (ok && nkv > 0) {
+    if (ok && nkv > 0 && p.cluster == 1) {
       const float inv = portion_inverse(l_run, key0 < key1);
       float bad = 0.f;  // NaN once a sum is not finite
 #pragma unroll
@@ -321,6 +400,11 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+  if (p.cluster > 1) {  // every CTA of it comes here, whatever its waits gave
+    cluster_barrier();
+    join_cluster(p, block, smem, hk, rank);
+    cluster_barrier();  // the peers have read this CTA's part
+  }
 }
 
 bool encode(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -353,9 +437,23 @@ int portions_umma(const PortionParams &p, cudaStream_t st) {
       return AXB200_DEVICE_ERROR;
     opted[dev] = true;
   }
-  const int64_t ctas = (int64_t)p.units * p.hkv;
-  if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
-  return launch_dependent(portion_umma_kernel, dim3((unsigned)ctas), dim3(kThreads), kSmem, st, mq, mk, mv, p);
+  if (p.cluster == 1)
+    return launch_dependent(portion_umma_kernel, dim3((unsigned)(p.units * p.hkv)), dim3(kThreads), kSmem, st, mq, mk, mv, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.units * p.hkv * p.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)p.cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, portion_umma_kernel, mq, mk, mv, p) == cudaSuccess) return AXB200_OK;
+  cudaGetLastError();
+  return AXB200_DEVICE_ERROR;
 }
 
 }  // namespace axb
