@@ -4,13 +4,20 @@
 // and part of its keys, two CTAs per SM.  Tiles of 64 keys, each in one page, whose 64 rows of a KV head are one run of memory: TMA fetches
 // them through a map of the pool (d, page_tokens, hkv, num_pages).  S = Q.K^T (128 x 64) and O += P.V are tcgen05.mma with the sums in
 // tensor memory; thread t owns virtual row t: scores from tensor memory, online softmax in registers, P as fp16 pairs over the scores,
-// from where P.V takes its A operand.  S is computed two tiles ahead.  A short call's few blocks are clusters of up to eight CTAs that
-// divide a block's keys and join their sums through each other's shared memory: one launch, and no scratch.  Few rows leave most of the 128 empty: their warps stay out, and
-// the products, which take as long as full ones, keep up with memory all the same (a tile of 32 KB in 660 cycles of an SM, 12 TB/s).
+// from where P.V takes its A operand.  S is computed two tiles ahead.
 //
 // Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
 // still meet weights of zero in P.V, so rows of V behind the sequence's end, where anything may stand, are cleared in shared memory
 // before the product, and rows that are not finite are done over without them (redo_portion_row).
+//
+// Few rows leave most of the 128 empty: their warps stay out, and the products, which take as long as full ones, keep up with memory all
+// the same (37 sequences of 16384 tokens, a row each, 8 KV heads: 350 us, 7.1 TB/s; 10.1 from L2).  A short call's few blocks are clusters
+// of up to eight CTAs that divide a block's keys and join their sums through each other's shared memory: one launch, no scratch.
+//
+// Bound by the latency of a tile's chain - scores, softmax, weights - on two CTAs: 2368 rows over 14000 tokens, 16 / 8 heads of 128, 263 us
+// (1110 TFLOP/s), 1050 cycles of an SM per tile where the products take 660 and the exponentials 510; heads of 64: 211 us.  Tried, not
+// kept: three stages of V and two of K (drafts 118 -> 124 us), four of each with one CTA per SM (161), up to 32 rows four times in the block
+// with a quarter of a tile's keys for each warp (no change: few rows wait for memory or for the chain around the softmax, not in it).
 #include <math.h>
 
 #include <mutex>
@@ -259,7 +266,8 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int token = threadIdx.x / p.group, head = hk * p.group + threadIdx.x % p.group;
     const bool there = token < block.rows;
     // Rows that are none (a group that does not divide 128, the last block of a sequence) are left unmasked: what they compute is stored
-    // nowhere and moves no maximum, and a mask for one row costs its warp 200 instructions with every tile (heads of 64, three to a KV head: 538 us and FILL).
+    // nowhere and moves no maximum, and a mask for one row costs its warp 200 instructions with every tile (heads of 64, three to a KV
+    // head, 2368 rows over 14000 tokens: 538 us, and 398 so).
     const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0x7fffffff;
     const int key_begin = there && p.window ? max(0, pos + 1 - p.window) : 0;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;

@@ -667,15 +667,13 @@ def _elsewhere(op):
     raise RuntimeError(f"{op}: tensors on different devices")
 
 
-def _launch_on(device, op, call, *args):
-    """The call on the device's current stream, with the device as the current one (a launch goes to the current device whatever its
-    stream).  torch.cuda.current_stream and current_device take 5 us of the 15 that a call of these operators has."""
+# torch.cuda.current_stream and current_device take 5 us of the 14 that a call of these operators has; these two take 0.2
+_device_now = torch._C._cuda_getDevice
+_stream_now = torch._C._cuda_getCurrentRawStream
+
+
+def _launched(status, op):
     global _launches
-    if device == torch._C._cuda_getDevice():
-        status = call(*args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            status = call(*args, torch._C._cuda_getCurrentRawStream(device))
     if status:
         _capi.check(status, op)
     _launches += 1
@@ -749,6 +747,9 @@ def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float =
     if not x.is_cuda:
         raise RuntimeError(f"{op}: expected CUDA tensors (this package has no CPU path)")
     dtype, device, shape = x.dtype, x.get_device(), x.shape
+    if device != _device_now():  # a launch goes to the current device whatever its stream
+        with torch.cuda.device(device):
+            return qk_norm_rope(q, k, pos, inv_freq, q_weight, k_weight, eps, interleaved, factor, mrope_section)
     dt = _TURN_DTYPES.get(dtype)
     if dt is None:
         _capi.check(3, op)
@@ -771,8 +772,8 @@ def qk_norm_rope(q, k, pos, inv_freq, q_weight=None, k_weight=None, eps: float =
         wk = _norm_weight(k_weight, x, d, op)
     # `pos` is held until the launch: it may be a copy
     pos, at, freq, rot_dim, mrope, h, w = _rotation(op, x, d, inv_freq, pos, rows, mrope_section, True)
-    _launch_on(device, op, _capi.lib().axb200_qk_norm_rope, q_at, q_ld, k_at, k_ld, wq, wk, eps, at, freq, rot_dim, interleaved, factor,
-               mrope, h, w, qo_at, ko_at, rows, hq, hkv, d, dt)
+    _launched(_capi.lib().axb200_qk_norm_rope(q_at, q_ld, k_at, k_ld, wq, wk, eps, at, freq, rot_dim, bool(interleaved), factor, mrope, h, w, qo_at,
+                                              ko_at, rows, hq, hkv, d, dt, _stream_now(device)), op)
     return q_out, k_out
 
 
@@ -806,6 +807,10 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
     op = "qkv_norm_rope_append_portions"
     dt = _dt(qkv, op)
     dtype, device = qkv.dtype, qkv.get_device()
+    if device != _device_now():
+        with torch.cuda.device(device):
+            return qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens,
+                                                 row_start, pos, inv_freq, interleaved, factor, mrope_section, advance, out)
     if qkv.dim() != 2:
         _capi.check(4, op)
     batch, *pages = _portion_tables(op, qkv, k_pages, v_pages, block_table, seq_lens, row_start)
@@ -823,9 +828,9 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
         out = qkv.new_empty((rows, n_q_heads, d))
     elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
-    _launch_on(device, op, _capi.lib().axb200_qkv_norm_rope_append_portions, qkv.data_ptr(), ld, wq, wk, eps, out.data_ptr(), *pages, at,
-               freq, rot_dim, interleaved, factor, mrope, h, w, rows, batch, n_q_heads, hkv, d, page_tokens, block_table.shape[1],
-               num_pages, dt, advance)
+    _launched(_capi.lib().axb200_qkv_norm_rope_append_portions(
+        qkv.data_ptr(), ld, wq, wk, eps, out.data_ptr(), *pages, at, freq, rot_dim, bool(interleaved), factor, mrope, h, w, rows, batch, n_q_heads,
+        hkv, d, page_tokens, block_table.shape[1], num_pages, dt, bool(advance), _stream_now(device)), op)
     return out
 
 
@@ -839,6 +844,9 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
     if q.dim() != 3:
         _capi.check(4, op)
     dtype, device = q.dtype, q.get_device()
+    if device != _device_now():
+        with torch.cuda.device(device):
+            return gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row_start, max_seq_len, window, out)
     batch, *pages = _portion_tables(op, q, k_pages, v_pages, block_table, seq_lens, row_start)
     rows, hq, d = q.shape
     num_pages, hkv, page_tokens, dk = k_pages.shape
@@ -851,10 +859,11 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
     elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
     lib, blocks = _capi.lib(), block_table.shape[1]
-    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, max_seq_len, window, dt)
+    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, int(max_seq_len), int(window), dt)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None  # of this call alone: streams may overlap
-    _launch_on(device, op, lib.axb200_gqa_attention_portions_paged, q.data_ptr(), out.data_ptr(), *pages, rows, batch, hq, hkv, d,
-               page_tokens, blocks, num_pages, max_seq_len, window, dt, ws.data_ptr() if need else None, need)
+    _launched(lib.axb200_gqa_attention_portions_paged(
+        q.data_ptr(), out.data_ptr(), *pages, rows, batch, hq, hkv, d, page_tokens, blocks, num_pages, int(max_seq_len), int(window),
+        dt, ws.data_ptr() if need else None, need, _stream_now(device)), op)
     return out
 
 
