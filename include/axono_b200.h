@@ -425,7 +425,9 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *     length stays; a page outside the pool sets AXB200_ERR_BAD_PAGE, its rows are not written and the length stays.  FLOAT16, FLOAT32.
  *   gqa_attention_portions_paged: q, out (rows, hq, d): row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
  *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
- *     counts the portion.  A row that sees no key gets zeros.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
+ *     counts the portion.  A row that sees no key gets zeros; keys and values that a row does not see, and what stands behind a sequence's
+ *     end, do not touch it whatever they are.  Rows whose result is not finite, and in FLOAT32 blocks with values that are not finite,
+ *     above 3.39e38 or, unless zero, below 2^-100, are computed a second time without the tensor cores, at that speed.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
  *     sets AXB200_ERR_CAPACITY and its keys beyond are not read.  FLOAT16, FLOAT32.  workspace: at least the bytes that
  *     portions_workspace_bytes gives for the same arguments (0: none), 16-byte aligned, of this call alone until its kernels are done. */
 int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *q_norm_w, const void *k_norm_w, float eps,
