@@ -264,9 +264,9 @@ turn_rows_kernel(const TurnParams p, int ways, int32_t *seq_lens) {
       }
     }
     T *out_q = static_cast<T *>(p.q_out) + row * p.hq * p.d, *out_k, *out_v;
-    int head_step = p.d;  // between the heads of keys
+    int64_t head_step = p.d;  // between the heads of keys
     if constexpr (kAppend) {
-      head_step = p.page_tokens * p.d;
+      head_step = (int64_t)p.page_tokens * p.d;
       out_k = static_cast<T *>(p.k_pages) + place.element;
       out_v = static_cast<T *>(p.v_pages) + place.element;
     } else {
@@ -285,7 +285,7 @@ turn_rows_kernel(const TurnParams p, int ways, int32_t *seq_lens) {
       if (h >= end || !place.alive) continue;
       const bool query = h < p.hq;
       if (kAppend && h >= rotated) {  // a value: the bits as they came
-        uint4 *dst = reinterpret_cast<uint4 *>(out_v + (int64_t)(h - rotated) * head_step);
+        uint4 *dst = reinterpret_cast<uint4 *>(out_v + (h - rotated) * head_step);
         if (written && has_a) dst[va] = raw[0];
         if (written && has_b) dst[vb] = raw[1];
         continue;
@@ -340,7 +340,7 @@ turn_rows_kernel(const TurnParams p, int ways, int32_t *seq_lens) {
         }
       }
       if (!query && !written) continue;
-      uint4 *dst = reinterpret_cast<uint4 *>(query ? out_q + h * p.d : out_k + (int64_t)(h - p.hq) * head_step);
+      uint4 *dst = reinterpret_cast<uint4 *>(query ? out_q + h * p.d : out_k + (h - p.hq) * head_step);
       if (has_a) dst[va] = pack16(x[0], kType);
       if (has_b) dst[vb] = pack16(x[1], kType);
     }
@@ -503,6 +503,8 @@ int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld
   if (rows == 0) return AXB200_OK;
   if ((hq > 0 && (!q || !q_out)) || (hkv > 0 && (!k || !k_out)) || (rot_dim > 0 && (!pos || !inv_freq))) return AXB200_INVALID_PTR;
   if ((hq > 0 && q_ld < (int64_t)hq * d) || (hkv > 0 && k_ld < (int64_t)hkv * d)) return AXB200_SHAPE_MISMATCH;
+  // in place where rows are contiguous: a head's threads have read it before they write
+  if ((hq > 0 && q == q_out && q_ld != (int64_t)hq * d) || (hkv > 0 && k == k_out && k_ld != (int64_t)hkv * d)) return AXB200_SHAPE_MISMATCH;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, false>(p, nullptr, st)
          : dtype == AXB200_FLOAT16 ? axb::launch_turn<__half, false>(p, nullptr, st)
@@ -522,7 +524,8 @@ int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void
                     hq, hkv, d, k_pages, v_pages, block_table, seq_lens, row_start, batch, page_tokens, max_blocks, num_pages,
                     advance != 0};
   if (!axb::turn_sizes_ok(p) || hq == 0 || hkv == 0 || rot_dim < 0 || rot_dim % 2 || rot_dim > d || h_sec < 0 || w_sec < 0 || batch <= 0 ||
-      page_tokens <= 0 || page_tokens % 64 || max_blocks <= 0 || num_pages <= 0)
+      page_tokens <= 0 || page_tokens % 64 || max_blocks <= 0 || num_pages <= 0 || (int64_t)max_blocks * page_tokens > 0x7fffffff - 4096 ||
+      (qkv && qkv == q_out))
     return AXB200_INVALID_ARGUMENT;
   if (rows == 0) return AXB200_OK;
   if (!qkv || !q_out || !k_pages || !v_pages || !block_table || !seq_lens || !row_start || (rot_dim > 0 && !inv_freq))

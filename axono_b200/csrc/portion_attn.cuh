@@ -207,9 +207,11 @@ __device__ __forceinline__ float4 load4(const __half *p) {
 
 // A warp does one row of a block over - its keys from key0 to key1 - as the definition has it, with fp32 multiplications and only the keys
 // that the row sees: what the tensor-core kernels cannot finish (a weight of zero times an infinite value, values without exact parts).
-// Scores with lane = key, sums with lane = four columns.  d: a multiple of 4 up to 128.
+// Scores with lane = key, sums with lane = four columns.  d: a multiple of 4 up to 128.  lift: weights are 2^lift times what they are, as
+// in the parts that this one is joined with.
 template <typename T>
-__device__ __noinline__ void redo_portion_row(const PortionParams &p, const PortionBlock &block, int token, int head, int key0, int key1) {
+__device__ __noinline__ void redo_portion_row(const PortionParams &p, const PortionBlock &block, int token, int head, int key0, int key1,
+                                              float lift) {
   const int lane = threadIdx.x & 31, hk = head / p.group, row = block.row0 + token, pos = block.first_pos + token;
   key1 = min(key1, min(pos + 1, block.key_limit));
   if (p.window) key0 = max(key0, pos + 1 - p.window);
@@ -236,7 +238,7 @@ __device__ __noinline__ void redo_portion_row(const PortionParams &p, const Port
     float m_new = fmaxf(m, s);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, off));
-    const float shift = m_new == -INFINITY ? 0.f : m_new, corr = exp2f(m - shift), w = key < key1 ? exp2f(s - shift) : 0.f;
+    const float shift = m_new == -INFINITY ? 0.f : m_new, corr = exp2f(m - shift), w = key < key1 ? exp2f(s - shift + lift) : 0.f;
     m = m_new;
     l = l * corr + warp_sum(w);
     acc.x *= corr, acc.y *= corr, acc.z *= corr, acc.w *= corr;

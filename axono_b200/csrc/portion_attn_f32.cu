@@ -399,7 +399,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   if (*bad_flag && !*abort_flag)
     for (int r = warp; r < block.rows * p.group; r += kThreads / 32)
-      redo_portion_row<float>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
+      redo_portion_row<float>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN, 0.f);
 }
 
 template <int kB>

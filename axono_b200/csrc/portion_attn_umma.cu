@@ -35,7 +35,10 @@ constexpr int kKStages = 3, kVStages = 2;
 constexpr int kOffK = kQBytes, kOffV = kOffK + kKStages * kTileBytes, kOffBar = kOffV + kVStages * kTileBytes;
 constexpr int kOffPages = kOffBar + 160, kPageRing = 64, kOffSearch = kOffPages + kPageRing * 4;
 constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
-constexpr float kLazyLog2 = 8.0f;
+// The running maximum moves only for scores more than 2^kLazyLog2 above it, and weights are 2^kLift times what they are: at most 2^15, which
+// fp16 holds, and normal numbers down to 2^-21 of the largest, where they would be subnormal from 2^-14 on (what is
+// left out below is 2^-32).
+constexpr float kLazyLog2 = 8.0f, kLift = 7.0f;
 constexpr int kOffMl = kM * (kD + 4) * 4;  // of a cluster's part: (maximum, denominator) behind its sums, both where tiles were
 
 // A peer's shared memory in the cluster.
@@ -94,7 +97,7 @@ __device__ __forceinline__ void join_cluster(const PortionParams &p, const Porti
           make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
     __syncwarp();  // other lanes write such a row anew
     if (__any_sync(0xffffffffu, bad != 0.f && lane * 4 < p.d))
-      redo_portion_row<__half>(p, block, token, head, block.tile0 * kN, (block.tile0 + block.tiles) * kN);
+      redo_portion_row<__half>(p, block, token, head, block.tile0 * kN, (block.tile0 + block.tiles) * kN, kLift);
   }
 }
 
@@ -300,7 +303,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         m_run = m_new;
       }
       const float m_safe = m_run == -INFINITY ? 0.f : m_run;
-      const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), shift2 = pack_f32x2(-m_safe, -m_safe);
+      const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), shift2 = pack_f32x2(kLift - m_safe, kLift - m_safe);
       uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -401,7 +404,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const unsigned again = __ballot_sync(0xffffffffu, there && bad != 0.f);
       for (unsigned left = again; left; left &= left - 1) {
         const int r = warp * 32 + __ffs(left) - 1;
-        redo_portion_row<__half>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN);
+        redo_portion_row<__half>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN, kLift);
       }
     }
   }

@@ -419,11 +419,11 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *     product), to contiguous q_out and k_out; q_out may be q where its rows are contiguous, likewise k.  hq or hkv may be 0.  FLOAT16,
  *     BFLOAT16, FLOAT32.
  *   qkv_norm_rope_append_portions: qkv (rows, ld) holds per row hq query heads, hkv key heads, hkv value heads; the turned queries go to
- *     q_out (rows, hq, d), keys and values into the pages: with `advance` (the first layer of a step) behind the seq_lens[b] cached
+ *     q_out (rows, hq, d; apart from qkv), keys and values into the pages: with `advance` (the first layer of a step) behind the seq_lens[b] cached
  *     tokens, whose number then grows by the portion; else (later layers) into the last slots of seq_lens[b], which counts them already.
  *     pos NULL: a row's position is its slot.  A portion that does not fit sets AXB200_ERR_CAPACITY, nothing of it is appended and its
  *     length stays; a page outside the pool sets AXB200_ERR_BAD_PAGE, its rows are not written and the length stays.  FLOAT16, FLOAT32.
- *   gqa_attention_portions_paged: q, out (rows, hq, d): row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
+ *   gqa_attention_portions_paged: q, out (rows, hq, d), which do not overlap: row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
  *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
  *     counts the portion.  A row that sees no key gets zeros; keys and values that a row does not see, and what stands behind a sequence's
  *     end, do not touch it whatever they are.  Rows whose result is not finite, and in FLOAT32 blocks with values that are not finite,

@@ -74,7 +74,8 @@ class Cache:
 
 def attend(q, k, v, start, window=0):
     """Rows q (n, hq, d) at positions start.. over k, v (len, hkv, d): the result, and sum of weight * |value| (which errors of the
-    weights scale with) and the largest |score|."""
+    weights scale with; each weight at least 2^-21 of the largest possible, 1, below which an fp16 weight is subnormal and off by 2^-32)
+    and the largest |score|."""
     n, hq, d = q.shape
     group = hq // k.shape[1]
     out, mag, top = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device), 0.0
@@ -90,9 +91,9 @@ def attend(q, k, v, start, window=0):
         if hidden.any():  # 0 * inf: the sum over what a row sees
             for i, r in enumerate(some.nonzero()[:, 0].tolist()):
                 out[r, h] = w[i][seen[r]] @ vh[seen[r]]
-                mag[r, h] = w[i][seen[r]] @ vh[seen[r]].abs()
+                mag[r, h] = (w[i][seen[r]] + 2.0 ** -21) @ vh[seen[r]].abs()
         else:
-            out[some, h], mag[some, h] = w @ vh, w @ vh.abs()
+            out[some, h], mag[some, h] = w @ vh, (w + 2.0 ** -21 * seen[some]) @ vh.abs()
         if some.any():
             top = max(top, float(s[some][seen[some]].abs().max()))
     return out, mag, top
@@ -111,7 +112,9 @@ def attend_all(q, cache, counts, starts, window=0):
 
 def attend_tolerance(dtype, ref, mag, top):
     """The result's rounding; scores in fp32, off by 2^-21 of the largest, and an exponential by 2^-21, which change a weight by as
-    much; and in fp16 the weights' own rounding (half a step, 2^-11) before they meet the values."""
+    much; and in fp16 the weights' own rounding (half a step, 2^-11) before they meet the values.  A result below the smallest normal
+    number is rounded to a multiple of that number times eps, so that half of this is added."""
     half = torch.finfo(dtype).eps / 2
+    subnormal = torch.finfo(dtype).smallest_normal * half
     weights = 2.0 ** -21 * (2 + 2 * top) + (2.0 ** -11 if dtype == torch.float16 else 0.0)
-    return ref.abs() * half * (1 + 2.0 ** -10) + mag * weights
+    return ref.abs() * half * (1 + 2.0 ** -10) + mag * weights + subnormal

@@ -436,6 +436,85 @@ def test_other_streams_graphs_and_two_calls_at_once():
     assert ops.last_error() == 0
 
 
+def test_turn_in_place():
+    """Through the C ABI, whose outputs may be its inputs where rows are contiguous."""
+    from axono_b200 import _capi, ops
+
+    for dtype, d, rot, interleaved in ((torch.float16, 128, 128, False), (torch.float32, 80, 40, True), (torch.float16, 20, 20, False)):
+        q, k, w = rnd((300, 6, d), dtype, 1), rnd((300, 2, d), dtype, 2), 1 + rnd((d,), dtype, 3, 0.1)
+        pos, f = torch.arange(300, device="cuda") * 7, freqs(rot)
+        oq, ok = ops.qk_norm_rope(q, k, pos, f, w, w, EPS, interleaved)
+        code = _capi.FLOAT16 if dtype == torch.float16 else _capi.FLOAT32
+        assert _capi.lib().axb200_qk_norm_rope(q.data_ptr(), 6 * d, k.data_ptr(), 2 * d, w.data_ptr(), w.data_ptr(), EPS, pos.data_ptr(),
+                                               f.data_ptr(), rot, int(interleaved), 1.0, 0, 0, 0, q.data_ptr(), k.data_ptr(), 300, 6, 2, d,
+                                               code, torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(q, oq) and torch.equal(k, ok)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_attention_of_many_sequences(dtype):
+    """More sequences than a CTA has threads, most of them with nothing new, some long."""
+    from axono_b200 import ops
+
+    g = torch.Generator().manual_seed(3)
+    for batch, most in ((500, 2), (900, 1)):
+        counts = [int(n) if i % 5 else 0 for i, n in enumerate(torch.randint(0, most + 1, (batch,), generator=g))]
+        cached = [int(n) for n in torch.randint(0, 90, (batch,), generator=g)]
+        cached[7], cached[batch - 2], counts[batch - 2] = 3000, 2000, 1
+        q, cache, starts, out = run_attention(counts, cached, 4, 2, 64, dtype, first=2, behind=2)
+        check_attention(q, cache, counts, starts, out)
+    counts, cached = [0] * 400, [1] * 400
+    counts[350], cached[350] = 3, 4000
+    q, cache, starts, out = run_attention(counts, cached, 4, 2, 128, dtype)
+    check_attention(q, cache, counts, starts, out)
+    assert ops.last_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_attention_takes_any_alignment(dtype):
+    """Queries and outputs that start off 16 bytes go through the FMA kernel, long caches in parts."""
+    from axono_b200 import ops
+
+    counts, lens = (3, 40), (2500, 60)
+    cache, starts = Cache(lens, 2, 64, dtype), row_table(counts)
+    q = rnd((43, 4, 64), dtype, 5)
+    buf, obuf = torch.empty(q.numel() + 1, dtype=dtype, device="cuda"), torch.empty(q.numel() + 1, dtype=dtype, device="cuda")
+    shifted, out = buf[1:].view(q.shape), obuf[1:].view(q.shape)
+    shifted.copy_(q)
+    for a, b in ((shifted, None), (q, out), (shifted, out)):
+        got = ops.gqa_attention_portions_paged(a, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, 2500, out=b)
+        check_attention(q, cache, counts, starts.tolist(), got)
+    assert ops.last_error() == 0
+    with pytest.raises(RuntimeError):
+        ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, 2500, out=q)
+
+
+@pytest.mark.parametrize("what,scale", [("v", 1e-36), ("k", 1e-36), ("q", 1e-34), ("v", 1e36), ("v", 0.0)])
+def test_fp32_attention_of_values_without_exact_parts(what, scale):
+    """Values below 2^-100, whose lower bf16 parts would be subnormal, and large ones; a single such value is enough."""
+    from axono_b200 import ops
+
+    counts, lens = (70, 2), (300, 2500)
+    cache, starts = Cache(lens, 2, 64, torch.float32), row_table(counts)
+    q = rnd((72, 4, 64), torch.float32, 5)
+    for some in (True, False):
+        for b, n in enumerate(lens):
+            at = slice(n // 3, n // 3 + 1) if some else slice(0, n)
+            x = {"k": cache.k, "v": cache.v, "q": cache.k}[what][b]
+            if what != "q":
+                x[at] *= scale
+                cache.write(b, 0, cache.k[b], cache.v[b])
+        if what == "q":
+            q[1 if some else slice(None)] *= scale
+        out = ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, 2500)
+        for rows, ref, mag, top in attend_all(q, cache, counts, starts.tolist()):
+            err = (out[rows].double() - ref).abs()
+            tol = attend_tolerance(torch.float32, ref, mag, top) + 2.0 ** -149  # a subnormal result's own step
+            # (1e36 twice is infinite: that key's value, and every result it joins)
+            assert ((err <= tol) | (out[rows].double() == ref)).all(), (some, float((err / tol).max()))
+    assert ops.last_error() == 0
+
+
 # ---- in the tower ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("use_mrope,qk_norm,dtype", [(True, True, torch.float16), (False, False, torch.float16), (False, True, torch.float32)])

@@ -11,14 +11,14 @@ FAKE = 1 << 20  # an address that nothing follows: every call here is refused on
 
 
 def turn(**kw):
-    a = dict(q=FAKE, q_ld=256, k=FAKE, k_ld=128, qw=None, kw=None, eps=1e-6, pos=FAKE, freq=FAKE, rot=64, inter=0, factor=1.0, mrope=0, h=0,
-             w=0, qo=FAKE, ko=FAKE, rows=4, hq=4, hkv=2, d=64, dtype=_capi.FLOAT16, stream=None)
+    a = dict(q=FAKE, q_ld=256, k=FAKE + 64, k_ld=128, qw=None, kw=None, eps=1e-6, pos=FAKE, freq=FAKE, rot=64, inter=0, factor=1.0, mrope=0, h=0,
+             w=0, qo=FAKE, ko=FAKE + 4096, rows=4, hq=4, hkv=2, d=64, dtype=_capi.FLOAT16, stream=None)
     a.update(kw)
     return _capi.lib().axb200_qk_norm_rope(*a.values())
 
 
 def append(**kw):
-    a = dict(qkv=FAKE, ld=512, qw=None, kw=None, eps=1e-6, qo=FAKE, k=FAKE, v=FAKE, table=FAKE, lens=FAKE, start=FAKE, pos=None, freq=FAKE, rot=64,
+    a = dict(qkv=FAKE, ld=512, qw=None, kw=None, eps=1e-6, qo=FAKE + 4096, k=FAKE, v=FAKE, table=FAKE, lens=FAKE, start=FAKE, pos=None, freq=FAKE, rot=64,
              inter=0, factor=1.0, mrope=0, h=0, w=0, rows=4, batch=2, hq=4, hkv=2, d=64, page=64, blocks=4, pages=8, dtype=_capi.FLOAT16,
              advance=1, stream=None)
     a.update(kw)
@@ -26,7 +26,7 @@ def append(**kw):
 
 
 def attend(**kw):
-    a = dict(q=FAKE, out=FAKE, k=FAKE, v=FAKE, table=FAKE, lens=FAKE, start=FAKE, rows=4, batch=2, hq=4, hkv=2, d=64, page=64, blocks=4, pages=8,
+    a = dict(q=FAKE, out=FAKE + 4096, k=FAKE, v=FAKE, table=FAKE, lens=FAKE, start=FAKE, rows=4, batch=2, hq=4, hkv=2, d=64, page=64, blocks=4, pages=8,
              max_len=200, window=0, dtype=_capi.FLOAT16, ws=FAKE, bytes=1 << 40, stream=None)
     a.update(kw)
     return _capi.lib().axb200_gqa_attention_portions_paged(*a.values())
@@ -39,7 +39,7 @@ def test_turn_refuses():
     for kw, status in ((dict(dtype=_capi.INT32), TYPE), (dict(rot=3), INVALID), (dict(rot=66), INVALID), (dict(rot=-2), INVALID),
                        (dict(d=257), INVALID), (dict(d=0), INVALID), (dict(rows=-1), INVALID), (dict(hq=0, hkv=0), INVALID),
                        (dict(q=None), POINTER), (dict(ko=None), POINTER), (dict(pos=None), POINTER), (dict(freq=None), POINTER),
-                       (dict(q_ld=255), SHAPE), (dict(k_ld=127), SHAPE), (dict(rows=0), 0), (dict(h=-1), INVALID)):
+                       (dict(q_ld=255), SHAPE), (dict(k_ld=127), SHAPE), (dict(q_ld=300), SHAPE), (dict(rows=0), 0), (dict(h=-1), INVALID)):
         assert turn(**kw) == status, kw
 
 
@@ -47,14 +47,15 @@ def test_append_refuses():
     for kw, status in ((dict(dtype=_capi.BFLOAT16), TYPE), (dict(rot=65), INVALID), (dict(batch=0), INVALID), (dict(page=32), INVALID),
                        (dict(page=0), INVALID), (dict(blocks=0), INVALID), (dict(pages=0), INVALID), (dict(hkv=0), INVALID),
                        (dict(hq=0), INVALID), (dict(ld=511), SHAPE), (dict(start=None), POINTER), (dict(lens=None), POINTER),
-                       (dict(freq=None), POINTER), (dict(qkv=None), POINTER), (dict(d=300, rot=0), INVALID), (dict(rows=0), 0)):
+                       (dict(freq=None), POINTER), (dict(qkv=None), POINTER), (dict(d=300, rot=0), INVALID), (dict(qo=FAKE), INVALID),
+                       (dict(blocks=1 << 26), INVALID), (dict(rows=0), 0)):
         assert append(**kw) == status, kw
 
 
 def test_attention_refuses():
     for kw, status in ((dict(dtype=_capi.BFLOAT16), TYPE), (dict(d=257), INVALID), (dict(hkv=3), SHAPE), (dict(page=96), INVALID),
                        (dict(max_len=0), INVALID), (dict(max_len=1 << 31), INVALID), (dict(window=-1), INVALID), (dict(batch=0), INVALID),
-                       (dict(rows=-1), INVALID), (dict(out=None), POINTER), (dict(table=None), POINTER), (dict(rows=0), 0),
+                       (dict(rows=-1), INVALID), (dict(out=None), POINTER), (dict(out=FAKE), INVALID), (dict(table=None), POINTER), (dict(rows=0), 0),
                        (dict(blocks=1 << 26), INVALID), (dict(max_len=1 << 20, blocks=1 << 14, ws=None), MEMORY),
                        (dict(max_len=1 << 20, blocks=1 << 14, bytes=16), MEMORY), (dict(max_len=1 << 20, blocks=1 << 14, ws=FAKE + 4), POINTER)):
         assert attend(**kw) == status, kw
