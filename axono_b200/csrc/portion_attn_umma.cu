@@ -17,7 +17,8 @@
 // Bound by the latency of a tile's chain - scores, softmax, weights - on two CTAs: 2368 rows over 14000 tokens, 16 / 8 heads of 128, 263 us
 // (1110 TFLOP/s), 1050 cycles of an SM per tile where the products take 660 and the exponentials 510; heads of 64: 211 us.  Tried, not
 // kept: three stages of V and two of K (drafts 118 -> 124 us), four of each with one CTA per SM (161), up to 32 rows four times in the block
-// with a quarter of a tile's keys for each warp (no change: few rows wait for memory or for the chain around the softmax, not in it).
+// with a quarter of a tile's keys for each warp (no change), a third buffer of S for heads of 64 (no change), the next tile's scores asked
+// for before this one's weights are handed over (211 -> 223: a slow warp's weights hold up the others').
 #include <math.h>
 
 #include <mutex>
