@@ -117,12 +117,13 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
       v += search->totals[1][w];
       most = fmaxf(most, search->totals[2][w]);
     }
-    const float share = v / p.at_once, joining = p.join_cost + 0.12f;
+    const float share = v / p.at_once;
     float best = n <= p.at_once ? most + p.part_cost : share + n / p.at_once * p.part_cost + 0.5f * most;
     const auto consider = [&](float length, bool rounds) {
       length = fmaxf(ceilf(fmaxf(length, v * 1.001f / (p.units - n))), 1.f);
       const float parts = v / length + n;
-      const float time = (rounds ? share + parts / p.at_once * p.part_cost + 0.5f * length : length + p.part_cost) + joining + 0.12f * most / length;
+      const float time = (rounds ? share + parts / p.at_once * p.part_cost + 0.5f * length : length + p.part_cost) + p.join_cost +
+                         0.12f * (1.f + most / length);
       if (length < most && time < best) best = time, part_tiles = fminf((float)kPortionMostTiles, length);
     };
     if (n < p.units && n < p.at_once) consider(fmaxf(v * 1.001f / (p.at_once - n), sqrtf(0.12f * most)), false);
@@ -172,6 +173,7 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
     if (s_found || before > index) break;
   }
   block = search->block;
+  block.rows = min(block.rows, p.rows - block.row0);  // whatever a table that does not count up has led to
   return s_found && block.part < block.parts;
 }
 

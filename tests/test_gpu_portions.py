@@ -515,6 +515,42 @@ def test_fp32_attention_of_values_without_exact_parts(what, scale):
     assert ops.last_error() == 0
 
 
+def test_a_replayed_step_follows_the_growing_cache():
+    """Single tokens as portions, captured once: every replay appends behind what the last one left, over the edges of tiles and pages,
+    with the bits of eager calls."""
+    from axono_b200 import ops
+
+    hq, hkv, d, steps = 4, 2, 64, 70
+    for lens, bound in (((30, 100, 0), 256), ((60, 4000, 900), 4200)):  # clusters, and parts
+        caches = [Cache(lens, hkv, d, torch.float16, more=steps, poison=0.0) for _ in range(2)]
+        starts, f = row_table([1, 1, 1]), freqs(d)
+        qkv = torch.empty((3, (hq + 2 * hkv) * d), dtype=torch.float16, device="cuda")
+        out = torch.empty((3, hq, d), dtype=torch.float16, device="cuda")
+
+        def step(c, out=None):
+            q = ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, c.k_pages, c.v_pages, c.table, c.lens, starts, inv_freq=f)
+            return ops.gqa_attention_portions_paged(q, c.k_pages, c.v_pages, c.table, c.lens, starts, bound, out=out)
+
+        qkv.zero_()
+        first = caches[0].lens.clone()
+        step(caches[0], out)  # once before the capture, taken back
+        caches[0].lens.copy_(first)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(caches[0], out)
+        for i in range(steps):
+            qkv.copy_(rnd(qkv.shape, torch.float16, i))
+            graph.replay()
+            assert torch.equal(out, step(caches[1])), i
+        assert caches[0].lens.tolist() == [n + steps for n in lens] and torch.equal(caches[0].lens, caches[1].lens)
+        assert torch.equal(caches[0].k_pages, caches[1].k_pages) and torch.equal(caches[0].v_pages, caches[1].v_pages)
+        for b in range(3):
+            caches[1].k[b], caches[1].v[b] = caches[1].read(b, 0, lens[b] + steps)
+        q = ops.qk_norm_rope(qkv[:, :hq * d].view(3, hq, d), None, caches[1].lens.long() - 1, f)[0]
+        check_attention(q, caches[1], (1, 1, 1), [0, 1, 2, 3], out)
+    assert ops.last_error() == 0
+
+
 # ---- in the tower ---------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("use_mrope,qk_norm,dtype", [(True, True, torch.float16), (False, False, torch.float16), (False, True, torch.float32)])
