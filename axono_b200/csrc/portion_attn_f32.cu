@@ -88,9 +88,10 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   uint64_t *bar_p = bars + 10;                         // P_j and its rescale factor written, per parity
   uint64_t *bar_c = bars + 12;                         // O_j added up, per parity
   uint64_t *bar_q = bars + 14, *bar_l = bars + 15;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 17);
-  volatile int *bad_flag = reinterpret_cast<volatile int *>(bars + 18);
+  uint64_t *bar_m = bars + 16;                         // the products of P_j . V_j done that read the place of S_{j+2}
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 17);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 18);
+  volatile int *bad_flag = reinterpret_cast<volatile int *>(bars + 19);
   int *pages = reinterpret_cast<int *>(smem + L::kOffPages);
   float *corr_s = reinterpret_cast<float *>(smem + L::kOffCorr), *l_s = reinterpret_cast<float *>(smem + L::kOffL);
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -116,6 +117,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int i = 0; i < kKBufs; ++i) mbar_init(&full_k[i], kHelpers);
     mbar_init(full_v, kHelpers);
     mbar_init(bar_o, 1);
+    mbar_init(bar_m, 1);
     for (int i = 0; i < 2; ++i) mbar_init(&bar_s[i], 1), mbar_init(&bar_p[i], active), mbar_init(&bar_c[i], 2 * active);
     mbar_init(bar_q, 2 * active);
     mbar_init(bar_l, active);
@@ -176,7 +178,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int d_steps = (p.d + 15) / 16;
     const uint32_t idesc_qk = bf16 | ((kN >> 3) << 17), idesc_pv = bf16 | (1u << 16) | ((uint32_t)(d_steps * 2) << 17);
     const uint64_t dk = smem_desc(smem_u32(smem + L::kOffK), 16, 1024), dv = smem_desc(smem_u32(smem + L::kOffV), kBox, 1024);
-    constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kC[6] = {2, 0, 1, 1, 0, 0};  // parts of A and B, smallest products first
+    // parts of A and B, smallest products first; of P.V those of the lower parts of P, then those of its highest, which stands beside S
+    constexpr int kA[6] = {0, 2, 1, 0, 1, 0}, kC[6] = {2, 0, 1, 1, 0, 0}, kPa[6] = {2, 1, 1, 0, 0, 0}, kPc[6] = {0, 1, 0, 2, 1, 0};
     // round i: P_{i-2}.V_{i-2}, then S_i in its place, with one copy of each in the instruction cache
     bool ok = nkv > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.wait_ns);
 #pragma unroll 1
@@ -190,15 +193,17 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int c = 0; c < 6; ++c)
+          for (int c = 0; c < 6; ++c) {
+            if (c == 3) umma_commit(bar_m);
 #pragma unroll
             for (int ks = 0; ks < kN / 16; ++ks)
-              umma_f16_ts(tmem_o, tmem_sp + s * L::kSpCols + kA[c] * 32 + ks * 8, dv + (uint64_t)((kC[c] * L::kPart + ks * 2048) >> 4),
+              umma_f16_ts(tmem_o, tmem_sp + s * L::kSpCols + kPa[c] * 32 + ks * 8, dv + (uint64_t)((kPc[c] * L::kPart + ks * 2048) >> 4),
                           idesc_pv, c > 0 || ks > 0);
+          }
           umma_commit(bar_o);
         }
         if (i >= nkv) continue;
-        ok = mbar_wait_warp(bar_o, j & 1, abort_flag, p.wait_ns);  // S_i takes the place of P_{i-2}
+        ok = mbar_wait_warp(bar_m, j & 1, abort_flag, p.wait_ns);  // S_i takes the place of P_j's lower parts
         if (!ok) break;
       }
       if (i >= nkv) continue;
@@ -212,7 +217,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 #pragma unroll
           for (int ks = 0; ks < 4 * kB; ++ks) {
             if (ks >= d_steps) break;
-            umma_f16_ts(tmem_sp + s * L::kSpCols, tmem + kA[c] * 32 * kB + ks * 8,
+            umma_f16_ts(tmem_sp + s * L::kSpCols + 32, tmem + kA[c] * 32 * kB + ks * 8,
                         dks + (uint64_t)((kC[c] * L::kPart + (ks >> 2) * kBox + (ks & 3) * 32) >> 4), idesc_qk, c > 0 || ks > 0);
           }
         umma_commit(&bar_s[s]);
@@ -230,8 +235,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         tc_fence_after();
         const uint32_t sp = tmem_sp + s * L::kSpCols + lane_base;
         uint32_t sr[2][32];
-        tmem_ld32_async(sp, sr[0]);
-        tmem_ld32_async(sp + 32, sr[1]);
+        tmem_ld32_async(sp + 32, sr[0]);
+        tmem_ld32_async(sp + 64, sr[1]);
         tmem_wait_ld();
         const int n0 = (tile0 + j) * kN;
         if (n0 + kN > key_end || n0 < key_begin) {
@@ -245,6 +250,10 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const float corr = fast_exp2((m_run - m_safe) * p.scale_log2);  // 0 at the first tile
         m_run = m_new;
         const uint64_t shift2 = pack_f32x2(-m_safe, -m_safe);
+        if (j >= 2) {  // O_{j-2} is added up: its weights and its factor have been read
+          ok = mbar_wait_warp(&bar_c[s], ((j >> 1) - 1) & 1, abort_flag, p.wait_ns);
+          if (!ok) break;
+        }
         uint64_t sum2[4] = {0, 0, 0, 0}, unused = 0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -262,10 +271,6 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         const float2 sum = unpack_f32x2(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])));
         l_run = l_run * corr + (sum.x + sum.y);
-        if (j >= 2) {  // the factor of tile j - 2 has been read
-          ok = mbar_wait_warp(&bar_c[s], ((j >> 1) - 1) & 1, abort_flag, p.wait_ns);
-          if (!ok) break;
-        }
         corr_s[s * kM + vrow] = corr;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
