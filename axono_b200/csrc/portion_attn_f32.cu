@@ -358,19 +358,31 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       const int c = lane % (16 * kB), row0 = kB == 1 ? lane >> 4 : 0;
       uint8_t *dst0 = parts_at + (c >> 4) * kBox + (helper * 8 + row0) * 128 + (c & 1) * 8;
       const int chunk = (c & 15) >> 1;
-#pragma unroll 4
-      for (int i = 0; i < 4 * kB; ++i) {
-        const int r = i * (2 / kB);  // row0 + r is the row among the warp's eight
-        float4 x = src[i * 32];
-        if (!whole && helper * 8 + row0 + r >= left) x = make_float4(0.f, 0.f, 0.f, 0.f);
-        range.see(x.x), range.see(x.y), range.see(x.z), range.see(x.w);
-        uint2 h, m, l;
-        split3(x.x, x.y, h.x, m.x, l.x, range.check);
-        split3(x.z, x.w, h.y, m.y, l.y, range.check);
-        uint8_t *dst = dst0 + r * 128 + ((chunk ^ (row0 + r)) << 4);
-        *reinterpret_cast<uint2 *>(dst) = h;
-        *reinterpret_cast<uint2 *>(dst + L::kPart) = m;
-        *reinterpret_cast<uint2 *>(dst + 2 * L::kPart) = l;
+      // four pieces at a time, loaded and split before the first is stored (the compiler keeps loads behind stores that may alias)
+#pragma unroll 1
+      for (int base = 0; base < 4 * kB; base += 4) {
+        float4 x[4];
+        uint2 h[4], m[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (base + i) * (2 / kB);  // row0 + r is the row among the warp's eight
+          x[i] = src[(base + i) * 32];
+          if (!whole && helper * 8 + row0 + r >= left) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          range.see(x[i].x), range.see(x[i].y), range.see(x[i].z), range.see(x[i].w);
+          split3(x[i].x, x[i].y, h[i].x, m[i].x, l[i].x, range.check);
+          split3(x[i].z, x[i].w, h[i].y, m[i].y, l[i].y, range.check);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (base + i) * (2 / kB);
+          uint8_t *dst = dst0 + r * 128 + ((chunk ^ (row0 + r)) << 4);
+          *reinterpret_cast<uint2 *>(dst) = h[i];
+          *reinterpret_cast<uint2 *>(dst + L::kPart) = m[i];
+          *reinterpret_cast<uint2 *>(dst + 2 * L::kPart) = l[i];
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
