@@ -56,15 +56,22 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t &h, uint32_t &
   l = pack_bf16x2(s.x, s.y);
 }
 
-// What has no three parts among the values seen: not finite ones by `check` above, and by the smallest magnitude, zero aside, those
-// below 2^-100.
+// What has no three parts among the values seen: not finite ones by `check` above; and those below 2^-100, zero aside, which 2^-26 makes
+// subnormal and so zero: what comes back from that differs, and leaves its bits.  (On the FMA pipe, whose turn it is: the integer
+// operations of the splitting take 22 of a scheduler's cycles per pair, its multiplications 6.)
 struct Range {
   uint64_t check = 0;
-  uint32_t least = 0xffffffffu;  // of twice the bits of a magnitude, less one
-  __device__ __forceinline__ void see(float x) { least = __viaddmin_u32(__float_as_uint(x) << 1, 0xffffffffu, least); }
+  uint32_t small = 0;
+  __device__ __forceinline__ void see(float a, float b) {
+    const uint64_t x = pack_f32x2(a, b);
+    uint64_t down;
+    asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(down) : "l"(x), "l"(pack_f32x2(0x1p-26f, 0x1p-26f)));
+    const float2 lost = unpack_f32x2(fma_f32x2(down, pack_f32x2(-0x1p26f, -0x1p26f), x));
+    small |= __float_as_uint(lost.x) | __float_as_uint(lost.y);
+  }
   __device__ __forceinline__ bool unsplittable() const {
     const float2 c = unpack_f32x2(check);
-    return !(c.x == 0.f && c.y == 0.f) || least < (27u << 24) - 1u;
+    return !(c.x == 0.f && c.y == 0.f) || small != 0;
   }
 };
 
@@ -296,7 +303,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         for (int u = 0; u < 8; ++u) {
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (there && half * 32 * kB + c * 32 + u * 4 < p.d) x = *reinterpret_cast<const float4 *>(src + c * 32 + u * 4);
-          range.see(x.x), range.see(x.y), range.see(x.z), range.see(x.w);
+          range.see(x.x, x.y), range.see(x.z, x.w);
           split3(x.x, x.y, parts[0][2 * u], parts[1][2 * u], parts[2][2 * u], range.check);
           split3(x.z, x.w, parts[0][2 * u + 1], parts[1][2 * u + 1], parts[2][2 * u + 1], range.check);
         }
@@ -371,7 +378,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          range.see(x[i].x), range.see(x[i].y), range.see(x[i].z), range.see(x[i].w);
+          range.see(x[i].x, x[i].y), range.see(x[i].z, x[i].w);
           split3(x[i].x, x[i].y, h[i].x, m[i].x, l[i].x, range.check);
           split3(x[i].z, x[i].w, h[i].y, m[i].y, l[i].y, range.check);
         }
