@@ -170,16 +170,11 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" {
 
 size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
-                                                     int64_t max_seq_len, int window, int dtype) {
+                                                     int64_t max_seq_len, int window, int aligned, int dtype) {
   if (!axb::portion_sizes_ok(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window) || rows == 0 || hq % hkv) return 0;
-  const auto need = [&](bool tensor) {
-    axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, dtype, tensor);
-    return axb::portion_scratch(p, nullptr);
-  };
-  const size_t fma = need(false);
-  if (!axb::portion_tensor_sizes(hq / hkv, d, dtype)) return fma;
-  const size_t tensor = need(true);
-  return tensor > fma ? tensor : fma;  // which kernel serves a call depends on its addresses too
+  const bool tensor = aligned && axb::portion_tensor_sizes(hq / hkv, d, dtype);
+  axb::PortionParams p = axb::portion_params(rows, batch, hq, hkv, d, page_tokens, max_blocks, 1, max_seq_len, window, dtype, tensor);
+  return axb::portion_scratch(p, nullptr);
 }
 
 int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,

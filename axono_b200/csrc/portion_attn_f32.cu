@@ -11,10 +11,12 @@
 // Splitting in the kernel needs no scratch for a cache whose lengths the host does not know, and hides behind the products: a tile's
 // scores take 2400 cycles and its sums 1600.  K's parts have two buffers, V's one: V is split while the next scores are formed.
 //
-// Bound by the products and the waits between them: a tile takes 5100 cycles of the 4000 (heads of 128; 3070 of 2400, heads of 64); 922 rows
-// over 5686 keys, 16 / 8 heads of 128, 174 us, of which the longest block's 52 tiles are 150 while the even share is 34 tiles (the FMA
-// kernel: 2099).  Error against 64 bits 4.5e-7, of the plain form in fp32 1.2e-6.  Tried: one buffer for K's parts and four tiles of
-// floats (168 to 173, the same), cuts of the loops that all warps' code shares an instruction cache with (194 -> 168: kept).
+// Bound by the products - 4000 cycles of a tile's 5000 with heads of 128, 2400 of 2900 with heads of 64 - and by shared memory beside them,
+// which carries 416 KB of floats, parts and operands per tile, 3300 cycles.  922 rows over 5686 keys, 16 / 8 heads of 128: 162 us, of which
+// the longest block's 52 tiles are 140 while the even share is 34 tiles (the FMA kernel: 2099).  Error against 64 bits 4.5e-7, of the plain
+// form in fp32 1.2e-6.  What moved it: one copy of each loop, since all warps' code shares an instruction cache (194 -> 168 us), scores
+// beside the part of the weights that is read last (172.5 -> 170.6), four pieces split at a time (162.3).  Tried: one buffer for K's parts
+// and four tiles of floats (the same), the middle part by multiplications instead of conversions and masks (the same).
 //
 // Values that have no exact parts (infinities, NaN, values that round to infinity in bf16, below 2^-100) are noticed while splitting,
 // and the CTA does its rows over with plain multiplications (redo_portion_row).

@@ -17,6 +17,8 @@ binding allocates them (nanobind_module.cpp:1019).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _capi
@@ -834,6 +836,12 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _portions_workspace_bytes(*sizes) -> int:
+    """A function of sizes alone, and a ctypes call takes 1.3 us."""
+    return _capi.lib().axb200_gqa_attention_portions_workspace_bytes(*sizes)
+
+
 def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row_start, max_seq_len, window: int = 0, out=None):
     """Causal attention of portions over a paged cache that holds them: q (rows, hq, d), sequence b's rows row_start[b] ..
     row_start[b + 1] - 1 are the last of its seq_lens[b] tokens (`qkv_norm_rope_append_portions` has appended them); each attends the
@@ -858,12 +866,13 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
-    lib, blocks = _capi.lib(), block_table.shape[1]
-    need = lib.axb200_gqa_attention_portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, int(max_seq_len), int(window), dt)
+    blocks, q_at, out_at = block_table.shape[1], q.data_ptr(), out.data_ptr()
+    aligned = not (q_at | out_at | pages[0] | pages[1]) & 15
+    need = _portions_workspace_bytes(rows, batch, hq, hkv, d, page_tokens, blocks, int(max_seq_len), int(window), aligned, dt)
     ws = q.new_empty(need, dtype=torch.uint8) if need else None  # of this call alone: streams may overlap
-    _launched(lib.axb200_gqa_attention_portions_paged(
-        q.data_ptr(), out.data_ptr(), *pages, rows, batch, hq, hkv, d, page_tokens, blocks, num_pages, int(max_seq_len), int(window),
-        dt, ws.data_ptr() if need else None, need, _stream_now(device)), op)
+    _launched(_capi.lib().axb200_gqa_attention_portions_paged(
+        q_at, out_at, *pages, rows, batch, hq, hkv, d, page_tokens, blocks, num_pages, int(max_seq_len), int(window), dt,
+        ws.data_ptr() if need else None, need, _stream_now(device)), op)
     return out
 
 

@@ -429,7 +429,8 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *     end, do not touch it whatever they are.  Rows whose result is not finite, and in FLOAT32 blocks with values that are not finite,
  *     above 3.39e38 or, unless zero, below 2^-100, are computed a second time without the tensor cores, at that speed.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
  *     sets AXB200_ERR_CAPACITY and its keys beyond are not read.  FLOAT16, FLOAT32.  workspace: at least the bytes that
- *     portions_workspace_bytes gives for the same arguments (0: none), 16-byte aligned, of this call alone until its kernels are done. */
+ *     portions_workspace_bytes gives for the same arguments (0: none; aligned: q, out and the pages start on 16 bytes), itself 16-byte
+ *     aligned, of this call alone until its kernels are done. */
 int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld, const void *q_norm_w, const void *k_norm_w, float eps,
                         const int64_t *pos, const double *inv_freq, int rot_dim, int interleaved, float factor, int mrope, int h_sec,
                         int w_sec, void *q_out, void *k_out, int64_t rows, int hq, int hkv, int d, int dtype, void *stream);
@@ -440,7 +441,7 @@ int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void
                                          int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
                                          void *stream);
 size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
-                                                     int64_t max_seq_len, int window, int dtype);
+                                                     int64_t max_seq_len, int window, int aligned, int dtype);
 int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,
                                         const int32_t *seq_lens, const int32_t *row_start, int64_t rows, int batch, int hq, int hkv,
                                         int d, int page_tokens, int max_blocks, int num_pages, int64_t max_seq_len, int window,

@@ -63,7 +63,7 @@ def test_attention_refuses():
 
 def test_workspace_is_for_few_rows_over_many_keys():
     size = lambda rows, batch, max_len, hkv=8, window=0: _capi.lib().axb200_gqa_attention_portions_workspace_bytes(  # noqa: E731
-        rows, batch, 16, hkv, 128, 64, 1 << 14, max_len, window, _capi.FLOAT16)
+        rows, batch, 16, hkv, 128, 64, 1 << 14, max_len, window, 1, _capi.FLOAT16)
     assert size(8, 1, 32768) > 0
     assert size(8, 1, 64) == 0
     assert size(8, 1, 32768, window=64) == 0
@@ -118,6 +118,6 @@ def test_frequencies():
 
 def test_signatures_hold_what_the_header_declares():
     for name, args in (("axb200_qk_norm_rope", 23), ("axb200_qkv_norm_rope_append_portions", 30),
-                       ("axb200_gqa_attention_portions_workspace_bytes", 10), ("axb200_gqa_attention_portions_paged", 21)):
+                       ("axb200_gqa_attention_portions_workspace_bytes", 11), ("axb200_gqa_attention_portions_paged", 21)):
         assert len(_capi.SIGNATURES[name][1]) == args
     assert _capi.SIGNATURES["axb200_gqa_attention_portions_workspace_bytes"][0] is ctypes.c_size_t
