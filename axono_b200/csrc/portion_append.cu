@@ -459,6 +459,8 @@ int launch_lanes(const TurnParams &p, int32_t *seq_lens, bool &done, cudaStream_
     }
   }
   while (p.rows * ways < 148 * 16 && ways * 2 <= groups) ways *= 2;
+  const int share = (n_heads + ways - 1) / ways;
+  ways = (n_heads + share - 1) / share;  // none without a head: the copies ahead would take a round for it
   const int64_t blocks = (p.rows * ways + kRowThreads / 32 - 1) / (kRowThreads / 32), most = 148 * kRowBlocks;
   return launch_rows<T, kAppend, kLanes, false>(p, ways, (int)(blocks < most ? blocks : most), kRowThreads / 32, nullptr, st);
 }

@@ -637,3 +637,37 @@ def test_frequencies_of_the_single_token_operators():
     a = ops.rope(x, pos, 5e5)
     b, _ = ops.qk_norm_rope(x, None, pos, ops.reference_frequencies(128, 5e5))
     assert (a - b).abs().max() <= 2.0 ** -20 * x.abs().max()
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv,rows", [(torch.float32, 256, 60, 8, 60), (torch.float32, 128, 120, 10, 73), (torch.bfloat16, 256, 124, 5, 66),
+                                                 (torch.float32, 256, 193, 7, 33), (torch.float16, 128, 250, 7, 40)])
+def test_turn_of_many_heads(dtype, d, hq, hkv, rows):
+    """Heads of few rows are shared among warps, some of which take part of two rows."""
+    from axono_b200 import ops
+
+    q, k, (wq, wk) = rnd((rows, hq, d), dtype, 1), rnd((rows, hkv, d), dtype, 2), weights(d, dtype, True)
+    pos = torch.arange(rows, device="cuda") * 11
+    oq, ok = ops.qk_norm_rope(q, k, pos, freqs(d), wq, wk, EPS)
+    check_turn(oq, turn(q, wq, EPS, pos, freqs(d)))
+    check_turn(ok, turn(k, wk, EPS, pos, freqs(d)))
+    assert ops.last_error() == 0
+
+
+def test_append_of_many_heads():
+    from axono_b200 import ops
+
+    hq, hkv, d, counts, cached = 56, 6, 256, (35, 0, 25), (3, 5, 64)
+    cache = Cache(list(cached), hkv, d, torch.float32, more=40)
+    qkv, (wq, wk) = rnd((60, (hq + 2 * hkv) * d), torch.float32, 4), weights(d, torch.float32, True)
+    oq = ops.qkv_norm_rope_append_portions(qkv, hq, wq, wk, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table(counts),
+                                           inv_freq=freqs(d))
+    at = 0
+    for b, n in enumerate(counts):
+        q, k, v = qkv[at:at + n].view(n, hq + 2 * hkv, d).split([hq, hkv, hkv], 1)
+        pos = cached[b] + torch.arange(n, device="cuda")
+        ck, cv = cache.read(b, cached[b], n)
+        check_turn(oq[at:at + n], turn(q, wq, EPS, pos, freqs(d)))
+        check_turn(ck, turn(k, wk, EPS, pos, freqs(d)))
+        assert torch.equal(cv, v)
+        at += n
+    assert cache.lens.tolist() == [38, 5, 89] and ops.last_error() == 0
