@@ -92,8 +92,10 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // blocks that do not fill the GPU are divided into as many parts as run at once; blocks of few rows, which are bound by memory and cheap to
 // join, into parts that take some rounds.  Room in the grid that the lengths do not use costs time: three rounds of CTAs that find no work 18
 // us (8192 rows of a prompt 255 and 298 us), while 64 sequences of 16 K to 32 K tokens with a row each take 1087 us whole and 963 in parts.
-// Few blocks of few tiles are clusters (13 rows over 700 tokens: 11.5 us with a second launch that joins, 8.9 so; over 2000 14.3 and 11.5;
-// over 8000 they would be 16 tiles in a row, about 27 us, and are 21 in parts).
+// Few blocks of few tiles are clusters, of the size that takes least by what was measured, in tiles of 0.85 us: joining takes 1.6 and 0.024 per
+// virtual row, and clusters crowd on the SMs beyond 96 CTAs (8 KV heads of 128, two queries each, us in clusters of 1, 2, 4, 8: 13 rows over
+// 512 tokens 12.3, 10.2, 8.8, 8.2; 64 over 192 8.5, 11.2, 11.1, 11.2; 256 over 512 13.0, 12.8, 12.3, 15.3; with a second launch that joins
+// 11.3, 11.2, 14.8).  Over 8000 tokens 13 rows would be 16 tiles in a row, about 27 us, and are 21 in parts.
 // A part has 1024 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 65536 keys are 4096 products.
 constexpr int kMostClusterTiles = 48;
 void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32) {
@@ -113,10 +115,20 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32)
   const size_t per_part = (size_t)p.rows * p.hq * (p.d + 2) * sizeof(float);
   const float fill = (float)p.rows / ((float)blocks * p.tokens);  // of the blocks' rows
   p.cluster = 1;
-  if (tensor && !f32 && tiles <= kMostClusterTiles)
-    while (p.cluster < kMostCluster && p.cluster * 2 <= tiles && blocks * p.hkv * p.cluster * 2 <= places) p.cluster *= 2;
+  bool whole = false;  // few tiles in a row, and nothing to gain by dividing them
+  if (tensor && !f32 && tiles <= kMostClusterTiles) {
+    float best = (float)tiles;
+    whole = 2 * blocks * p.hkv <= places;
+    for (int size = 2, log = 1; size <= kMostCluster && size <= tiles && blocks * p.hkv * size <= places; size *= 2, ++log) {
+      if (size > 2 && blocks * p.hkv * size > 256) break;  // 288 CTAs in clusters of four take two rounds (26 us, in twos 20)
+      const int64_t ctas = blocks * p.hkv * size, virtual_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
+      const float crowd = ctas > 96 ? 0.016f * log * (ctas - 96) : 0.f;
+      const float time = (float)((tiles + size - 1) / size) + 1.6f + 0.024f * virtual_rows + crowd;
+      if (time < best) best = time, p.cluster = size;
+    }
+  }
   int64_t room = 0;  // units beside the blocks
-  if (p.cluster > 1) {
+  if (p.cluster > 1 || whole) {
   } else if (blocks < at_once && (2 * blocks < at_once || (fill > 0.5f && !f32)))
     room = at_once - blocks;
   else if (blocks < 4 * at_once && tiles >= 32 && (fill <= 0.5f || f32))

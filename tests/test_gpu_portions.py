@@ -346,7 +346,13 @@ def test_attention_reports_lengths_and_tables_that_are_wrong():
     good = run(row_table([4, 4]))
     assert ops.last_error() == 0
     out = run(row_table([4, 4]), bound=128)  # the first sequence is longer than the bound: its first 128 keys
-    assert ops.last_error() == 4 and torch.isfinite(out).all() and torch.equal(out[4:], good[4:])
+    # The bound sizes the launch and so decides how keys are divided; a row whose keys are added up in another order is rounded otherwise:
+    # with S the sum over keys before the last rounding and |S - exact| <= e for either division (what attend_tolerance counts beside that
+    # rounding), the two may differ by 2e and land in neighbouring halves, but each is as near to the definition as any result.
+    rows, ref, mag, top = attend_all(q, cache, (4, 4), [0, 4, 8])[1]
+    for o in (out, good):
+        assert ((o[rows].double() - ref).abs() <= attend_tolerance(torch.float16, ref, mag, top)).all()
+    assert ops.last_error() == 4 and torch.isfinite(out).all()
     table = cache.table.clone()
     table[0, 1] = -5
     out = run(row_table([4, 4]), table=table)
