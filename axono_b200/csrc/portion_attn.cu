@@ -129,7 +129,7 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32)
   }
   int64_t room = 0;  // units beside the blocks
   if (p.cluster > 1 || whole) {
-  } else if (blocks < at_once && (2 * blocks < at_once || (fill > 0.5f && !f32)))
+  } else if (blocks < at_once && (2 * blocks <= at_once || (fill > 0.5f && !f32 && p.batch > 1)))
     room = at_once - blocks;
   else if (blocks < 4 * at_once && tiles >= 32 && (fill <= 0.5f || f32))
     room = 3 * at_once < blocks * (tiles / 16) ? 3 * at_once : blocks * (tiles / 16);

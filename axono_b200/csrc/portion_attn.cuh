@@ -119,15 +119,17 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
     }
     const float share = v / p.at_once;
     float best = n <= p.at_once ? most + p.part_cost : share + n / p.at_once * p.part_cost + 0.5f * most;
+    // the least L whose parts fit one round: by the sum above, or with every block as long as the longest
+    const float fit = (float)min(p.at_once, p.units), least = fminf(v * 1.001f / (fit - n), ceilf(most / floorf(fit / n)));
     const auto consider = [&](float length, bool rounds) {
-      length = fmaxf(ceilf(fmaxf(length, v * 1.001f / (p.units - n))), 1.f);
+      length = fmaxf(ceilf(length), 1.f);
       const float parts = v / length + n;
       const float time = (rounds ? share + parts / p.at_once * p.part_cost + 0.5f * length : length + p.part_cost) + p.join_cost +
                          0.12f * (1.f + most / length);
       if (length < most && time < best) best = time, part_tiles = fminf((float)kPortionMostTiles, length);
     };
-    if (n < p.units && n < p.at_once) consider(fmaxf(v * 1.001f / (p.at_once - n), sqrtf(0.12f * most)), false);
-    if (n < p.units && p.units > p.at_once) consider(sqrtf(2.f * share * p.part_cost), true);
+    if (n < fit) consider(fmaxf(least, sqrtf(0.12f * most)), false);
+    if (n < p.units && p.units > p.at_once) consider(fmaxf(v * 1.001f / (p.units - n), sqrtf(2.f * share * p.part_cost)), true);
   }
   int before = 0;  // blocks and parts of the sequences before this round's
   for (int base = 0; base < p.batch; base += blockDim.x) {
