@@ -95,9 +95,11 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Few blocks of few tiles are clusters, of the size that takes least by what was measured, in tiles of 0.85 us: joining takes 1.6 and 0.024 per
 // virtual row, and clusters crowd on the SMs beyond 96 CTAs (8 KV heads of 128, two queries each, us in clusters of 1, 2, 4, 8: 13 rows over
 // 512 tokens 12.3, 10.2, 8.8, 8.2; 64 over 192 8.5, 11.2, 11.1, 11.2; 256 over 512 13.0, 12.8, 12.3, 15.3; with a second launch that joins
-// 11.3, 11.2, 14.8).  Over 8000 tokens 13 rows would be 16 tiles in a row, about 27 us, and are 21 in parts.
+// 11.3, 11.2, 14.8).  A cluster divides its own block, a plan all of them: up to 96 tiles one sequence is better off in clusters (64 rows over
+// 5120 tokens 18.3 us, in parts 23.0; over 14400 they would be 29 tiles in a row, and parts take 33.5), several, where lengths may differ, only
+// while no more than 14 tiles are in a row (16 of 3500 / i tokens 33.0 in clusters of two, in parts 21.3; 4 of them 14.8 and 19.6).
 // A part has 1024 tiles at most: the tensor core truncates its sums, by about 2^-26 of them per product, and 65536 keys are 4096 products.
-constexpr int kMostClusterTiles = 48;
+constexpr int kMostClusterTiles = 96;  // eight times 12
 void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32) {
   p.tokens = tensor ? kPortionRows / p.group : portion_fma_tokens(p.group);
   const int places = tensor && f32 ? kSms : 2 * kSms;
@@ -118,9 +120,11 @@ void plan_portions(PortionParams &p, int64_t max_seq_len, bool tensor, bool f32)
   bool whole = false;  // few tiles in a row, and nothing to gain by dividing them
   if (tensor && !f32 && tiles <= kMostClusterTiles) {
     float best = (float)tiles;
-    whole = 2 * blocks * p.hkv <= places;
+    const int64_t most_in_row = p.batch == 1 ? kMostClusterTiles / 2 : 14;
+    whole = tiles <= 14;
     for (int size = 2, log = 1; size <= kMostCluster && size <= tiles && blocks * p.hkv * size <= places; size *= 2, ++log) {
       if (size > 2 && blocks * p.hkv * size > 256) break;  // 288 CTAs in clusters of four take two rounds (26 us, in twos 20)
+      if ((tiles + size - 1) / size > most_in_row) continue;
       const int64_t ctas = blocks * p.hkv * size, virtual_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
       const float crowd = ctas > 96 ? 0.016f * log * (ctas - 96) : 0.f;
       const float time = (float)((tiles + size - 1) / size) + 1.6f + 0.024f * virtual_rows + crowd;
