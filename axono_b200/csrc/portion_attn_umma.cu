@@ -113,7 +113,8 @@ __device__ __forceinline__ void join_cluster(const PortionParams &p, const Porti
           make_uint2(pack_half2(o.x * scale, o.y * scale), pack_half2(o.z * scale, o.w * scale));
       if (fmaf(o.x, 0.f, fmaf(o.y, 0.f, fmaf(o.z, 0.f, o.w * 0.f))) != 0.f) bad |= 1u << r;
     }
-    bad = __reduce_or_sync(0xffffffffu, bad);  // other lanes write such a row anew
+    bad = __reduce_or_sync(0xffffffffu, bad);
+    __syncwarp();  // other lanes write such a row anew: behind what this one has stored of it
     for (; bad; bad &= bad - 1) {
       const int again = row_of((__ffs(bad) - 1) * kSize);
       redo_portion_row<__half>(p, block, again / p.group, hk * p.group + again % p.group, block.tile0 * kN,

@@ -677,3 +677,37 @@ def test_append_of_many_heads():
         assert torch.equal(cv, v)
         at += n
     assert cache.lens.tolist() == [38, 5, 89] and ops.last_error() == 0
+
+
+# counts, cached tokens, query and KV heads, where values that are not finite stand: (sequence, token)
+HIDDEN = {
+    "clusters of two": ((3,) * 16, (900,) * 16, 16, 8, [(0, 902), (5, 448), (5, 449), (9, 901), (15, 0)]),
+    "clusters of four": ((4,), (296,), 4, 2, [(0, 298), (0, 127)]),
+    "clusters of eight": ((90,), (620,), 4, 2, [(0, 660), (0, 709), (0, 200)]),
+    "clusters of eight, some without a key": ((90, 2), (0, 700), 4, 2, [(0, 60), (1, 701)]),
+    "parts": ((20, 1, 3), (7000, 30, 6500), 4, 2, [(0, 7010), (0, 3000), (1, 30), (2, 6502), (2, 64)]),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("where", HIDDEN)
+def test_hidden_infinities_where_keys_are_divided(where, d, dtype):
+    """Values that are not finite in one part of a block's keys: a row that does not see them is as if they were not there, one that does
+    has what the definition gives, whichever CTAs the keys were divided among."""
+    from axono_b200 import ops
+
+    counts, cached, hq, hkv, places = HIDDEN[where]
+    lens = [n + c for n, c in zip(counts, cached)]
+    for bad, in_key in ((math.inf, False), (-math.inf, False), (math.nan, False), (math.nan, True)):
+        cache = Cache(lens, hkv, d, dtype, seed=2)
+        for i, (b, at) in enumerate(places):
+            (cache.k if in_key else cache.v)[b][at, i % hkv, (7 * i) % d] = bad
+            cache.write(b, 0, cache.k[b], cache.v[b])
+        q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, dtype, cache=cache, first=1, behind=2)
+        for rows, ref, mag, top in attend_all(q, cache, counts, starts):
+            got, fine = out[rows].double(), torch.isfinite(ref)
+            assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)])
+            tol = attend_tolerance(dtype, ref, mag, top if math.isfinite(top) else 8.0)[fine]
+            assert ((got - ref)[fine].abs() <= tol).all()
+    assert ops.last_error() == 0
