@@ -16,6 +16,7 @@
 
 #include <mutex>
 
+#include "portion_rows.cuh"
 #include "tcgen05.cuh"
 #include "vec.cuh"
 
@@ -57,8 +58,7 @@ struct RowPlace {
   bool alive;       // belongs to a sequence
 };
 
-// A warp finds a row's sequence, slot and position.  row_start counts up, so that the sequence is the number of entries that are not
-// above the row; a table that does not count up is noticed where the entries found do not enclose the row.
+// A warp finds a row's sequence, slot and position.
 template <bool kAppend>
 __device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowPlace &place) {
   place.alive = true;
@@ -66,16 +66,12 @@ __device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowP
   int64_t here = 0;  // the row's slot, which is its position where none is given, even where the portion does not fit
   if constexpr (kAppend) {
     const int lane = threadIdx.x & 31;
-    int count = 0;
-    for (int i = lane; i <= p.batch; i += 32) count += p.row_start[i] <= row;
-    const int b = __reduce_add_sync(0xffffffffu, count) - 1;
+    bool falls;
+    const int b = portion_sequence(p.row_start, p.batch, (int)p.rows, row, falls);
+    if (falls && lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
     place.alive = false;
-    if (b < 0 || b >= p.batch) return;  // a row of no sequence
+    if (b < 0) return;  // a row of no sequence
     const int r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
-    if (r0 < 0 || r0 > row || r1 <= row || r1 > p.rows) {
-      if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
-      return;
-    }
     place.alive = true;
     here = (p.advance ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);
     if (first_slot(p, len, r1 - r0) < 0) {
@@ -129,7 +125,9 @@ struct Heads {
 // A sequence's length with its portion added, found by a warp; -1 where it stays: nothing new, no room, or a page outside the pool.
 __device__ __forceinline__ int advanced_length(const TurnParams &p, int b) {
   const int lane = threadIdx.x & 31, r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
-  if (r0 < 0 || r1 < r0 || r1 > p.rows) {
+  int earlier = -0x7fffffff - 1;
+  for (int i = lane; i < b; i += 32) earlier = max(earlier, p.row_start[i]);
+  if (!portion_counts_up(r0, r1, (int)p.rows, __reduce_max_sync(0xffffffffu, earlier))) {
     if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
     return -1;
   }

@@ -19,8 +19,10 @@ join_portions_kernel(const PortionParams p) {
   grid_dependency_launch();
   grid_dependency_wait();
   if (row >= p.rows) return;
-  const int first_row = p.row_start[0], end_row = p.row_start[p.batch], parts = min(p.row_parts[row], p.parts);
-  if (row < first_row || row >= end_row || parts <= 1) return;
+  bool falls;
+  if (portion_sequence(p.row_start, p.batch, p.rows, row, falls) < 0) return;  // a row that no CTA had: nothing was written for it
+  const int parts = min(p.row_parts[row], p.parts);
+  if (parts <= 1) return;
   float m = -INFINITY;
   for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.ml[portion_place(p, k, row, head)].x);
 #pragma unroll

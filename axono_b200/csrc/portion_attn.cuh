@@ -9,7 +9,7 @@
 
 #include <math.h>
 
-#include "common.cuh"
+#include "portion_rows.cuh"
 
 namespace axb {
 
@@ -55,15 +55,26 @@ struct PortionSearch {
   float totals[3][kPortionWarps];
 };
 
+// Whether no entry of a launch's row table is below the one before it: then no sequence has to look further back than that.  Called by all
+// threads of a CTA.
+__device__ __forceinline__ bool portion_table_counts_up(const PortionParams &p) {
+  bool up = true;
+  for (int b = threadIdx.x; b < p.batch; b += blockDim.x) up = up && p.row_start[b] <= p.row_start[b + 1];
+  return __syncthreads_and(up) != 0;
+}
+
 // One sequence of a launch.
 struct PortionSpan {
   int r0, count, len, blocks;
-  __device__ __forceinline__ PortionSpan(const PortionParams &p, int b) {
+  __device__ __forceinline__ PortionSpan(const PortionParams &p, int b, bool table_counts_up) {
     r0 = 0, len = 0;
     int r1 = 0;
     if (b < p.batch) {
       r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
-      if (r0 < 0 || r1 < r0 || r1 > p.rows) {
+      int earlier = -0x7fffffff - 1;
+      if (!table_counts_up)
+        for (int i = 0; i < b; ++i) earlier = max(earlier, p.row_start[i]);
+      if (!portion_counts_up(r0, r1, p.rows, earlier)) {
         atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
         r0 = r1 = 0;
       }
@@ -93,11 +104,12 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
   int *s_sums = search->sums;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
   if (threadIdx.x == 0) s_found = 0;
+  const bool up = portion_table_counts_up(p);
   float part_tiles = (float)kPortionMostTiles;  // L
   if (p.parts > 1) {
     float n = 0.f, v = 0.f, most = 0.f;
     for (int b = threadIdx.x; b < p.batch; b += blockDim.x) {
-      const PortionSpan s(p, b);
+      const PortionSpan s(p, b, up);
       if (s.blocks == 0) continue;
       int tile0, last;
       s.tiles(p, (s.blocks - 1) * p.tokens, s.count - (s.blocks - 1) * p.tokens, tile0, last);
@@ -133,7 +145,7 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
   }
   int before = 0;  // blocks and parts of the sequences before this round's
   for (int base = 0; base < p.batch; base += blockDim.x) {
-    const PortionSpan s(p, base + (int)threadIdx.x);
+    const PortionSpan s(p, base + (int)threadIdx.x, up);
     int tile0, tiles, parts = 1;
     if (p.parts > 1 && s.blocks) {
       s.tiles(p, (s.blocks - 1) * p.tokens, s.count - (s.blocks - 1) * p.tokens, tile0, tiles);
@@ -175,8 +187,14 @@ __device__ __forceinline__ bool find_portion_block(const PortionParams &p, int i
     if (s_found || before > index) break;
   }
   block = search->block;
-  block.rows = min(block.rows, p.rows - block.row0);  // whatever a table that does not count up has led to
+  block.rows = min(block.rows, p.rows - block.row0);  // as the table says already; without it the fp32 kernel spills more (164 -> 171 us)
   return s_found && block.part < block.parts;
+}
+
+// The number of parts of a block's rows, for those that join them: written by the CTAs of one KV head, whatever becomes of their waits.
+// (A block has at most as many rows as a CTA has threads.)
+__device__ __forceinline__ void count_portion_parts(const PortionParams &p, const PortionBlock &block) {
+  if (p.parts > 1 && block.part == 0 && (int)threadIdx.x < block.rows) p.row_parts[block.row0 + threadIdx.x] = block.parts;
 }
 
 __host__ __device__ inline int portion_part_begin(int tiles, int part, int parts) { return (int)((int64_t)tiles * part / parts); }
@@ -198,8 +216,10 @@ __device__ __forceinline__ int portion_page(const PortionParams &p, int seq, int
 
 // 1 / l; no key gives zero, and scores that are all -inf give NaN, as 0 / 0 does in the definition.
 __device__ __forceinline__ float portion_inverse(float l, bool some_key) { return l > 0.f ? 1.0f / l : l == 0.f && !some_key ? 0.f : NAN; }
-// (maximum in powers of two, denominator) of a part; -1 as denominator: keys, but scores of -inf alone.
+// (maximum in powers of two, denominator) of a part; -1 as denominator: keys, but scores of -inf alone.  NaN, which makes its rows NaN when
+// parts are joined: a wait of the part ran out, and its sums were not written.
 __device__ __forceinline__ float2 portion_ml(float m, float l, bool some_key) { return make_float2(m, l == 0.f && some_key ? -1.f : l); }
+__device__ __forceinline__ float2 portion_ml_given_up() { return make_float2(NAN, NAN); }
 
 // Four consecutive elements as floats.
 __device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }

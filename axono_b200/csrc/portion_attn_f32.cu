@@ -83,6 +83,13 @@ struct TileOrder {
   __device__ __forceinline__ bool next_is_k(int tiles) const { return k < tiles && k < v + 2; }  // else V, the last of them one too far
 };
 
+// A wait ran out.  (Out of line: what it needs would take registers all along.)
+__device__ __noinline__ void give_up_part(const PortionParams &p, const PortionBlock &block, int hk) {
+  const int token = threadIdx.x / p.group;
+  if (block.parts > 1 && threadIdx.x < kM && token < block.rows)
+    p.ml[portion_place(p, block.part, block.row0 + token, hk * p.group + threadIdx.x % p.group)] = portion_ml_given_up();
+}
+
 template <int kB>
 __global__ void __launch_bounds__(kThreads, 1)
 portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -119,6 +126,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   if (!find_portion_block(p, index, block, reinterpret_cast<PortionSearch *>(corr_s))) return;
   const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
   const int nkv = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts) - tile0;
+  if (hk == 0) count_portion_parts(p, block);
   const int active = (block.rows * p.group + 31) >> 5;  // warps' worth of rows: tensor memory's quarters that matter
 
   if (threadIdx.x == 0) {
@@ -405,9 +413,8 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     if (ok && mine) ok = mbar_wait_warp(bar_l, 0, abort_flag, p.wait_ns);
     if ((ok || nkv == 0) && mine && there) {
       const bool some_key = max(key_begin, tile0 * kN) < min(key_end, (tile0 + nkv) * kN), divided = block.parts > 1;
-      const float l = nkv > 0 ? l_s[vrow] : 0.f;
       const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
-      if (p.parts > 1 && block.part == 0 && head == 0 && half == 0) p.row_parts[row] = block.parts;
+      const float l = nkv > 0 ? l_s[vrow] : 0.f;
       if (divided && half == 0) p.ml[place] = portion_ml(l_s[kM + vrow], l, some_key);
       const float inv = divided ? 1.f : portion_inverse(l, some_key);
       float *dst = divided ? p.sums + place * p.d : static_cast<float *>(p.out) + ((size_t)row * p.hq + head) * p.d;
@@ -423,6 +430,7 @@ portion_f32_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (*abort_flag) give_up_part(p, block, hk);
   if (*bad_flag && !*abort_flag)
     for (int r = warp; r < block.rows * p.group; r += kThreads / 32)
       redo_portion_row<float>(p, block, r / p.group, hk * p.group + r % p.group, tile0 * kN, (tile0 + nkv) * kN, 0.f);

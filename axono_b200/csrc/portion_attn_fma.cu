@@ -36,6 +36,7 @@ portion_fma_kernel(const PortionParams p) {
   unit /= p.hkv;
   PortionBlock block;
   if (!find_portion_block(p, unit, block, &search)) return;
+  if (kSplit && hk == 0 && slice == 0) count_portion_parts(p, block);
   const int head0 = hk * p.group + slice * at_once, heads = min(at_once, p.group - slice * at_once);
   const int tile0 = block.tile0 + portion_part_begin(block.tiles, block.part, block.parts);
   const int tile1 = block.tile0 + portion_part_begin(block.tiles, block.part + 1, block.parts);
@@ -118,7 +119,6 @@ portion_fma_kernel(const PortionParams p) {
   if (!there) return;
   const int at_row = block.row0 + token, at_head = head0 + head;
   const bool divided = kSplit && block.parts > 1;
-  if (kSplit && block.part == 0 && at_head == 0 && sub == 0) p.row_parts[at_row] = block.parts;
   const size_t place = kSplit ? portion_place(p, block.part, at_row, at_head) : 0;
   const bool some_key = max(key_begin, tile0 * kPortionKeys) < min(key_end, tile1 * kPortionKeys);
   if (divided && sub == 0) p.ml[place] = portion_ml(m, l, some_key);

@@ -156,6 +156,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const int part = p.cluster > 1 ? rank : block.part, parts = p.cluster > 1 ? p.cluster : block.parts;
   const int tile0 = block.tile0 + portion_part_begin(block.tiles, part, parts);
   const int nkv = block.tile0 + portion_part_begin(block.tiles, part + 1, parts) - tile0;
+  if (hk == 0) count_portion_parts(p, block);
   const int virtual_rows = block.rows * p.group, active_warps = (virtual_rows + 31) >> 5;
   const bool two_boxes = p.d > 64;
   const uint32_t tile_bytes = two_boxes ? kTileBytes : kTileBytes / 2;
@@ -367,23 +368,25 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool divided = block.parts > 1;
     const int key0 = max(key_begin, tile0 * kN), key1 = min(key_end, (tile0 + nkv) * kN);
     const size_t place = divided ? portion_place(p, block.part, row, head) : 0;
-    if (ok && p.parts > 1 && block.part == 0 && there && head == 0) p.row_parts[row] = block.parts;
-    if (p.cluster > 1) {
-      if (ok) {
-        float *sums = reinterpret_cast<float *>(smem) + threadIdx.x * (p.d + 4);
+    if (!ok) {
+      if (p.cluster > 1)
+        reinterpret_cast<float2 *>(smem + kOffMl)[threadIdx.x] = portion_ml_given_up();
+      else if (divided && there)
+        p.ml[place] = portion_ml_given_up();
+    } else if (p.cluster > 1) {
+      float *sums = reinterpret_cast<float *>(smem) + threadIdx.x * (p.d + 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 >= p.d || nkv == 0) break;
-          uint32_t r[32];
-          tmem_ld32(tmem_o + lane_base + c * 32, r);
+      for (int c = 0; c < 4; ++c) {
+        if (c * 32 >= p.d || nkv == 0) break;
+        uint32_t r[32];
+        tmem_ld32(tmem_o + lane_base + c * 32, r);
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            if (c * 32 + u * 4 < p.d)
-              *reinterpret_cast<uint4 *>(sums + c * 32 + u * 4) = make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
-        }
-        reinterpret_cast<float2 *>(smem + kOffMl)[threadIdx.x] = portion_ml(m_run, l_run, nkv > 0 && key0 < key1);
+        for (int u = 0; u < 8; ++u)
+          if (c * 32 + u * 4 < p.d)
+            *reinterpret_cast<uint4 *>(sums + c * 32 + u * 4) = make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
       }
-    } else if (ok && nkv == 0 && there) {  // no key at all
+      reinterpret_cast<float2 *>(smem + kOffMl)[threadIdx.x] = portion_ml(m_run, l_run, nkv > 0 && key0 < key1);
+    } else if (nkv == 0 && there) {  // no key at all
       uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + ((size_t)row * p.hq + head) * p.d);
       for (int c = 0; c < p.d / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
     }

@@ -1,0 +1,40 @@
+// The table that gives the rows of a launch to sequences: sequence b has the rows row_start[b] .. row_start[b + 1] - 1.  An entry counts up
+// if it is in 0 .. rows and none before it is larger; a sequence with an entry that does not is left out.  So the sequences that are left
+// share no row, and every kernel that follows a table leaves out the same ones.
+#pragma once
+
+#include "common.cuh"
+
+namespace axb {
+
+// Whether sequence b's two entries count up; `earlier`: the largest entry before them (INT_MIN for none).
+__device__ __forceinline__ bool portion_counts_up(int r0, int r1, int rows, int earlier) {
+  return r0 >= 0 && r0 >= earlier && r1 >= r0 && r1 <= rows;
+}
+
+// The sequence of a row, found by a warp, or -1.  Its end is the first entry above the row, so that all before are not.  `falls`: the
+// table does not count up around this row (every fall does so around the rows between the two entries, if there are any).
+__device__ __forceinline__ int portion_sequence(const int32_t *row_start, int batch, int rows, int64_t row, bool &falls) {
+  const int lane = threadIdx.x & 31;
+  unsigned first = 0x7fffffffu;
+  int below = 0;
+  for (int i = lane; i <= batch; i += 32) {
+    if (row_start[i] <= row)
+      ++below;
+    else
+      first = min(first, (unsigned)i);
+  }
+  first = __reduce_min_sync(0xffffffffu, first);
+  below = __reduce_add_sync(0xffffffffu, below);
+  falls = first <= (unsigned)batch && below != (int)first;
+  if (first == 0 || first > (unsigned)batch) return -1;
+  const int b = (int)first - 1;
+  int earlier = -0x7fffffff - 1;
+  for (int i = lane; i < b; i += 32) earlier = max(earlier, row_start[i]);
+  earlier = __reduce_max_sync(0xffffffffu, earlier);
+  if (portion_counts_up(row_start[b], row_start[b + 1], rows, earlier)) return b;
+  falls = true;
+  return -1;
+}
+
+}  // namespace axb

@@ -406,7 +406,8 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  * A launch of `rows` rows: sequence b (row b of block_table) owns the rows row_start[b] .. row_start[b + 1] - 1, a whole prompt, a
  * portion of one, a token or none; row_start int32 (batch + 1) counts up, in device memory like the lengths, so that a captured graph
  * follows both.  Rows before row_start[0] and from row_start[batch] on belong to none and are left as they are, in the outputs too.  An
- * entry of row_start that does not count up or passes `rows` sets AXB200_ERR_BAD_ROWS; what it names is left out.  Pages as in
+ * entry of row_start that does not count up - below zero, below an entry before it, or above `rows` - sets AXB200_ERR_BAD_ROWS, and the
+ * sequences that begin or end with it are left out: nothing of them is read, written or counted.  Pages as in
  * axb200_gqa_decode_paged.  No counterparts in the reference.
  *
  * Rotation of these operators: the first rot_dim elements of a head (even, 0: none) in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with

@@ -711,3 +711,64 @@ def test_hidden_infinities_where_keys_are_divided(where, d, dtype):
             tol = attend_tolerance(dtype, ref, mag, top if math.isfinite(top) else 8.0)[fine]
             assert ((got - ref)[fine].abs() <= tol).all()
     assert ops.last_error() == 0
+
+
+BAD_TABLES = {  # rows of the launch, table, the sequences that are left
+    "passes the rows": (8, [0, 4, 9], [0]),
+    "falls at the end": (8, [0, 8, 4], [0]),
+    "falls and rises": (9, [0, 6, 2, 9], [0]),  # what begins at 2 would share rows with the first
+    "rises behind a fall": (9, [0, 2, 1, 5, 9], [0, 3]),
+    "falls at the beginning": (8, [5, 3, 8], []),
+    "begins below zero": (8, [-2, 4, 8], [1]),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 20])
+@pytest.mark.parametrize("cached", [100, 7000])
+@pytest.mark.parametrize("what", BAD_TABLES)
+def test_tables_that_do_not_count_up(what, cached, d, dtype):
+    """What an entry names that does not count up is left out - not read, not written, whether keys are divided or not - and the other
+    sequences have what they have under a good table."""
+    from axono_b200 import ops
+
+    rows, table, left = BAD_TABLES[what]
+    hq, hkv, batch = 4, 2, len(table) - 1
+    cache = Cache([cached + 10 * b for b in range(batch)], hkv, d, dtype, more=16, poison=0.0)
+    lens, starts = cache.lens.tolist(), torch.tensor(table, dtype=torch.int32, device="cuda")
+    qkv = rnd((rows, (hq + 2 * hkv) * d), dtype, 3)
+    counts = [table[b + 1] - table[b] if b in left else 0 for b in range(batch)]
+    before = (cache.k_pages.clone(), cache.v_pages.clone())
+    # a workspace that holds counts and sums of another call
+    q0 = rnd((rows, hq, d), dtype, 9)
+    for _ in range(2):
+        ops.gqa_attention_portions_paged(q0, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows] + [0] * (batch - 1)), 7100)
+    assert ops.last_error() == 0
+    q = torch.full((rows, hq, d), 7.0, dtype=dtype, device="cuda")
+    ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, out=q)
+    assert ops.last_error() == 16
+    assert cache.lens.tolist() == [n + c for n, c in zip(lens, counts)]
+    owned = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(counts):
+        if not n:
+            continue
+        r = slice(table[b], table[b + 1])
+        owned[r] = True
+        want_q, want_k, want_v = qkv[r].view(n, hq + 2 * hkv, d).split([hq, hkv, hkv], 1)
+        k, v = cache.read(b, lens[b], n)
+        assert torch.equal(q[r], want_q) and torch.equal(k, want_k) and torch.equal(v, want_v)
+        cache.k[b], cache.v[b] = cache.read(b, 0, lens[b] + n)
+        cache.write(b, lens[b], *(torch.zeros_like(k) for _ in range(2)))
+    assert (q[~owned] == 7).all()
+    assert torch.equal(cache.k_pages, before[0]) and torch.equal(cache.v_pages, before[1])  # and nothing else was written
+    for b, n in enumerate(counts):
+        if n:
+            cache.write(b, 0, cache.k[b], cache.v[b])
+    for _ in range(2):
+        ops.gqa_attention_portions_paged(q0, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows] + [0] * (batch - 1)), 7100)
+    out = torch.full((rows, hq, d), 7.0, dtype=dtype, device="cuda")
+    ops.gqa_attention_portions_paged(q0, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, 7100, out=out)
+    assert ops.last_error() == 16
+    assert (out[~owned] == 7).all()
+    good = list(zip(*[(table[b], n) for b, n in enumerate(counts)]))[0]
+    check_attention(q0, cache, counts, list(good), out)
