@@ -88,6 +88,8 @@ SIGNATURES = {
     "axb200_qk_norm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _f, _vp, _vp, _i, _i, _f, _i, _i, _i, _vp, _vp, _i64, _i, _i, _i, _i, _vp]),
     "axb200_qkv_norm_rope_append_portions": (_i, [_vp, _i64, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _i, _i,
                                                   _i64, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "axb200_qkv_norm_rope_append_portions_at": (_i, [_vp, _i64, _vp, _vp, _f, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _f, _i, _i, _i,
+                                                     _i64, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     "axb200_gqa_attention_portions_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _i]),
     "axb200_gqa_attention_portions_paged": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i, _i, _vp, _sz, _vp]),
     "axb200_rope": (_i, [_vp, _vp, _f, _vp, _i64, _i, _i, _i, _vp]),

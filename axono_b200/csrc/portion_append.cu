@@ -43,11 +43,18 @@ struct TurnParams {
   void *k_pages, *v_pages;
   const int32_t *block_table, *seq_lens, *row_start;
   int batch, page_tokens, max_blocks, num_pages, advance;
+  int32_t *slots;  // (batch) or null: every portion's first slot, or -1, as the launch that advanced the lengths has left it
 };
 
-// Where a sequence's portion goes: its first slot, or -1 where it does not fit.
-__device__ __forceinline__ int64_t first_slot(const TurnParams &p, int len, int count) {
+// Where a sequence's portion goes: its first slot; -1 where it does not fit, or is not what the length counts; -2 where the launch that
+// advanced the lengths refused it - a length that did not grow would give it the slots of older tokens.
+__device__ __forceinline__ int64_t first_slot(const TurnParams &p, int b, int len, int count) {
   const int64_t first = p.advance ? (int64_t)len : (int64_t)len - count;
+  if (!p.advance && p.slots) {
+    const int slot = p.slots[b];
+    if (slot == -1) return -2;
+    if (slot != first) return -1;
+  }
   return first < 0 || first + count > (int64_t)p.max_blocks * p.page_tokens ? -1 : first;
 }
 
@@ -73,9 +80,10 @@ __device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowP
     if (b < 0) return;  // a row of no sequence
     const int r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
     place.alive = true;
-    here = (p.advance ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);
-    if (first_slot(p, len, r1 - r0) < 0) {
-      if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
+    const int64_t first = first_slot(p, b, len, r1 - r0);
+    here = (first >= 0 ? first : p.advance || p.slots ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);
+    if (first < 0) {
+      if (first == -1 && lane == 0) atomicOr(&g_error_word, AXB200_ERR_CAPACITY);
     } else {
       const int slot = (int)here, block = slot / p.page_tokens;
       const int page = p.block_table[(int64_t)b * p.max_blocks + block];
@@ -131,7 +139,7 @@ __device__ __forceinline__ int advanced_length(const TurnParams &p, int b) {
     if (lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
     return -1;
   }
-  const int64_t first = first_slot(p, len, r1 - r0);
+  const int64_t first = first_slot(p, b, len, r1 - r0);
   if (r1 == r0 || first < 0) return -1;
   bool ok = true;
   for (int64_t i = first / p.page_tokens + lane; i <= (first + r1 - r0 - 1) / p.page_tokens; i += 32) {
@@ -139,6 +147,12 @@ __device__ __forceinline__ int advanced_length(const TurnParams &p, int b) {
     ok = ok && page >= 0 && page < p.num_pages;
   }
   return __all_sync(0xffffffffu, ok) ? len + (r1 - r0) : -1;
+}
+
+// The length that advanced_length gave, written by one lane, and for the launches that follow where the portion went.
+__device__ __forceinline__ void store_length(const TurnParams &p, int b, int advanced, int32_t *seq_lens) {
+  if (p.slots) p.slots[b] = advanced >= 0 ? seq_lens[b] : -1;
+  if (advanced >= 0) seq_lens[b] = advanced;
 }
 
 __device__ __forceinline__ void copy_async16(void *dst, const void *src) {
@@ -347,7 +361,7 @@ turn_rows_kernel(const TurnParams p, int ways, int32_t *seq_lens) {
     __syncthreads();  // every warp has read the lengths
     for (int b = warp; b < p.batch; b += blockDim.x >> 5) {
       if (b != warp) advanced = advanced_length(p, b);
-      if (lane == 0 && advanced >= 0) seq_lens[b] = advanced;
+      if (lane == 0) store_length(p, b, advanced, seq_lens);
     }
   }
 }
@@ -412,7 +426,7 @@ advance_lengths_kernel(const TurnParams p, int32_t *seq_lens) {
   grid_dependency_wait();
   if (b >= p.batch) return;
   const int advanced = advanced_length(p, b);
-  if ((threadIdx.x & 31) == 0 && advanced >= 0) seq_lens[b] = advanced;
+  if ((threadIdx.x & 31) == 0) store_length(p, b, advanced, seq_lens);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -511,18 +525,18 @@ int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld
                                    : axb::launch_turn<__nv_bfloat16, false>(p, nullptr, st);
 }
 
-int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
-                                         void *k_pages, void *v_pages, const int32_t *block_table, int32_t *seq_lens,
-                                         const int32_t *row_start, const int64_t *pos, const double *inv_freq, int rot_dim,
-                                         int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
-                                         int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
-                                         void *stream) {
+int axb200_qkv_norm_rope_append_portions_at(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
+                                            void *k_pages, void *v_pages, const int32_t *block_table, int32_t *seq_lens,
+                                            const int32_t *row_start, const int64_t *pos, const double *inv_freq, int rot_dim,
+                                            int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
+                                            int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
+                                            int32_t *slots, void *stream) {
   if (dtype != AXB200_FLOAT16 && dtype != AXB200_FLOAT32) return AXB200_UNSUPPORTED_TYPE;
   const size_t e = axb::dtype_size(dtype);
   axb::TurnParams p{qkv, static_cast<const char *>(qkv) + (size_t)(hq > 0 ? hq : 0) * (d > 0 ? d : 0) * e, ld, ld, q_norm_w, k_norm_w,
                     eps, pos, inv_freq, rot_dim / 2, interleaved != 0, mrope != 0, 3 * h_sec, 3 * w_sec, factor, q_out, nullptr, rows,
                     hq, hkv, d, k_pages, v_pages, block_table, seq_lens, row_start, batch, page_tokens, max_blocks, num_pages,
-                    advance != 0};
+                    advance != 0, slots};
   if (!axb::turn_sizes_ok(p) || hq == 0 || hkv == 0 || rot_dim < 0 || rot_dim % 2 || rot_dim > d || h_sec < 0 || w_sec < 0 || batch <= 0 ||
       page_tokens <= 0 || page_tokens % 64 || max_blocks <= 0 || num_pages <= 0 || (int64_t)max_blocks * page_tokens > 0x7fffffff - 4096 ||
       (qkv && qkv == q_out))
@@ -534,6 +548,17 @@ int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t *advanced = advance ? seq_lens : nullptr;
   return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, true>(p, advanced, st) : axb::launch_turn<__half, true>(p, advanced, st);
+}
+
+int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
+                                         void *k_pages, void *v_pages, const int32_t *block_table, int32_t *seq_lens,
+                                         const int32_t *row_start, const int64_t *pos, const double *inv_freq, int rot_dim,
+                                         int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
+                                         int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
+                                         void *stream) {
+  return axb200_qkv_norm_rope_append_portions_at(qkv, ld, q_norm_w, k_norm_w, eps, q_out, k_pages, v_pages, block_table, seq_lens, row_start,
+                                                 pos, inv_freq, rot_dim, interleaved, factor, mrope, h_sec, w_sec, rows, batch, hq, hkv, d,
+                                                 page_tokens, max_blocks, num_pages, dtype, advance, nullptr, stream);
 }
 
 }  // extern "C"

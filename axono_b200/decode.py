@@ -183,13 +183,16 @@ class TextTower:
         """The next tokens of the batch's sequences at once: counts[b] (host) tokens of sequence b, 0 for none - whole prompts, portions
         of them, single tokens - whose ids stand one sequence after the other in token_ids.  Appends them to every layer's cache and
         leaves every sequence that brought some ready for `decode_step`: the greedy next token of its last one in `token_ids`, its
-        position in `pos3`.  Returns those tokens, and their logits are `last_logits` (one row per such sequence)."""
+        position in `pos3`.  Returns those tokens, and their logits are `last_logits` (one row per such sequence).  A sequence whose tokens
+        do not fit (`ops.last_error` tells) stays as it was, in every layer and in `token_ids` and `pos3`, and -1 is returned for it."""
         cfg, d = self.cfg, self.cfg.head_dim
         counts = torch.as_tensor(counts, dtype=torch.int64).cpu()
         ids = torch.as_tensor(token_ids, dtype=torch.int64).reshape(-1)
         rows = int(counts.sum())
         if counts.shape != (self.batch,) or int(counts.min()) < 0 or rows != ids.numel() or rows == 0:
             raise RuntimeError("extend: a count for every sequence, and as many tokens as they add up to (at least one)")
+        if int(counts.max()) > self.cache.max_seq_len:
+            raise RuntimeError(f"extend: more tokens of a sequence than the cache holds ({self.cache.max_seq_len})")
         starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
         seq = torch.repeat_interleave(torch.arange(self.batch), counts)
         offset = (torch.arange(rows) - starts[seq]).to(self.device)
@@ -212,9 +215,11 @@ class TextTower:
             h, mlp_out = self._feed_forward(lw, self._linear(attn.reshape(rows, cfg.n_q_heads * d), lw["o"]), h)
         self.last_logits = self._logits(mlp_out[last], h[last])
         nxt = ops.argmax_last_dim(self.last_logits)
-        self.token_ids[brought] = nxt
-        self.pos3 += counts.to(self.device)
-        return nxt
+        fitted = self.cache.portion_slots[:self.batch] >= 0
+        self.pos3 += counts.to(self.device) * fitted
+        fitted = fitted[brought]
+        self.token_ids[brought] = torch.where(fitted, nxt, self.token_ids[brought])
+        return torch.where(fitted, nxt, -1)
 
     def _feed_forward(self, lw, attn_out, h):
         """The second half of a layer as single operators: (h, what is still to be added to it)."""

@@ -84,6 +84,9 @@ class KVCache:
         raise NotImplementedError
 
 
+_NO_PORTION = 0x7fffffff  # no length is so far: a layer's portion before any of the first layer is refused
+
+
 class PagedKVCache(KVCache):
     """Per-layer page pools (num_pages, n_kv_heads, page_tokens, head_dim) shared by `batch`
     sequences, one block table and one device-resident length vector per cache.
@@ -112,6 +115,7 @@ class PagedKVCache(KVCache):
             page_order = torch.arange(self.num_pages, dtype=torch.int32)
         self.block_table = page_order.to(torch.int32).reshape(batch, self.max_blocks).contiguous().to(device)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.portion_slots = torch.full((batch,), _NO_PORTION, dtype=torch.int32, device=device)
         self._host_len_bound = 0  # host-side upper bound of seq_lens (sizes grids, no sync)
 
     # -- reference interface ------------------------------------------------------------------
@@ -152,12 +156,13 @@ class PagedKVCache(KVCache):
         """The next tokens of several sequences - whole prompts, portions, single tokens - straight from the QKV projection: sequence
         b's are the rows row_start[b] .. row_start[b + 1] - 1 of qkv.  Per-head norm and rotation (`ops.qkv_norm_rope_append_portions`),
         keys and values behind the cached ones; returns q (rows, hq, d).  longest: host bound of the tokens one sequence brings
-        (default: all rows)."""
+        (default: all rows).  The first layer's call decides what fits: `portion_slots` holds the slot that each sequence's portion begins
+        at, or -1 for one that was refused (capacity, or a page outside the pool), of which the other layers append nothing either."""
         first = layer_idx == 0
         q = ops.qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, self.k_pages[layer_idx],
                                               self.v_pages[layer_idx], self.block_table, self.seq_lens, row_start, pos=pos,
                                               inv_freq=inv_freq, interleaved=interleaved, factor=factor, mrope_section=mrope_section,
-                                              advance=first, out=out)
+                                              advance=first, out=out, slots=self.portion_slots)
         if first:
             self._host_len_bound = min(self.max_seq_len, self._host_len_bound + (qkv.shape[0] if longest is None else int(longest)))
         return q
@@ -377,6 +382,7 @@ class KVArena:
                                                         (self.max_seqs, self.max_blocks), "<i4"), device=dev)
             c.seq_lens = torch.as_tensor(_DeviceView(lib.axb200_kv_arena_seq_lens(self._h), (self.max_seqs,), "<i4"),
                                          device=dev)
+            c.portion_slots = torch.full((self.max_seqs,), _NO_PORTION, dtype=torch.int32, device=dev)
             c._host_len_bound = 0
             self._cache = c
         return self._cache

@@ -800,19 +800,23 @@ def _portion_tables(op, x, k_pages, v_pages, block_table, seq_lens, row_start):
 
 
 def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens, row_start,
-                                  pos=None, inv_freq=None, interleaved=False, factor=1.0, mrope_section=None, advance=True, out=None):
+                                  pos=None, inv_freq=None, interleaved=False, factor=1.0, mrope_section=None, advance=True, out=None,
+                                  slots=None):
     """`qkv_norm_rope_append` for rows that bring several sequences their next tokens: sequence b owns the rows row_start[b] ..
     row_start[b + 1] - 1 of qkv (rows, (hq + 2 * hkv) * d) (rows may be strided), row_start int32 (batch + 1) on the device.  Per-head
     norm and rotation as in `qk_norm_rope` (pos None: the slot; inv_freq None: no rotation); keys and values go behind the seq_lens[b]
     cached tokens, which grow by the portion (advance, the first layer of a step), or into the last of them (later layers).  Returns
-    the turned q (rows, hq, d); rows of no sequence are left as they are in `out`."""
+    the turned q (rows, hq, d); rows of no sequence are left as they are in `out`.
+    slots: int32 (batch) or more, one buffer for all layers of a step whose portions may not fit: the first layer's call leaves every
+    portion's first slot in it, -1 for one that it refused, and the others append nothing of that (without, they would write it over
+    the sequence's last tokens: the lengths do not tell)."""
     op = "qkv_norm_rope_append_portions"
     dt = _dt(qkv, op)
     dtype, device = qkv.dtype, qkv.get_device()
     if device != _device_now():
         with torch.cuda.device(device):
             return qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, k_pages, v_pages, block_table, seq_lens,
-                                                 row_start, pos, inv_freq, interleaved, factor, mrope_section, advance, out)
+                                                 row_start, pos, inv_freq, interleaved, factor, mrope_section, advance, out, slots)
     if qkv.dim() != 2:
         _capi.check(4, op)
     batch, *pages = _portion_tables(op, qkv, k_pages, v_pages, block_table, seq_lens, row_start)
@@ -830,9 +834,17 @@ def qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, 
         out = qkv.new_empty((rows, n_q_heads, d))
     elif out.shape != (rows, n_q_heads, d) or out.dtype is not dtype or not out.is_contiguous() or out.get_device() != device:
         _capi.check(4, op)
-    _launched(_capi.lib().axb200_qkv_norm_rope_append_portions(
+    if slots is not None:
+        if slots.dtype is not torch.int32:
+            _capi.check(3, op)
+        if slots.dim() != 1 or slots.shape[0] < batch or not slots.is_contiguous():
+            _capi.check(4, op)
+        if slots.get_device() != device:
+            _elsewhere(op)
+    _launched(_capi.lib().axb200_qkv_norm_rope_append_portions_at(
         qkv.data_ptr(), ld, wq, wk, eps, out.data_ptr(), *pages, at, freq, rot_dim, bool(interleaved), factor, mrope, h, w, rows, batch, n_q_heads,
-        hkv, d, page_tokens, block_table.shape[1], num_pages, dt, bool(advance), _stream_now(device)), op)
+        hkv, d, page_tokens, block_table.shape[1], num_pages, dt, bool(advance), None if slots is None else slots.data_ptr(),
+        _stream_now(device)), op)
     return out
 
 

@@ -424,6 +424,9 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *     tokens, whose number then grows by the portion; else (later layers) into the last slots of seq_lens[b], which counts them already.
  *     pos NULL: a row's position is its slot.  A portion that does not fit sets AXB200_ERR_CAPACITY, nothing of it is appended and its
  *     length stays; a page outside the pool sets AXB200_ERR_BAD_PAGE, its rows are not written and the length stays.  FLOAT16, FLOAT32.
+ *     The lengths alone do not tell later layers of a portion that the first refused: they would write it over its sequence's last tokens.
+ *     So where a portion may not fit, all layers of a step take append_portions_at with one buffer `slots`, int32 (batch): the launch with
+ *     `advance` leaves in it the first slot of every portion, -1 for one that it refused, and the others write only to those.
  *   gqa_attention_portions_paged: q, out (rows, hq, d), which do not overlap: row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
  *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
  *     counts the portion.  A row that sees no key gets zeros; keys and values that a row does not see, and what stands behind a sequence's
@@ -441,6 +444,12 @@ int axb200_qkv_norm_rope_append_portions(const void *qkv, int64_t ld, const void
                                          int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
                                          int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
                                          void *stream);
+int axb200_qkv_norm_rope_append_portions_at(const void *qkv, int64_t ld, const void *q_norm_w, const void *k_norm_w, float eps, void *q_out,
+                                            void *k_pages, void *v_pages, const int32_t *block_table, int32_t *seq_lens,
+                                            const int32_t *row_start, const int64_t *pos, const double *inv_freq, int rot_dim,
+                                            int interleaved, float factor, int mrope, int h_sec, int w_sec, int64_t rows, int batch, int hq,
+                                            int hkv, int d, int page_tokens, int max_blocks, int num_pages, int dtype, int advance,
+                                            int32_t *slots, void *stream);
 size_t axb200_gqa_attention_portions_workspace_bytes(int64_t rows, int batch, int hq, int hkv, int d, int page_tokens, int max_blocks,
                                                      int64_t max_seq_len, int window, int aligned, int dtype);
 int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_pages, const void *v_pages, const int32_t *block_table,

@@ -772,3 +772,76 @@ def test_tables_that_do_not_count_up(what, cached, d, dtype):
     assert (out[~owned] == 7).all()
     good = list(zip(*[(table[b], n) for b, n in enumerate(counts)]))[0]
     check_attention(q0, cache, counts, list(good), out)
+
+
+@pytest.mark.parametrize("what", ["capacity", "page", "both"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_a_refused_portion_leaves_every_layer_as_it_was(what, dtype):
+    """A portion that does not fit, or whose page is outside the pool, in a tower of three layers: no cached key or value of its sequence
+    changes in any of them, nor its length, position and next token; the other sequences go on as if it had brought nothing."""
+    from axono_b200 import ops
+    from axono_b200.decode import TextTower, TextTowerConfig
+
+    cfg = TextTowerConfig(hidden=256, intermediate=512, n_q_heads=8, n_kv_heads=4, head_dim=64, vocab=1000, n_layers=3, use_mrope=False)
+    ids = torch.randint(0, 1000, (400,), generator=torch.Generator().manual_seed(1))
+    towers = [TextTower(cfg, 3, 320, dtype=dtype, seed=3) for _ in range(2)]
+    for t in towers:
+        t.extend(ids, [300, 20, 80])
+        assert ops.last_error() == 0
+    tower, other = towers
+    if what != "capacity":
+        tower.cache.block_table[2, 1] = tower.cache.num_pages + 3  # the page of slots 64 .. 127: the portion begins in the middle of it
+    refused, error = {"capacity": ([0], 4), "page": ([2], 2), "both": ([0, 2], 6)}[what]
+    counts = [50 if 0 in refused else 5, 7, 6]
+    fitting = [0 if b in refused else n for b, n in enumerate(counts)]
+    lens, pos, tokens = tower.cache.seq_lens.clone(), tower.pos3.clone(), tower.token_ids.clone()
+    pages = [[pool.clone() for pool in pools] for pools in (tower.cache.k_pages, tower.cache.v_pages)]
+    more = torch.randint(0, 1000, (sum(counts),), generator=torch.Generator().manual_seed(2))
+    nxt = tower.extend(more, counts)
+    assert ops.last_error() & error == error
+    parts = torch.split(more, counts)
+    expect = other.extend(torch.cat([p for p, n in zip(parts, fitting) if n]), fitting)
+    assert tower.cache.seq_lens.tolist() == other.cache.seq_lens.tolist() == [int(n) + c for n, c in zip(lens, fitting)]
+    assert torch.equal(tower.pos3, other.pos3) and torch.equal(tower.pos3[:, refused], pos[:, refused])
+    assert torch.equal(tower.token_ids[refused], tokens[refused])
+    assert nxt.tolist() == [-1 if b in refused else int(expect[[i for i, n in enumerate(fitting) if n].index(b)]) for b in range(3)]
+    table = other.cache.block_table
+    for pools, old, theirs in zip((tower.cache.k_pages, tower.cache.v_pages), pages, (other.cache.k_pages, other.cache.v_pages)):
+        for layer in range(cfg.n_layers):
+            for b in range(3):
+                n = int(lens[b]) if b in refused else int(lens[b]) + counts[b]
+                page, place = table[b, torch.arange(n, device="cuda") // 64].long(), torch.arange(n, device="cuda") % 64
+                got, was, want = (x[page, :, place] for x in (pools[layer], old[layer], theirs[layer]))
+                assert torch.equal(got[:int(lens[b])], was[:int(lens[b])]), (layer, b)
+                # another number of rows may take another algorithm of the projections
+                assert (got.double() - want.double()).abs().max() <= 2.0 ** -7 * want.abs().max(), (layer, b)
+    if what == "capacity":  # what fits is taken afterwards
+        tower.extend(more[:20], [20, 0, 0])
+        assert ops.last_error() == 0 and tower.cache.seq_lens.tolist() == [320, 27, 86]
+        with pytest.raises(RuntimeError):
+            tower.extend(ids[:321], [321, 0, 0])
+
+
+@pytest.mark.parametrize("rows", [2, 70])  # one launch that also advances, and two
+def test_slots_carry_what_was_accepted_to_later_layers(rows):
+    from axono_b200 import ops
+
+    hq, hkv, d = 4, 2, 64
+    cache = Cache([100, 60, 10], hkv, d, torch.float16, more=rows, poison=0.0)
+    counts, lens = [rows, 0, 1], cache.lens.clone()
+    cache.table[2, 0] = -1
+    qkv, slots = rnd((rows + 1, (hq + 2 * hkv) * d), torch.float16, 3), torch.full((5,), 77, dtype=torch.int32, device="cuda")
+    run = lambda advance, lens, slots=slots: ops.qkv_norm_rope_append_portions(  # noqa: E731
+        qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, lens, row_table(counts), advance=advance, slots=slots)
+    run(True, lens)
+    assert ops.last_error() == 2 and slots.tolist() == [100, -1, -1, 77, 77] and lens.tolist() == [100 + rows, 60, 10]
+    k = cache.read(0, 100, rows)[0].clone()
+    cache.write(0, 100, *(torch.zeros_like(k) for _ in range(2)))
+    run(False, lens)
+    assert ops.last_error() == 0 and torch.equal(cache.read(0, 100, rows)[0], k)  # and nothing is reported twice
+    k0 = cache.k_pages.clone()
+    run(False, cache.lens)  # lengths that are not those of the step
+    assert ops.last_error() == 4 and torch.equal(cache.k_pages, k0)
+    for bad in (slots[:2], slots.long(), slots[::2], slots.cpu()):
+        with pytest.raises(RuntimeError):
+            run(False, lens, bad)

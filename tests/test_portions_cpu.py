@@ -121,3 +121,12 @@ def test_signatures_hold_what_the_header_declares():
                        ("axb200_gqa_attention_portions_workspace_bytes", 11), ("axb200_gqa_attention_portions_paged", 21)):
         assert len(_capi.SIGNATURES[name][1]) == args
     assert _capi.SIGNATURES["axb200_gqa_attention_portions_workspace_bytes"][0] is ctypes.c_size_t
+
+
+def test_the_form_with_slots_refuses_what_the_other_does():
+    for kw, status in ((dict(dtype=_capi.BFLOAT16), TYPE), (dict(batch=0), INVALID), (dict(ld=511), SHAPE), (dict(lens=None), POINTER), (dict(rows=0), 0)):
+        a = dict(qkv=FAKE, ld=512, qw=None, kw=None, eps=1e-6, qo=FAKE + 4096, k=FAKE, v=FAKE, table=FAKE, lens=FAKE, start=FAKE, pos=None, freq=FAKE,
+                 rot=64, inter=0, factor=1.0, mrope=0, h=0, w=0, rows=4, batch=2, hq=4, hkv=2, d=64, page=64, blocks=4, pages=8,
+                 dtype=_capi.FLOAT16, advance=1, slots=FAKE, stream=None)
+        a.update(kw)
+        assert _capi.lib().axb200_qkv_norm_rope_append_portions_at(*a.values()) == status, kw
