@@ -669,9 +669,10 @@ def _elsewhere(op):
     raise RuntimeError(f"{op}: tensors on different devices")
 
 
-# torch.cuda.current_stream and current_device take 5 us of the 14 that a call of these operators has; these two take 0.2
-_device_now = torch._C._cuda_getDevice
-_stream_now = torch._C._cuda_getCurrentRawStream
+# torch.cuda.current_stream and current_device take 5 us of the 14 that a call of these operators has; these two take 0.2.  They are no
+# public names, and a torch without CUDA has neither.
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _launched(status, op):

@@ -1,6 +1,9 @@
 """What the operators for portions refuse before anything is launched, their plans, and the frequencies of stretched contexts."""
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -130,3 +133,13 @@ def test_the_form_with_slots_refuses_what_the_other_does():
                  dtype=_capi.FLOAT16, advance=1, slots=FAKE, stream=None)
         a.update(kw)
         assert _capi.lib().axb200_qkv_norm_rope_append_portions_at(*a.values()) == status, kw
+
+
+def test_the_operators_import_where_torch_lacks_cuda_bindings():
+    """A torch built without CUDA has neither of the two names that calls take device and stream from."""
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "from axono_b200 import ops\n"
+            "assert ops._device_now is torch.cuda.current_device and callable(ops._stream_now)\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
