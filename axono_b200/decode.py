@@ -7,7 +7,7 @@ RoPE on q/k -> KV-cache append -> gqa_decode_attention -> silu_mul.
 tower (axono/python/examples/vlm/qwen3vl/model.py:330-373 attention, :408-436 layer, :483-486 final
 norm + tied lm_head, :729-761 decode_step), extended from one sequence to a batch of rows.  Its
 projections are library GEMMs (one cuBLASLt call each through `ops.linear_nobias`, whose algorithm is
-timed per shape on first use; `lt_gemm=False` takes torch.matmul), which stay outside the rewritten path;
+timed per shape on first use; `lt_gemm=False`, and numbers of rows that only a portion has, take torch.matmul), which stay outside the rewritten path;
 everything between them is this package's kernels.  Two fusions the reference's layer does not have:
 the residual add that ends a layer is folded into the next layer's input norm (one add_rms_norm),
 and rope + append is one launch.  `extend` brings prompts and portions of them to the same cache (`append_portions`,
@@ -73,6 +73,10 @@ def _rope_append_attend(cache, layer, q, k_new, v_new, pos, inv_freq, theta, mro
     return cache.attend(layer, q)
 
 
+def _plain_linear(x, w):
+    return torch.matmul(x, w.t())
+
+
 class TextTower:
     """Random-init text tower with a paged KV cache; `decode_step` is capturable in one CUDA graph."""
 
@@ -82,7 +86,7 @@ class TextTower:
         self.cfg, self.batch, self.device, self.dtype = cfg, batch, torch.device(device), dtype
         self.fused_qkv = fused_qkv
         self.lt_gemm, self.row_chain = lt_gemm, row_chain
-        self._linear = ops.linear_nobias if lt_gemm else (lambda x, w: torch.matmul(x, w.t()))
+        self._linear = ops.linear_nobias if lt_gemm else _plain_linear
         self.world, self.rank = world, rank
         self.peer_gather = None
         if world > 1 and fused_gather:
@@ -201,19 +205,20 @@ class TextTower:
         row_start, seq, brought = starts.to(torch.int32).to(self.device), seq.to(self.device), brought.to(self.device)
         pos = self.pos3[:, seq] + offset if cfg.use_mrope else self.pos3[0, seq] + offset
         h, mlp_out = ops.embedding(ids.to(self.device), self.embed), None
+        linear = self._linear_for(rows)
         for li, lw in enumerate(self.layers):
             if mlp_out is None:
                 xn = ops.rms_norm(h, lw["input_ln"], cfg.eps)
             else:
                 h, xn = ops.add_rms_norm(mlp_out, h, lw["input_ln"], cfg.eps)
-            q = self.cache.append_portions(li, self._linear(xn, lw["qkv"]), self.local_q, row_start, int(counts.max()),
+            q = self.cache.append_portions(li, linear(xn, lw["qkv"]), self.local_q, row_start, int(counts.max()),
                                            lw["q_norm"] if cfg.qk_norm else None, lw["k_norm"] if cfg.qk_norm else None, cfg.eps, pos=pos,
                                            inv_freq=self.portion_freq, mrope_section=cfg.mrope_section if cfg.use_mrope else None)
             attn = self.cache.attend_portions(li, q, row_start)
             if self.world > 1:
                 attn = sharding.all_gather_heads(attn)
-            h, mlp_out = self._feed_forward(lw, self._linear(attn.reshape(rows, cfg.n_q_heads * d), lw["o"]), h)
-        self.last_logits = self._logits(mlp_out[last], h[last])
+            h, mlp_out = self._feed_forward(lw, linear(attn.reshape(rows, cfg.n_q_heads * d), lw["o"]), h, linear)
+        self.last_logits = self._logits(mlp_out[last], h[last], self._linear_for(len(last)))
         nxt = ops.argmax_last_dim(self.last_logits)
         fitted = self.cache.portion_slots[:self.batch] >= 0
         self.pos3 += counts.to(self.device) * fitted
@@ -221,20 +226,27 @@ class TextTower:
         self.token_ids[brought] = torch.where(fitted, nxt, self.token_ids[brought])
         return torch.where(fitted, nxt, -1)
 
-    def _feed_forward(self, lw, attn_out, h):
+    def _linear_for(self, rows: int):
+        """The projections of that many rows.  `decode_step` has the batch's every time, and the algorithm that is timed on their first
+        use serves them for good; portions have other numbers with nearly every call, and a hundred trial products for each - and a plan
+        kept for it - would cost more than the library's first choice."""
+        return self._linear if rows == self.batch else _plain_linear
+
+    def _feed_forward(self, lw, attn_out, h, linear=None):
         """The second half of a layer as single operators: (h, what is still to be added to it)."""
         cfg = self.cfg
+        linear = linear or self._linear
         h, xn2 = ops.add_rms_norm(attn_out, h, lw["post_ln"], cfg.eps)
-        gu = self._linear(xn2, lw["gate_up"])
+        gu = linear(xn2, lw["gate_up"])
         if self.fused_qkv:
             act = ops.silu_mul_rows(gu, cfg.intermediate)
         else:
             act = ops.silu_mul(gu[:, :cfg.intermediate].contiguous(), gu[:, cfg.intermediate:].contiguous())
-        return h, self._linear(act, lw["down"])
+        return h, linear(act, lw["down"])
 
-    def _logits(self, mlp_out, h):
+    def _logits(self, mlp_out, h, linear=None):
         _, xf = ops.add_rms_norm(mlp_out, h, self.final_ln, self.cfg.eps)
-        return self._linear(xf, self.embed)
+        return (linear or self._linear)(xf, self.embed)
 
     def _chains(self) -> bool:
         """Whether everything between two attention calls is one launch (`ops.row_chain`): one rank, the fused forms, few

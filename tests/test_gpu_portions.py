@@ -845,3 +845,20 @@ def test_slots_carry_what_was_accepted_to_later_layers(rows):
     for bad in (slots[:2], slots.long(), slots[::2], slots.cpu()):
         with pytest.raises(RuntimeError):
             run(False, lens, bad)
+
+
+def test_extending_by_new_numbers_of_rows_makes_no_trial_products():
+    """The product whose algorithm is timed on the first use of a shape takes the batch's rows alone; every other number of rows is one
+    product per projection."""
+    from axono_b200 import ops
+    from axono_b200.decode import TextTower, TextTowerConfig
+
+    cfg = TextTowerConfig(hidden=256, intermediate=512, n_q_heads=4, n_kv_heads=2, head_dim=64, vocab=500, n_layers=2, use_mrope=False)
+    tower, timed = TextTower(cfg, 3, 640, seed=3), []
+    inner = ops.linear_nobias
+    tower._linear = lambda x, w: timed.append(x.shape[0]) or inner(x, w)
+    for counts in ([70, 0, 0], [1, 1, 0], [5, 100, 33], [0, 0, 1], [1, 1, 1], [0, 3, 0]):
+        tower.extend(torch.arange(sum(counts)) % 500, counts)
+    tower.decode_step()
+    assert timed and set(timed) == {3}
+    assert ops.last_error() == 0
