@@ -4,7 +4,8 @@
 // and part of its keys, two CTAs per SM.  Tiles of 64 keys, each in one page, whose 64 rows of a KV head are one run of memory: TMA fetches
 // them through a map of the pool (d, page_tokens, hkv, num_pages).  S = Q.K^T (128 x 64) and O += P.V are tcgen05.mma with the sums in
 // tensor memory; thread t owns virtual row t: scores from tensor memory, online softmax in registers, P as fp16 pairs over the scores,
-// from where P.V takes its A operand.  S is computed two tiles ahead.
+// from where P.V takes its A operand (kNarrow, heads below 128: in two parts, which fill the place of the scores).  S is computed two
+// tiles ahead.
 //
 // Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
 // still meet weights of zero in P.V, so rows of V behind the sequence's end, where anything may stand, are cleared in shared memory
@@ -15,10 +16,10 @@
 // of up to eight CTAs that divide a block's keys and join their sums through each other's shared memory: one launch, no scratch.
 //
 // Bound by the latency of a tile's chain - scores, softmax, weights - on two CTAs: 2368 rows over 14000 tokens, 16 / 8 heads of 128, 263 us
-// (1110 TFLOP/s), 1050 cycles of an SM per tile where the products take 660 and the exponentials 510; heads of 64: 211 us.  Tried, not
+// (1110 TFLOP/s), 1050 cycles of an SM per tile where the products take 660 and the exponentials 510; heads of 64: 264 us.  Tried, not
 // kept: three stages of V and two of K (drafts 118 -> 124 us), four of each with one CTA per SM (161), up to 32 rows four times in the block
 // with a quarter of a tile's keys for each warp (no change), a third buffer of S for heads of 64 (no change), the next tile's scores asked
-// for before this one's weights are handed over (211 -> 223: a slow warp's weights hold up the others').
+// for before this one's weights are handed over (heads of 64 with one part: 211 -> 223; a slow warp's weights hold up the others').
 #include <math.h>
 
 #include <mutex>
@@ -40,7 +41,37 @@ constexpr int kSmem = kOffSearch + (int)sizeof(PortionSearch);
 // fp16 holds, and normal numbers down to 2^-21 of the largest, where they would be subnormal from 2^-14 on (what is
 // left out below is 2^-32).
 constexpr float kLazyLog2 = 8.0f, kLift = 7.0f;
+// Heads below 128 hold their weights in two fp16 parts, and O starts anew every kFlushTiles tiles, 1024 keys, since the tensor core's sums
+// truncate: as prompts over contiguous keys have it (prefill_attn.cu), so that a prompt is as precise in portions as at once.  Its error
+// against 64 bits is the result's rounding, 2.1e-4 (with one part 2.9e-4).  2368 rows over 14000 tokens, heads of 64, two queries each:
+// 213 us with one part, 250 with two, 264 with the sums as well; three portions of 700 to 1900 rows, three queries each, window of 2048:
+// 131, 154 and 160.  Heads of 128 hold one part in one sum, as there and as decoding does: 263 us, with two parts 328, with the sums 366.
+constexpr int kFlushTiles = 16;
 constexpr int kOffMl = kM * (kD + 4) * 4;  // of a cluster's part: (maximum, denominator) behind its sums, both where tiles were
+
+// Two fp16 parts of a pair of weights: hi + lo holds 22 bits of each.
+__device__ __forceinline__ uint32_t split_half2(float a, float b, uint32_t &lo) {
+  const __half2 hi = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(hi);
+  lo = pack_half2(a - f.x, b - f.y);
+  return *reinterpret_cast<const uint32_t *>(&hi);
+}
+
+// What O holds joins a thread's sums in local memory, kept in fp32 with the rescaling they still owe.  (Out of line, so that the sums stay
+// out of the registers of the loop that calls it.)
+__device__ __noinline__ void flush_sums(float4 *sums, uint32_t tmem_o, int d, bool first, float owed) {
+#pragma unroll 1
+  for (int c = 0; c * 32 < d; ++c) {
+    uint32_t r[32];
+    tmem_ld32(tmem_o + c * 32, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 old = first ? make_float4(0.f, 0.f, 0.f, 0.f) : sums[c * 8 + i];
+      sums[c * 8 + i] = make_float4(fmaf(old.x, owed, __uint_as_float(r[4 * i])), fmaf(old.y, owed, __uint_as_float(r[4 * i + 1])),
+                                    fmaf(old.z, owed, __uint_as_float(r[4 * i + 2])), fmaf(old.w, owed, __uint_as_float(r[4 * i + 3])));
+    }
+  }
+}
 
 // A peer's shared memory in the cluster.
 __device__ __forceinline__ uint32_t peer_address(uint32_t address, int rank) {
@@ -127,6 +158,7 @@ __device__ __forceinline__ void join_cluster(const PortionParams &p, const Porti
 // stage, bar_s (S_j ready, per buffer), bar_p (P_j written, per buffer, one arrival per softmax warp that has rows), bar_o (P_j.V_j
 // done), bar_fin (the last of them: the softmax warps skip phases of bar_o, and a wait by parity there would alias).  Every wait is
 // bounded.
+template <bool kNarrow>
 __global__ void __launch_bounds__(kThreads, 2)
 portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PortionParams p) {
@@ -261,8 +293,11 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const uint64_t dvs = dv + (uint64_t)(sv * (kTileBytes >> 4));
         if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kN / 16; ++ks)
-            umma_f16_ts(tmem_o, tmem + s * kN + ks * 8, dvs + (uint64_t)(ks * (2048 >> 4)), idesc_pv, j > 0 || ks > 0);
+          for (int part = 0; part < (kNarrow ? 2 : 1); ++part)
+#pragma unroll
+            for (int ks = 0; ks < kN / 16; ++ks)
+              umma_f16_ts(tmem_o, tmem + s * kN + part * (kN / 2) + ks * 8, dvs + (uint64_t)(ks * (2048 >> 4)), idesc_pv,
+                          (kNarrow ? j % kFlushTiles != 0 : j > 0) || part > 0 || ks > 0);
           umma_commit(bar_o);
           umma_commit(&empty_v[sv]);
           if (j == nkv - 1) umma_commit(bar_fin);
@@ -293,11 +328,13 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool there = token < block.rows;
     // Rows that are none (a group that does not divide 128, the last block of a sequence) are left unmasked: what they compute is stored
     // nowhere and moves no maximum, and a mask for one row costs its warp 200 instructions with every tile (heads of 64, three to a KV
-    // head, 2368 rows over 14000 tokens: 538 us, and 398 so).
+    // head in one part, 2368 rows over 14000 tokens: 538 us, and 398 so).
     const int pos = block.first_pos + token, key_end = there ? min(pos + 1, block.key_limit) : 0x7fffffff;
     const int key_begin = there && p.window ? max(0, pos + 1 - p.window) : 0;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     float m_run = -INFINITY, l_run = 0.f;
+    float4 sums[kNarrow ? kD / 4 : 1];  // what flush_sums has taken, and the factor it has to be multiplied with
+    float owed = 1.f;
     bool ok = true;
     for (int j = 0; j < nkv && ok; ++j) {
       const int sb = j & 1;
@@ -330,31 +367,42 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       uint64_t sum2[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t packed[16];
+        uint32_t packed[16], low[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1])), scale2, shift2));
           const float a = fast_exp2(x.x), b = fast_exp2(x.y);
           sum2[(i >> 1) & 3] = add_f32x2(sum2[(i >> 1) & 3], pack_f32x2(a, b));
-          packed[i >> 1] = pack_half2(a, b);
+          if (kNarrow)
+            packed[i >> 1] = split_half2(a, b, low[i >> 1]);
+          else
+            packed[i >> 1] = pack_half2(a, b);
         }
         tmem_st16(tmem + sb * kN + lane_base + c * 16, packed);
+        if (kNarrow) tmem_st16(tmem + sb * kN + lane_base + kN / 2 + c * 16, low);
       }
       const float2 sum = unpack_f32x2(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])));
       l_run = l_run * corr + (sum.x + sum.y);
       // O moves with the maximum once P_{j-1}.V_{j-1} is done (P_j.V_j waits for this warp, so the barrier is at most a phase ahead)
-      if (j > 0 && moved) {
+      const bool flush = kNarrow && j > 0 && j % kFlushTiles == 0;  // P_j.V_j starts O anew
+      if (j > 0 && (moved || flush)) {
         ok = mbar_wait_warp(bar_o, (j - 1) & 1, abort_flag, p.wait_ns);
         if (!ok) break;
         tc_fence_after();
+        if (flush) {
+          flush_sums(sums, tmem_o + lane_base, p.d, j == kFlushTiles, owed);
+          owed = corr;
+        } else {
+          if (kNarrow) owed *= corr;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 >= p.d) break;
-          uint32_t r[32];
-          tmem_ld32(tmem_o + lane_base + c * 32, r);
+          for (int c = 0; c < 4; ++c) {
+            if (c * 32 >= p.d) break;
+            uint32_t r[32];
+            tmem_ld32(tmem_o + lane_base + c * 32, r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-          tmem_st32(tmem_o + lane_base + c * 32, r);
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+            tmem_st32(tmem_o + lane_base + c * 32, r);
+          }
         }
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -364,6 +412,14 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
     if (ok && nkv > 0) ok = mbar_wait_warp(bar_fin, 0, abort_flag, p.wait_ns);
     tc_fence_after();
+    const auto load_o = [&](int c, uint32_t (&r)[32]) {
+      tmem_ld32(tmem_o + lane_base + c * 32, r);
+      if (kNarrow && nkv > kFlushTiles) {
+        const float *old = reinterpret_cast<const float *>(sums) + c * 32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(fmaf(old[i], owed, __uint_as_float(r[i])));
+      }
+    };
     const int row = block.row0 + token;
     const bool divided = block.parts > 1;
     const int key0 = max(key_begin, tile0 * kN), key1 = min(key_end, (tile0 + nkv) * kN);
@@ -374,16 +430,16 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       else if (divided && there)
         p.ml[place] = portion_ml_given_up();
     } else if (p.cluster > 1) {
-      float *sums = reinterpret_cast<float *>(smem) + threadIdx.x * (p.d + 4);
+      float *dst = reinterpret_cast<float *>(smem) + threadIdx.x * (p.d + 4);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (c * 32 >= p.d || nkv == 0) break;
         uint32_t r[32];
-        tmem_ld32(tmem_o + lane_base + c * 32, r);
+        load_o(c, r);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
           if (c * 32 + u * 4 < p.d)
-            *reinterpret_cast<uint4 *>(sums + c * 32 + u * 4) = make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
+            *reinterpret_cast<uint4 *>(dst + c * 32 + u * 4) = make_uint4(r[u * 4], r[u * 4 + 1], r[u * 4 + 2], r[u * 4 + 3]);
       }
       reinterpret_cast<float2 *>(smem + kOffMl)[threadIdx.x] = portion_ml(m_run, l_run, nkv > 0 && key0 < key1);
     } else if (nkv == 0 && there) {  // no key at all
@@ -397,7 +453,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       for (int c = 0; c < 4; ++c) {
         if (c * 32 >= p.d) break;
         uint32_t r[32];
-        tmem_ld32(tmem_o + lane_base + c * 32, r);
+        load_o(c, r);
         if (there) {
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
@@ -455,6 +511,37 @@ bool encode(CUtensorMap *map, const void *base, int rank, const cuuint64_t *dims
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <bool kNarrow>
+int launch(const PortionParams &p, const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
+  static std::mutex mu;
+  static bool opted[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return AXB200_DEVICE_ERROR;
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (!opted[dev] && cudaFuncSetAttribute(portion_umma_kernel<kNarrow>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+      return AXB200_DEVICE_ERROR;
+    opted[dev] = true;
+  }
+  if (p.cluster == 1)
+    return launch_dependent(portion_umma_kernel<kNarrow>, dim3((unsigned)(p.units * p.hkv)), dim3(kThreads), kSmem, st, mq, mk, mv, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.units * p.hkv * p.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)p.cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, portion_umma_kernel<kNarrow>, mq, mk, mv, p) == cudaSuccess) return AXB200_OK;
+  cudaGetLastError();
+  return AXB200_DEVICE_ERROR;
+}
+
 }  // namespace
 
 int portions_umma(const PortionParams &p, cudaStream_t st) {
@@ -468,33 +555,7 @@ int portions_umma(const PortionParams &p, cudaStream_t st) {
   if (!tensor_map_encoder() || !encode(&mq, p.q, 3, q_dims, q_strides, q_box) || !encode(&mk, p.k_pages, 4, dims, strides, box) ||
       !encode(&mv, p.v_pages, 4, dims, strides, box))
     return AXB200_INTERNAL_ERROR;
-  static std::mutex mu;
-  static bool opted[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return AXB200_DEVICE_ERROR;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (!opted[dev] && cudaFuncSetAttribute(portion_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
-      return AXB200_DEVICE_ERROR;
-    opted[dev] = true;
-  }
-  if (p.cluster == 1)
-    return launch_dependent(portion_umma_kernel, dim3((unsigned)(p.units * p.hkv)), dim3(kThreads), kSmem, st, mq, mk, mv, p);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.units * p.hkv * p.cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {(unsigned)p.cluster, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, portion_umma_kernel, mq, mk, mv, p) == cudaSuccess) return AXB200_OK;
-  cudaGetLastError();
-  return AXB200_DEVICE_ERROR;
+  return p.d < kD ? launch<true>(p, mq, mk, mv, st) : launch<false>(p, mq, mk, mv, st);
 }
 
 }  // namespace axb

@@ -431,7 +431,10 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
  *     counts the portion.  A row that sees no key gets zeros; keys and values that a row does not see, and what stands behind a sequence's
  *     end, do not touch it whatever they are.  Rows whose result is not finite, and in FLOAT32 blocks with values that are not finite,
- *     above 3.39e38 or, unless zero, below 2^-100, are computed a second time without the tensor cores, at that speed.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
+ *     above 3.39e38 or, unless zero, below 2^-100, are computed a second time without the tensor cores, at that speed.  Scores, maxima and
+ *     sums are fp32; weights meet the values in fp32 (FLOAT32), in 22 bits (FLOAT16, heads below 128) or rounded to FLOAT16 (heads of 128,
+ *     as axb200_sdpa and decoding have them), and in fp32 wherever the FMA pipe serves a FLOAT16 call: heads above 128 or not a multiple of
+ *     8, more than 128 query heads to a KV head, operands that do not start on 16 bytes.  max_seq_len bounds the lengths and sizes the grid; a longer sequence
  *     sets AXB200_ERR_CAPACITY and its keys beyond are not read.  FLOAT16, FLOAT32.  workspace: at least the bytes that
  *     portions_workspace_bytes gives for the same arguments (0: none; aligned: q, out and the pages start on 16 bytes), itself 16-byte
  *     aligned, of this call alone until its kernels are done. */

@@ -862,3 +862,46 @@ def test_extending_by_new_numbers_of_rows_makes_no_trial_products():
     tower.decode_step()
     assert timed and set(timed) == {3}
     assert ops.last_error() == 0
+
+
+def narrow_tolerance(ref, mag, top, keys, largest):
+    """What `attend_tolerance` counts for scores, exponentials and the result's rounding; weights in two fp16 parts, off by 2^-22 of themselves
+    and 2^-32 of the largest where a part is subnormal; and the tensor core's sums over 1024 keys at most, 8 products to 64 of them, each of
+    which drops less than a unit of the last place, 2^-23 of what is added up: 128 * 2^-23."""
+    half = torch.finfo(torch.float16).eps / 2
+    return ref.abs() * half * (1 + 2.0 ** -10) + mag * (2.0 ** -21 * (2 + 2 * top) + 2.0 ** -22 + 2.0 ** -16) + 2.0 ** -32 * keys * largest + \
+        torch.finfo(torch.float16).smallest_normal * half
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (6, 2, 80), (3, 1, 96), (4, 2, 40), (2, 2, 8), (8, 1, 120)])
+def test_weights_of_narrow_heads_keep_more_than_their_type(hq, hkv, d):
+    """Few keys that carry the weight, where a rounded weight would show: whole blocks, clusters, parts."""
+    from axono_b200 import ops
+
+    for counts, cached in (((200, 3), (0, 60)), ((90,), (600,)), ((20, 2), (7000, 40))):
+        for window in (0, 50):
+            q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, torch.float16, window=window, spread=3.0)
+            for rows, ref, mag, top in attend_all(q, cache, counts, starts, window):
+                tol = narrow_tolerance(ref, mag, top, max(cached) + max(counts), max(float(v.abs().max()) for v in cache.v))
+                err = (out[rows].double() - ref).abs()
+                assert (err <= tol).all(), float((err / tol).max())
+    assert ops.last_error() == 0
+
+
+def test_long_sums_of_narrow_heads_are_not_pulled_towards_zero():
+    """16384 keys in a row, values with a common offset: each product of the tensor core drops a part of a last bit, always towards zero, so
+    that one sum over all keys is too small by 2^-15.  Sums over 1024 keys stay within 2^-16 of the whole, 128 products of less than 2^-23
+    each; rounding the result is not biased: its mean over n elements is within four times 2^-11 / sqrt(3 n) of zero."""
+    from axono_b200 import ops
+
+    hq = hkv = 64  # three blocks per head: more than half of what runs at once, so that keys are not divided
+    counts, cached, d = (384,), (16000,), 64
+    cache = Cache([16384], hkv, d, torch.float16)
+    cache.v[0].mul_(0.25).add_(1.0)
+    cache.write(0, 0, cache.k[0], cache.v[0])
+    assert ops._portions_workspace_bytes(384, 1, hq, hkv, d, 64, cache.table.shape[1], 16384, 0, True, 0) == 0
+    q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, torch.float16, cache=cache, spread=0.5)
+    [(rows, ref, mag, top)] = attend_all(q, cache, counts, starts)
+    bias = float(((out[rows].double() - ref) / ref).mean())
+    assert abs(bias) <= 2.0 ** -16 + 4 * 2.0 ** -11 / math.sqrt(3 * ref.numel()), bias
+    assert ops.last_error() == 0
