@@ -905,3 +905,182 @@ def test_long_sums_of_narrow_heads_are_not_pulled_towards_zero():
     bias = float(((out[rows].double() - ref) / ref).mean())
     assert abs(bias) <= 2.0 ** -16 + 4 * 2.0 ** -11 / math.sqrt(3 * ref.numel()), bias
     assert ops.last_error() == 0
+
+
+# ---- what the cases above do not reach ------------------------------------------------------------------------------
+
+EDGES = {  # counts, cached, query and KV heads: how the keys are divided is a function of these
+    "whole": ((300, 130), (0, 10), 4, 2), "clusters of two": ((3,) * 16, (900,) * 16, 16, 8), "clusters of four": ((4,), (296,), 4, 2),
+    "clusters of eight": ((13,), (1500,), 4, 2), "a long cluster": ((20,), (5000,), 4, 2), "parts": ((20, 1, 3), (7000, 30, 6500), 4, 2),
+    "parts of a long cache": ((2,), (70000,), 2, 1), "parts of full blocks": ((640,), (9000,), 2, 1)}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128, 20])
+@pytest.mark.parametrize("what", EDGES)
+def test_no_key_is_lost_or_doubled_where_tiles_meet(what, d, dtype):
+    """All the weight on the first and last key of every tile of 64, in equal shares: a key that is missing or counts twice changes a row by
+    a share of it, many times the tolerance."""
+    from axono_b200 import ops
+
+    counts, cached, hq, hkv = EDGES[what]
+    lens = [n + c for n, c in zip(counts, cached)]
+    cache = Cache(lens, hkv, d, dtype, seed=4)
+    u = torch.ones(d, device="cuda", dtype=torch.float64) / math.sqrt(d)
+    height = 4.0 * d ** 0.25  # scores of +-16
+    # with fp16 weights the tolerance is 2^-11 of the mean |value|, so that no more than a few hundred keys may share the weight: every
+    # `apart`-th tile at a time
+    apart = -(-max(lens) // 16384)
+    starts, rows = row_table(counts), sum(counts)
+    q = (height * u).expand(rows, hq, d).to(dtype).contiguous()
+    q += (2.0 ** -6 * torch.randn(q.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")).to(dtype)
+    for phase in range(apart):
+        for b, n in enumerate(lens):
+            at = torch.arange(n, device="cuda")
+            edge = (((at % 64 == 0) | (at % 64 == 63)) & (at // 64 % apart == phase)).double() * 2 - 1
+            cache.k[b] = (height * edge[:, None, None] * u).expand(n, hkv, d).to(dtype).contiguous()
+            cache.write(b, 0, cache.k[b], cache.v[b])
+        out = ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, max(lens))
+        for r, ref, mag, top in attend_all(q, cache, counts, starts.tolist()):
+            tol = attend_tolerance(dtype, ref, mag, top)
+            err = (out[r].double() - ref).abs()
+            assert (err <= tol).all(), float((err / tol).max())
+            if len(counts) == 1:  # that a key's share stands out from the tolerance
+                assert 0.5 * float(cache.v[0].abs().mean()) / (2 * lens[0] / 64 / apart) > 2 * float(tol.median())
+    assert ops.last_error() == 0
+
+
+@pytest.mark.parametrize("lens,bound,parts", [((700, 650, 90), 800, False), ((6100, 9000, 130), 9100, True)])
+def test_a_replayed_step_with_clusters_and_with_parts(lens, bound, parts):
+    """Captured once, replayed over a cache that grows past the edges of tiles and pages and over rows that move from one sequence to another:
+    the bits of eager calls, with the keys divided in clusters and in parts that a second kernel joins."""
+    from axono_b200 import ops
+
+    hq, hkv, d, rows, steps = 4, 2, 128, 6, 24
+    caches = [Cache(lens, hkv, d, torch.float16, more=rows * steps, poison=0.0) for _ in range(2)]
+    blocks = caches[0].table.shape[1]
+    assert (ops._portions_workspace_bytes(rows, 3, hq, hkv, d, 64, blocks, bound, 0, True, 0) > 0) == parts
+    starts, f = row_table([2, 2, 2]), freqs(d)
+    qkv = torch.zeros((rows, (hq + 2 * hkv) * d), dtype=torch.float16, device="cuda")
+    out = torch.empty((rows, hq, d), dtype=torch.float16, device="cuda")
+
+    def step(c, out=None):
+        q = ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, c.k_pages, c.v_pages, c.table, c.lens, starts, inv_freq=f)
+        return ops.gqa_attention_portions_paged(q, c.k_pages, c.v_pages, c.table, c.lens, starts, bound, out=out)
+
+    first = caches[0].lens.clone()
+    step(caches[0], out)
+    caches[0].lens.copy_(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(caches[0], out)
+    for i in range(steps):
+        starts.copy_(row_table([(2, 2, 2), (6, 0, 0), (0, 1, 5), (1, 4, 1)][i % 4]))
+        qkv.copy_(rnd(qkv.shape, torch.float16, i))
+        graph.replay()
+        assert torch.equal(out, step(caches[1])), i
+    assert torch.equal(caches[0].lens, caches[1].lens) and int(caches[0].lens.sum()) == sum(lens) + rows * steps
+    assert torch.equal(caches[0].k_pages, caches[1].k_pages) and torch.equal(caches[0].v_pages, caches[1].v_pages)
+    counts = [1, 4, 1]
+    for b in range(3):
+        caches[1].k[b], caches[1].v[b] = caches[1].read(b, 0, int(caches[1].lens[b]))
+    pos = torch.cat([torch.arange(int(n) - c, int(n)) for n, c in zip(caches[1].lens, counts)]).cuda()
+    q = ops.qk_norm_rope(qkv[:, :hq * d].view(rows, hq, d), None, pos, f)[0]
+    check_attention(q, caches[1], counts, starts.tolist(), out)
+    assert ops.last_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_positions_beyond_32_bits(interleaved, dtype):
+    """Frequencies of 2 pi / (3 * 2^k), for which a position's turns are known exactly: their upper 32 bits matter (2^32 is no multiple of
+    3 * 2^k).  The product in double is off by 2^-52 of the turns, thrice."""
+    from axono_b200 import ops
+
+    rows, d, n = 50, 64, 32
+    k = torch.arange(n) % 12 + 4
+    period = 3 * 2 ** k.long()
+    f = (2 * math.pi / period.double()).cuda()
+    for far in (1 << 33, 1 << 36):
+        pos = far + torch.randint(0, far, (rows,), generator=torch.Generator().manual_seed(5))
+        turns = (pos[:, None] % period).double() / period  # exact but for one rounding
+        x = rnd((rows, 2, d), dtype, 1)
+        out, _ = ops.qk_norm_rope(x, None, pos.cuda(), f, interleaved=interleaved)
+        c, s = (2 * math.pi * turns).cos().cuda()[:, None], (2 * math.pi * turns).sin().cuda()[:, None]
+        xd = x.double()
+        a, b = (xd[..., ::2], xd[..., 1::2]) if interleaved else (xd[..., :n], xd[..., n:])
+        pair = (a * c - b * s, b * c + a * s)
+        ref = torch.stack(pair, -1).flatten(-2) if interleaved else torch.cat(pair, -1)
+        slack = 2 * math.pi * 2 * far / 48 * 2.0 ** -52 * 3
+        half = torch.finfo(dtype).eps / 2
+        assert ((out.double() - ref).abs() <= ref.abs() * half * (1 + 2.0 ** -10) + ref.abs().amax(-1, keepdim=True) * (2.0 ** -20 + slack)).all()
+
+
+def test_far_keys_of_portions_and_of_single_tokens():
+    """Single tokens are turned by the product of position and frequency in fp32, off by half a step, 2^-24 of the angle; portions by the
+    angle itself.  So a key of either stands within that of the other, at any position of a long context."""
+    from axono_b200 import ops
+
+    hq, hkv, d, theta = 2, 2, 128, 1e6
+    f = ops.reference_frequencies(d, theta)
+    for at in (129, 4000, 30000, 131071):
+        qkv = rnd((1, (hq + 2 * hkv) * d), torch.float32, at)
+        caches = [Cache([5], hkv, d, torch.float32, more=1) for _ in range(2)]
+        pos = torch.tensor([at], device="cuda")
+        q1 = ops.qkv_norm_rope_append(qkv, hq, None, None, EPS, caches[0].k_pages, caches[0].v_pages, caches[0].table, caches[0].lens, pos=pos,
+                                      theta=theta)
+        q2 = ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, caches[1].k_pages, caches[1].v_pages, caches[1].table, caches[1].lens,
+                                               row_table([1]), pos=pos, inv_freq=f)
+        angle = (at * f * 2.0 ** -24).repeat(2)
+        for a, b in ((q1, q2), (caches[0].read(0, 5, 1)[0], caches[1].read(0, 5, 1)[0])):
+            a, b = a.double().view(-1, d), b.double().view(-1, d)
+            size = (b[:, :d // 2].square() + b[:, d // 2:].square()).sqrt().repeat(1, 2)
+            assert ((a - b).abs() <= size * (angle * (1 + 2.0 ** -10) + 2.0 ** -20)).all()
+    assert ops.last_error() == 0
+
+
+def test_tower_whose_heads_are_shared_between_two_ranks_extends():
+    """Two ranks as threads of this process, each with half of the heads; what they gather goes through the host's barrier.  (No kernel
+    waits for another rank's.)"""
+    import threading
+
+    from axono_b200 import ops, sharding
+    from axono_b200.decode import TextTower, TextTowerConfig
+
+    cfg = TextTowerConfig(hidden=256, intermediate=512, n_q_heads=8, n_kv_heads=4, head_dim=64, vocab=500, n_layers=2, use_mrope=False)
+    make = lambda world, rank: TextTower(cfg, 2, 320, dtype=torch.float32, seed=3, world=world, rank=rank, fused_gather=False)  # noqa: E731
+    towers, one, barrier, shares, me = [make(2, r) for r in range(2)], make(1, 0), threading.Barrier(2, timeout=60), {}, threading.local()
+
+    def gather(attn):
+        shares[me.rank] = attn
+        barrier.wait()
+        whole = torch.cat([shares[r] for r in range(2)], 1)
+        barrier.wait()
+        return whole
+
+    steps, results, errors = [([70, 3], 73), ([1, 0], 1), ([5, 130], 135)], {}, []
+
+    def run(rank):
+        try:
+            me.rank = rank
+            for i, (counts, n) in enumerate(steps):
+                results[rank, i] = (towers[rank].extend(torch.arange(n) * 7 % 500, counts), towers[rank].last_logits)
+        except BaseException as e:  # noqa: BLE001 - the other rank must not wait for good
+            errors.append(e)
+            barrier.abort()
+
+    inner = sharding.all_gather_heads
+    sharding.all_gather_heads = gather
+    try:
+        threads = [threading.Thread(target=run, args=(r,)) for r in range(2)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        sharding.all_gather_heads = inner
+    assert not errors, errors
+    for i, (counts, n) in enumerate(steps):
+        nxt = one.extend(torch.arange(n) * 7 % 500, counts)
+        for rank in range(2):
+            assert torch.equal(results[rank, i][0], nxt)
+            assert (results[rank, i][1] - one.last_logits).abs().max() <= 1e-4 * one.last_logits.abs().max()
+    assert ops.last_error() == 0
