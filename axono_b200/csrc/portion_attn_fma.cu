@@ -1,5 +1,6 @@
-// Attention of portions over a paged cache on the FMA pipe: FLOAT32, and FLOAT16 head sizes or alignments that the tensor-core kernel
-// does not take; head sizes up to 256.
+// Attention of portions over a paged cache on the FMA pipe: FLOAT16 and FLOAT32 for the sizes and alignments that the tensor-core kernels
+// do not take - heads of 129 to 256, others that are not a multiple of 8 (FLOAT32: 4), more than 128 query heads to a KV head, operands
+// that do not start on 16 bytes.
 //
 // One CTA per block of 64 virtual rows - rows of one sequence times the query heads of one KV head, which share every staged tile -
 // and part of its keys.  Per 32 keys: K and V rows into shared memory as fp32, scores with thread = (row, 8 keys), the running maximum
@@ -13,18 +14,24 @@ namespace {
 
 constexpr int kRows = 64, kKeys = 32, kThreads = 256, kMaxD = 256, kScoreStride = kKeys + 4;
 
-__host__ __device__ inline int row_stride(int d) { return (d + 3) / 4 * 4 + 4; }  // 16-byte rows, an odd number of 16 bytes apart
-inline size_t smem_bytes(int d) { return sizeof(float) * ((size_t)(kRows + 2 * kKeys) * row_stride(d) + (size_t)kRows * kScoreStride); }
+// Rows of d4 times 16 bytes, an odd number of these apart, so that the rows that a warp's lanes read together lie on different banks: d4 where
+// it is odd, else one more (500 rows over 2500 keys, 8 / 4 heads of 250: 63 apart 1137 us, 64 apart 2075).  kOdd is a constant of the
+// kernel: told apart inside, heads of 256 take 1225 us in the place of 1135.
+__host__ __device__ inline int row_stride(int d4, bool odd) { return odd ? d4 * 4 : d4 * 4 + 4; }
+inline size_t smem_bytes(int d) {
+  const int d4 = (d + 3) / 4;
+  return sizeof(float) * ((size_t)(kRows + 2 * kKeys) * row_stride(d4, d4 % 2) + (size_t)kRows * kScoreStride);
+}
 
 // Heads of a KV head that one CTA takes, and the rows that fit beside them.
 __host__ __device__ inline int heads_at_once(int group) { return group < kRows ? group : kRows; }
 
-template <typename T, bool kSplit>
+template <typename T, bool kSplit, bool kOdd>
 __global__ void __launch_bounds__(kThreads)
 portion_fma_kernel(const PortionParams p) {
   extern __shared__ __align__(16) float smem[];
   __shared__ PortionSearch search;
-  const int ld = row_stride(p.d), d4 = (p.d + 3) / 4;
+  const int d4 = (p.d + 3) / 4, ld = row_stride(d4, kOdd);
   float *q_s = smem, *k_s = q_s + kRows * ld, *v_s = k_s + kKeys * ld, *p_s = v_s + kKeys * ld;
   grid_dependency_launch();
   grid_dependency_wait();
@@ -138,8 +145,8 @@ portion_fma_kernel(const PortionParams p) {
   }
 }
 
-template <typename T, bool kSplit>
-int launch(const PortionParams &p, cudaStream_t st) {
+template <typename T, bool kSplit, bool kOdd>
+int launch_stride(const PortionParams &p, cudaStream_t st) {
   static std::mutex mu;
   static size_t opted[64] = {0};
   int dev = 0;
@@ -148,7 +155,7 @@ int launch(const PortionParams &p, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> lock(mu);
     if (opted[dev] < smem) {
-      if (cudaFuncSetAttribute(portion_fma_kernel<T, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      if (cudaFuncSetAttribute(portion_fma_kernel<T, kSplit, kOdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return AXB200_DEVICE_ERROR;
       opted[dev] = smem;
     }
@@ -156,7 +163,12 @@ int launch(const PortionParams &p, cudaStream_t st) {
   const int at_once = heads_at_once(p.group), slices = (p.group + at_once - 1) / at_once;
   const int64_t ctas = (int64_t)p.units * p.hkv * slices;
   if (ctas > 0x7fffffff) return AXB200_INVALID_ARGUMENT;
-  return launch_dependent(portion_fma_kernel<T, kSplit>, dim3((unsigned)ctas), dim3(kThreads), smem, st, p);
+  return launch_dependent(portion_fma_kernel<T, kSplit, kOdd>, dim3((unsigned)ctas), dim3(kThreads), smem, st, p);
+}
+
+template <typename T, bool kSplit>
+int launch(const PortionParams &p, cudaStream_t st) {
+  return (p.d + 3) / 4 % 2 ? launch_stride<T, kSplit, true>(p, st) : launch_stride<T, kSplit, false>(p, st);
 }
 
 }  // namespace
