@@ -73,12 +73,13 @@ __device__ __forceinline__ void place_row(const TurnParams &p, int64_t row, RowP
   int64_t here = 0;  // the row's slot, which is its position where none is given, even where the portion does not fit
   if constexpr (kAppend) {
     const int lane = threadIdx.x & 31;
+    int r0, r1;
     bool falls;
-    const int b = portion_sequence(p.row_start, p.batch, (int)p.rows, row, falls);
+    const int b = portion_sequence(p.row_start, p.batch, (int)p.rows, row, r0, r1, falls);
     if (falls && lane == 0) atomicOr(&g_error_word, AXB200_ERR_BAD_ROWS);
     place.alive = false;
     if (b < 0) return;  // a row of no sequence
-    const int r0 = p.row_start[b], r1 = p.row_start[b + 1], len = p.seq_lens[b];
+    const int len = p.seq_lens[b];
     place.alive = true;
     const int64_t first = first_slot(p, b, len, r1 - r0);
     here = (first >= 0 ? first : p.advance || p.slots ? (int64_t)len : (int64_t)len - (r1 - r0)) + (row - r0);

@@ -19,10 +19,11 @@ join_portions_kernel(const PortionParams p) {
   grid_dependency_launch();
   grid_dependency_wait();
   if (row >= p.rows) return;
-  bool falls;
-  if (portion_sequence(p.row_start, p.batch, p.rows, row, falls) < 0) return;  // a row that no CTA had: nothing was written for it
   const int parts = min(p.row_parts[row], p.parts);
   if (parts <= 1) return;
+  int r0, r1;
+  bool falls;
+  if (portion_sequence(p.row_start, p.batch, p.rows, row, r0, r1, falls) < 0) return;  // a row that no CTA had: its number of parts was not written
   float m = -INFINITY;
   for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.ml[portion_place(p, k, row, head)].x);
 #pragma unroll

@@ -12,13 +12,14 @@ __device__ __forceinline__ bool portion_counts_up(int r0, int r1, int rows, int 
   return r0 >= 0 && r0 >= earlier && r1 >= r0 && r1 <= rows;
 }
 
-// The sequence of a row, found by a warp, or -1.  Its end is the first entry above the row, so that all before are not.  `falls`: the
-// table does not count up around this row (every fall does so around the rows between the two entries, if there are any).
-__device__ __forceinline__ int portion_sequence(const int32_t *row_start, int batch, int rows, int64_t row, bool &falls) {
+// The sequence of a row, found by a warp, or -1; r0, r1: its entries.  Its end is the first entry above the row, so that all before are not.
+// `falls`: the table does not count up around this row (every fall does so around the rows between the two entries, if there are any).
+__device__ __forceinline__ int portion_sequence(const int32_t *row_start, int batch, int rows, int64_t row, int &r0, int &r1, bool &falls) {
   const int lane = threadIdx.x & 31;
-  unsigned first = 0x7fffffffu;
-  int below = 0;
-  for (int i = lane; i <= batch; i += 32) {
+  const int mine = lane <= batch ? row_start[lane] : 0x7fffffff;  // of the first 32 entries, which are all there are in most launches
+  unsigned first = mine > row ? (unsigned)lane : 0x7fffffffu;
+  int below = mine <= row;
+  for (int i = lane + 32; i <= batch; i += 32) {
     if (row_start[i] <= row)
       ++below;
     else
@@ -29,10 +30,16 @@ __device__ __forceinline__ int portion_sequence(const int32_t *row_start, int ba
   falls = first <= (unsigned)batch && below != (int)first;
   if (first == 0 || first > (unsigned)batch) return -1;
   const int b = (int)first - 1;
-  int earlier = -0x7fffffff - 1;
-  for (int i = lane; i < b; i += 32) earlier = max(earlier, row_start[i]);
+  int earlier = lane < b ? mine : -0x7fffffff - 1;
+  for (int i = lane + 32; i < b; i += 32) earlier = max(earlier, row_start[i]);
   earlier = __reduce_max_sync(0xffffffffu, earlier);
-  if (portion_counts_up(row_start[b], row_start[b + 1], rows, earlier)) return b;
+  if (b < 31) {
+    r0 = __shfl_sync(0xffffffffu, mine, b);
+    r1 = __shfl_sync(0xffffffffu, mine, b + 1);
+  } else {
+    r0 = row_start[b], r1 = row_start[b + 1];
+  }
+  if (portion_counts_up(r0, r1, rows, earlier)) return b;
   falls = true;
   return -1;
 }

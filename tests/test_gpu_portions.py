@@ -1084,3 +1084,45 @@ def test_tower_whose_heads_are_shared_between_two_ranks_extends():
             assert torch.equal(results[rank, i][0], nxt)
             assert (results[rank, i][1] - one.last_logits).abs().max() <= 1e-4 * one.last_logits.abs().max()
     assert ops.last_error() == 0
+
+
+@pytest.mark.parametrize("batch", [1, 5, 30, 31, 32, 33, 64, 100])
+def test_rows_of_random_tables(batch):
+    """Tables with and without entries that do not count up, about the 32 that a warp holds at once: which rows are appended and attended,
+    and which lengths grow, by the rule for each entry by itself."""
+    from axono_b200 import ops
+
+    rows, hq, hkv, d = 90, 2, 1, 64
+    g = torch.Generator().manual_seed(batch)
+    for trial in range(12):
+        table = torch.sort(torch.randint(0, rows + 1, (batch + 1,), generator=g)).values
+        for _ in range(trial // 3):  # none in the first three
+            table[int(torch.randint(0, batch + 1, (1,), generator=g))] = int(torch.randint(-3, rows + 4, (1,), generator=g))
+        table = table.tolist()
+        up = [0 <= e <= rows and e >= max(table[:i], default=e) for i, e in enumerate(table)]
+        owner = [-1] * rows
+        for b in range(batch):
+            if up[b] and up[b + 1]:
+                for r in range(table[b], table[b + 1]):
+                    assert owner[r] == -1
+                    owner[r] = b
+        grown = [owner.count(b) for b in range(batch)]
+        cache = Cache([3] * batch, hkv, d, torch.float16, more=rows, poison=0.0)
+        qkv, starts = rnd((rows, (hq + 2 * hkv) * d), torch.float16, trial), torch.tensor(table, dtype=torch.int32, device="cuda")
+        q = torch.full((rows, hq, d), 7.0, dtype=torch.float16, device="cuda")
+        ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, out=q)
+        assert bool(ops.last_error() & 16) == (not all(up))
+        assert cache.lens.tolist() == [3 + n for n in grown]
+        out = torch.full((rows, hq, d), 7.0, dtype=torch.float16, device="cuda")
+        ops.gqa_attention_portions_paged(qkv[:, :hq * d].reshape(rows, hq, d), cache.k_pages, cache.v_pages, cache.table, cache.lens, starts,
+                                         3 + rows, out=out)
+        assert bool(ops.last_error() & 16) == (not all(up))
+        owned = torch.tensor([o >= 0 for o in owner], device="cuda")
+        assert (q[~owned] == 7).all() and (out[~owned] == 7).all()
+        assert torch.equal(q[owned], qkv[owned, :hq * d].view(-1, hq, d)) and not (out[owned] == 7).all(-1).any()
+        for b in range(batch):
+            if grown[b]:
+                k, v = cache.read(b, 3, grown[b])
+                r0 = table[b]
+                assert torch.equal(k[:, 0], qkv[r0:r0 + grown[b], hq * d:(hq + 1) * d])
+                assert torch.equal(v[:, 0], qkv[r0:r0 + grown[b], (hq + 1) * d:])
