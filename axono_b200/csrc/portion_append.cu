@@ -520,6 +520,10 @@ int axb200_qk_norm_rope(const void *q, int64_t q_ld, const void *k, int64_t k_ld
   if ((hq > 0 && q_ld < (int64_t)hq * d) || (hkv > 0 && k_ld < (int64_t)hkv * d)) return AXB200_SHAPE_MISMATCH;
   // in place where rows are contiguous: a head's threads have read it before they write
   if ((hq > 0 && q == q_out && q_ld != (int64_t)hq * d) || (hkv > 0 && k == k_out && k_ld != (int64_t)hkv * d)) return AXB200_SHAPE_MISMATCH;
+  const int64_t e = (int64_t)axb::dtype_size(dtype), q_row = (int64_t)hq * d * e, k_row = (int64_t)hkv * d * e;
+  if ((hq > 0 && q != q_out && axb::shares_memory(q, q_ld * e, q_row, rows, q_out, rows * q_row)) ||
+      (hkv > 0 && k != k_out && axb::shares_memory(k, k_ld * e, k_row, rows, k_out, rows * k_row)))
+    return AXB200_INVALID_ARGUMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, false>(p, nullptr, st)
          : dtype == AXB200_FLOAT16 ? axb::launch_turn<__half, false>(p, nullptr, st)
@@ -546,6 +550,8 @@ int axb200_qkv_norm_rope_append_portions_at(const void *qkv, int64_t ld, const v
   if (!qkv || !q_out || !k_pages || !v_pages || !block_table || !seq_lens || !row_start || (rot_dim > 0 && !inv_freq))
     return AXB200_INVALID_PTR;
   if (ld < (int64_t)(hq + 2 * hkv) * d) return AXB200_SHAPE_MISMATCH;
+  const int64_t size = (int64_t)e;
+  if (axb::shares_memory(qkv, ld * size, (int64_t)(hq + 2 * hkv) * d * size, rows, q_out, rows * hq * d * size)) return AXB200_INVALID_ARGUMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t *advanced = advance ? seq_lens : nullptr;
   return dtype == AXB200_FLOAT32 ? axb::launch_turn<float, true>(p, advanced, st) : axb::launch_turn<__half, true>(p, advanced, st);

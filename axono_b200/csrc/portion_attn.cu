@@ -206,7 +206,8 @@ int axb200_gqa_attention_portions_paged(const void *q, void *out, const void *k_
   if (hq % hkv) return AXB200_SHAPE_MISMATCH;
   if (rows == 0) return AXB200_OK;
   if (!q || !out || !k_pages || !v_pages || !block_table || !seq_lens || !row_start) return AXB200_INVALID_PTR;
-  if (q == out) return AXB200_INVALID_ARGUMENT;  // rows that are done over read their queries again
+  const int64_t row = (int64_t)hq * d * (int64_t)axb::dtype_size(dtype);
+  if (axb::shares_memory(q, row, row, rows, out, rows * row)) return AXB200_INVALID_ARGUMENT;  // rows that are done over read their queries again
   const bool tensor = axb::portion_tensor_sizes(hq / hkv, d, dtype) && axb::aligned16(q) && axb::aligned16(out) &&
                       axb::aligned16(k_pages) && axb::aligned16(v_pages);
   axb::PortionParams p =

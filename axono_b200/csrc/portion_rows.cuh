@@ -12,6 +12,14 @@ __device__ __forceinline__ bool portion_counts_up(int r0, int r1, int rows, int 
   return r0 >= 0 && r0 >= earlier && r1 >= r0 && r1 <= rows;
 }
 
+// Whether `bytes` at `other` share memory with `rows` (at least one) pieces of row_bytes that begin ld_bytes apart.
+inline bool shares_memory(const void *base, int64_t ld_bytes, int64_t row_bytes, int64_t rows, const void *other, int64_t bytes) {
+  const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(other) - reinterpret_cast<uintptr_t>(base));
+  if (at <= 0) return at + bytes > 0;
+  const int64_t row = at / ld_bytes;
+  return row < rows && (at - row * ld_bytes < row_bytes || (row + 1 < rows && at + bytes > (row + 1) * ld_bytes));
+}
+
 // The sequence of a row, found by a warp, or -1; r0, r1: its entries.  Its end is the first entry above the row, so that all before are not.
 // `falls`: the table does not count up around this row (every fall does so around the rows between the two entries, if there are any).
 __device__ __forceinline__ int portion_sequence(const int32_t *row_start, int batch, int rows, int64_t row, int &r0, int &r1, bool &falls) {

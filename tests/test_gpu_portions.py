@@ -1126,3 +1126,24 @@ def test_rows_of_random_tables(batch):
                 r0 = table[b]
                 assert torch.equal(k[:, 0], qkv[r0:r0 + grown[b], hq * d:(hq + 1) * d])
                 assert torch.equal(v[:, 0], qkv[r0:r0 + grown[b], (hq + 1) * d:])
+
+
+def test_an_output_between_the_rows_of_a_strided_product():
+    """It shares no memory with what is read, and is taken."""
+    from axono_b200 import ops
+
+    hq, hkv, d, rows = 2, 1, 64, 5
+    columns = (hq + 2 * hkv) * d
+    buf = rnd((rows, columns + rows * hq * d + 64), torch.float16, 1)
+    qkv, out = buf[:, :columns], buf.view(-1)[buf.shape[1] + columns:][:rows * hq * d].view(rows, hq, d)
+    cache = Cache([0], hkv, d, torch.float16, more=64)
+    before = qkv.clone()
+    got = ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows]), out=out)
+    assert got is out and torch.equal(out, before[:, :hq * d].view(rows, hq, d)) and torch.equal(qkv, before)
+    for bad in (buf.view(-1)[columns // 2:][:rows * hq * d].view(rows, hq, d), buf.view(-1)[columns + 128:][:rows * hq * d].view(rows, hq, d)):
+        with pytest.raises(RuntimeError):
+            ops.qkv_norm_rope_append_portions(qkv, hq, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows]), out=bad)
+    q = rnd((2 * rows, hq, d), torch.float16, 2)
+    with pytest.raises(RuntimeError):
+        ops.gqa_attention_portions_paged(q[:rows], cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows]), 64, out=q[3:3 + rows])
+    assert cache.lens.tolist() == [rows] and ops.last_error() == 0

@@ -143,3 +143,17 @@ def test_the_operators_import_where_torch_lacks_cuda_bindings():
             "from axono_b200 import ops\n"
             "assert ops._device_now is torch.cuda.current_device and callable(ops._stream_now)\n")
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+
+def test_outputs_that_share_memory_with_inputs_are_refused():
+    """Wherever the output begins in or runs into what is read - but not between the rows of a strided input."""
+    q_bytes = 4 * 4 * 64 * 2
+    for off in (2, 128, q_bytes - 2, -2, 2 - q_bytes):
+        assert attend(out=FAKE + off) == INVALID, off
+        assert turn(k=None, hkv=0, ko=None, qo=FAKE + off) == INVALID, off
+        assert turn(q=None, hq=0, qo=None, k=FAKE, k_ld=256, hkv=4, ko=FAKE + off) == INVALID, off
+    for off in (2, 4 * 512 * 2 - 2, 2 - q_bytes):
+        assert append(qo=FAKE + off) == INVALID, off
+    # rows of 1024 bytes, 8192 apart: from the gap behind one into the next
+    for off in (8192 - 512, 3 * 8192 - 512, 3 * 8192 + 1022, 2 - q_bytes):
+        assert append(ld=4096, qo=FAKE + off) == INVALID, off
