@@ -9,7 +9,7 @@
 //
 // Masks: a row sees the keys up to its own and, with a window, only the last of them.  Scores of other keys become -inf.  Their values
 // still meet weights of zero in P.V, so rows of V behind the sequence's end, where anything may stand, are cleared in shared memory
-// before the product, and rows that are not finite are done over without them (redo_portion_row).
+// before the product, and rows that are not finite are done over without them (redo_portion_row), like those whose scores are too large.
 //
 // Few rows leave most of the 128 empty: their warps stay out, and the products, which take as long as full ones, keep up with memory all
 // the same (37 sequences of 16384 tokens, a row each, 8 KV heads: 350 us, 7.1 TB/s; 10.1 from L2).  A short call's few blocks are clusters
@@ -48,6 +48,10 @@ constexpr float kLazyLog2 = 8.0f, kLift = 7.0f;
 // 131, 154 and 160.  Heads of 128 hold one part in one sum, as there and as decoding does: 263 us, with two parts 328, with the sums 366.
 constexpr int kFlushTiles = 16;
 constexpr int kOffMl = kM * (kD + 4) * 4;  // of a cluster's part: (maximum, denominator) behind its sums, both where tiles were
+
+// Whether a row's maximum is so large, of either sign, that its weights may not be what they should: a score's exponent is the exact product
+// less the maximum, which is rounded, and from 2^24 on by more than a half.  (Inputs of thousands throughout.  Such a row is done over.)
+__device__ __forceinline__ bool maximum_too_large(float m) { return fabsf(m) > 0x1p24f && m != -INFINITY; }
 
 // Two fp16 parts of a pair of weights: hi + lo holds 22 bits of each.
 __device__ __forceinline__ uint32_t split_half2(float a, float b, uint32_t &lo) {
@@ -125,9 +129,10 @@ __device__ __forceinline__ void join_cluster(const PortionParams &p, const Porti
     float l = there ? weight * part.y : 0.f;
 #pragma unroll
     for (int off = kSize >> 1; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    const unsigned far = __ballot_sync(0xffffffffu, maximum_too_large(m));
     const unsigned use = __ballot_sync(0xffffffffu, there), some = __ballot_sync(0xffffffffu, part.y != 0.f);
     const float inv = portion_inverse(l, ((some >> (mine - mine % kSize)) & ((1u << kSize) - 1)) != 0);
-    unsigned bad = 0;  // rows whose sums are not finite
+    unsigned bad = 0;  // rows whose sums are not finite, or may be wrong
 #pragma unroll
     for (int r = 0; r < kLoads / kSize; ++r) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -139,6 +144,7 @@ __device__ __forceinline__ void join_cluster(const PortionParams &p, const Porti
       }
       const float scale = __shfl_sync(0xffffffffu, inv, r * kSize);
       const int place = __shfl_sync(0xffffffffu, at, r * kSize);
+      if ((far >> (r * kSize)) & 1) bad |= 1u << r;
       if (!column || row_of(r * kSize) >= rows) continue;
       *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + (size_t)place * p.d + lane * 4) =
           make_uint2(pack_half2(o.x * scale, o.y * scale), pack_half2(o.z * scale, o.w * scale));
@@ -448,7 +454,7 @@ portion_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
     if (ok && nkv > 0 && p.cluster == 1) {
       const float inv = portion_inverse(l_run, key0 < key1);
-      float bad = 0.f;  // NaN once a sum is not finite
+      float bad = maximum_too_large(m_run) ? NAN : 0.f;  // NaN once a sum is not finite
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (c * 32 >= p.d) break;

@@ -430,7 +430,8 @@ int axb200_decode_step_host(const void *q_host, const void *k_new_host, const vo
  *   gqa_attention_portions_paged: q, out (rows, hq, d), which do not overlap: row i of sequence b's c rows, at position t = seq_lens[b] - c + i, attends the
  *     cached keys max(0, t + 1 - window) .. t (window 0: 0 .. t); scale 1 / sqrt(d), head h reads KV head h / (hq / hkv); seq_lens
  *     counts the portion.  A row that sees no key gets zeros; keys and values that a row does not see, and what stands behind a sequence's
- *     end, do not touch it whatever they are.  Rows whose result is not finite, and in FLOAT32 blocks with values that are not finite,
+ *     end, do not touch it whatever they are.  Rows whose result is not finite or whose largest
+ *     score is beyond 2^24 (times log2 e), and in FLOAT32 blocks with values that are not finite,
  *     above 3.39e38 or, unless zero, below 2^-100, are computed a second time without the tensor cores, at that speed.  Scores, maxima and
  *     sums are fp32; weights meet the values in fp32 (FLOAT32), in 22 bits (FLOAT16, heads below 128) or rounded to FLOAT16 (heads of 128,
  *     as axb200_sdpa and decoding have them), and in fp32 wherever the FMA pipe serves a FLOAT16 call: heads above 128 or not a multiple of

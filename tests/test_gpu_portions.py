@@ -1147,3 +1147,42 @@ def test_an_output_between_the_rows_of_a_strided_product():
     with pytest.raises(RuntimeError):
         ops.gqa_attention_portions_paged(q[:rows], cache.k_pages, cache.v_pages, cache.table, cache.lens, row_table([rows]), 64, out=q[3:3 + rows])
     assert cache.lens.tolist() == [rows] and ops.last_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128, 20])
+@pytest.mark.parametrize("counts,cached,hq,hkv", [((130, 4), (0, 90), 4, 2), ((3,) * 16, (900,) * 16, 16, 8), ((20,), (700,), 4, 2), ((5, 1), (7000, 64), 4, 2)])
+def test_scores_as_large_as_fp16_inputs_give(counts, cached, hq, hkv, d, dtype):
+    """Scores of 2^30 and more, positive or negative, where one key carries all the weight: the result is its value.  (Rows whose two largest
+    scores are nearer than the rounding of a sum in fp32, 2^-20 of the largest, have no such key.)"""
+    from axono_b200 import ops
+
+    lens = [n + c for n, c in zip(counts, cached)]
+    for sign in (1, -1, 0):
+        cache = Cache(lens, hkv, d, dtype, seed=6)
+        rows = sum(counts)
+        q = rnd((rows, hq, d), dtype, 5, 15000.0).clamp(-60000, 60000)
+        for b in range(len(lens)):
+            cache.k[b] = (cache.k[b].float() * 15000.0).clamp(-60000, 60000).to(dtype)
+            if sign:  # all scores of one sign
+                cache.k[b] = cache.k[b].abs()
+            cache.write(b, 0, cache.k[b], cache.v[b])
+        if sign:
+            q = q.abs() * sign
+        starts = row_table(counts)
+        out = ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, max(lens))
+        assert torch.isfinite(out).all()
+        clear = 0
+        for b, (n, c) in enumerate(zip(counts, cached)):
+            r0 = int(starts[b])
+            seen = torch.arange(lens[b], device="cuda")[None] <= c + torch.arange(n, device="cuda")[:, None]
+            for h in range(hq):
+                s = (q[r0:r0 + n, h].double() @ cache.k[b][:, h * hkv // hq].double().T).masked_fill(~seen, -math.inf)
+                top = s.topk(min(2, lens[b]), -1)
+                alone = seen.sum(1) == 1
+                gap = alone if top.values.shape[1] < 2 else alone | (top.values[:, 0] - top.values[:, 1] > 2.0 ** -20 * top.values[:, 0].abs() + 1e4)
+                want = cache.v[b][top.indices[:, 0], h * hkv // hq]
+                assert torch.equal(out[r0:r0 + n, h][gap], want[gap])
+                clear += int(gap.sum())
+        assert clear > 0.9 * rows * hq
+    assert ops.last_error() == 0
