@@ -6,9 +6,11 @@
 // formed and reduced to a part of a turn in double: at position 30000 a product rounded to fp32 is off by up to 1e-3 of a radian,
 // more than a half holds.  (The single-token operators keep the reference's rule, an fp32 product, src/ops/cpu/sequence.cpp:54-110.)
 //
-// Bound by issue (60 %) and by the way from one row to the next: 8192 rows of 16 + 8 heads of 128 in fp16 take 24.5 us, 4.1 TB/s, 1750
-// instructions per row of which about 250 are its angles.  Before: a block per row 57 us, four rows per block 36, a warp per row with its
-// loads in registers 39 (what it holds leaves 16 warps per SM); with the norms' weights held as floats 25.5.  An append of 3092 rows takes 14.9 us, one of 8 tokens 7.3 in one launch.
+// 8192 rows of 16 + 8 heads of 128 in fp16 take 24.5 us, 4.1 of 6.55 TB/s, 1750 instructions per row of which about 250 are its angles.
+// Nothing is full - issue 60 %, warps 34 % -: between two rows a warp reads position, table, length and page and forms the angles in double
+// while none of its heads goes by.  Before: a block per row 57 us, four rows per block 36, a warp per row with its loads in registers 39 (what
+// it holds leaves 16 warps per SM); with the norms' weights held as floats 25.5.  An append of 3092 rows takes 14.8 us, one of 8 tokens 7.3 in
+// one launch.
 //
 // Sequence b of a launch owns the rows row_start[b] .. row_start[b + 1] - 1; its keys and values go behind its cached tokens.  Rows
 // before the first and behind the last sequence are left alone, in the outputs too.

@@ -12,7 +12,7 @@
 // scores take 2400 cycles and its sums 1600.  K's parts have two buffers, V's one: V is split while the next scores are formed.
 //
 // Bound by the products - 4000 cycles of a tile's 5000 with heads of 128, 2400 of 2900 with heads of 64 - and by shared memory beside them,
-// which carries 416 KB of floats, parts and operands per tile, 3300 cycles.  922 rows over 5686 keys, 16 / 8 heads of 128: 162 us, of which
+// which carries 416 KB of floats, parts and operands per tile, 3300 cycles.  922 rows over 5686 keys, 16 / 8 heads of 128: 164 us, of which
 // the longest block's 52 tiles are 140 while the even share is 34 tiles (the FMA kernel: 2099).  Error against 64 bits 4.5e-7, of the plain
 // form in fp32 1.2e-6.  What moved it: one copy of each loop, since all warps' code shares an instruction cache (194 -> 168 us), scores
 // beside the part of the weights that is read last (172.5 -> 170.6), four pieces split at a time (162.3).  Tried: one buffer for K's parts

@@ -187,7 +187,9 @@ class TextTower:
         """The next tokens of the batch's sequences at once: counts[b] (host) tokens of sequence b, 0 for none - whole prompts, portions
         of them, single tokens - whose ids stand one sequence after the other in token_ids.  Appends them to every layer's cache and
         leaves every sequence that brought some ready for `decode_step`: the greedy next token of its last one in `token_ids`, its
-        position in `pos3`.  Returns those tokens, and their logits are `last_logits` (one row per such sequence).  A sequence whose tokens
+        position in `pos3`.  Positions count on from `pos3` on all axes (other positions, and embeddings in the place of ids: the cache's
+        `append_portions` takes them).  Returns those tokens, and their logits are `last_logits` (one row per such sequence; a captured
+        `decode_step` writes the tensor that this was when it was captured).  A sequence whose tokens
         do not fit (`ops.last_error` tells) stays as it was, in every layer and in `token_ids` and `pos3`, and -1 is returned for it."""
         cfg, d = self.cfg, self.cfg.head_dim
         counts = torch.as_tensor(counts, dtype=torch.int64).cpu()

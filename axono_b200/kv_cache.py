@@ -156,7 +156,7 @@ class PagedKVCache(KVCache):
         """The next tokens of several sequences - whole prompts, portions, single tokens - straight from the QKV projection: sequence
         b's are the rows row_start[b] .. row_start[b + 1] - 1 of qkv.  Per-head norm and rotation (`ops.qkv_norm_rope_append_portions`),
         keys and values behind the cached ones; returns q (rows, hq, d).  longest: host bound of the tokens one sequence brings
-        (default: all rows).  The first layer's call decides what fits: `portion_slots` holds the slot that each sequence's portion begins
+        (default: all rows); a replayed capture tells `note_replayed` of it.  The first layer's call decides what fits: `portion_slots` holds the slot that each sequence's portion begins
         at, or -1 for one that was refused (capacity, or a page outside the pool), of which the other layers append nothing either."""
         first = layer_idx == 0
         q = ops.qkv_norm_rope_append_portions(qkv, n_q_heads, q_norm_weight, k_norm_weight, eps, self.k_pages[layer_idx],

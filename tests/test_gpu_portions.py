@@ -1186,3 +1186,56 @@ def test_scores_as_large_as_fp16_inputs_give(counts, cached, hq, hkv, d, dtype):
                 clear += int(gap.sum())
         assert clear > 0.9 * rows * hq
     assert ops.last_error() == 0
+
+
+def test_portions_over_an_arena_of_pages():
+    """The cache that an arena gives: portions into reserved pages, one refused for want of them, taken once they are reserved."""
+    from axono_b200 import ops
+    from axono_b200.kv_cache import KVArena
+
+    hq, hkv, d, layers = 4, 2, 64, 2
+    arena = KVArena(layers, 12, hkv, d, 3, 320)
+    cache, ids = arena.cache(), [arena.alloc_seq(64), arena.alloc_seq(128)]
+    arena.sync()
+    assert ids == [0, 1]
+    qkvs = [rnd((170, (hq + 2 * hkv) * d), torch.float16, i) for i in range(layers)]
+    f = freqs(d)
+
+    def bring(counts):
+        starts = row_table(counts)
+        return [cache.attend_portions(i, cache.append_portions(i, x[:sum(counts)], hq, starts, max(counts), inv_freq=f), starts)
+                for i, x in enumerate(qkvs)]
+
+    bring([60, 100, 0])
+    assert ops.last_error() == 0 and cache.seq_lens.tolist() == [60, 100, 0]
+    kept = [[t.clone() for t in cache.gather(i, 0)] for i in range(layers)]
+    bring([70, 20, 0])  # the first has no page behind its 64th token
+    assert ops.last_error() & 6 and cache.seq_lens.tolist() == [60, 120, 0] and cache.portion_slots.tolist() == [-1, 100, -1]
+    for i in range(layers):
+        assert all(torch.equal(a, b) for a, b in zip(cache.gather(i, 0), kept[i]))
+    arena.reserve(0, 130)
+    arena.sync()
+    outs = bring([70, 0, 0])
+    assert ops.last_error() == 0 and cache.seq_lens.tolist() == [130, 120, 0]
+    ref = Cache([130], hkv, d, torch.float16)
+    for i in range(layers):
+        k, v = cache.gather(i, 0)
+        assert torch.equal(k[:60], kept[i][0]) and torch.equal(v[:60], kept[i][1])
+        ref.k, ref.v = [k], [v]
+        q = ops.qk_norm_rope(qkvs[i][:70, :hq * d].view(70, hq, d), None, torch.arange(60, 130, device="cuda"), f)[0]
+        check_attention(q, ref, [70], [0], outs[i])
+    arena.close()
+
+
+def test_calls_without_rows():
+    from axono_b200 import ops
+
+    cache = Cache([70, 5], 2, 64, torch.float16)
+    before, starts = cache.k_pages.clone(), row_table([0, 0])
+    empty = torch.empty((0, 4 * 64 + 4 * 64), dtype=torch.float16, device="cuda")
+    q = ops.qkv_norm_rope_append_portions(empty, 4, None, None, EPS, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts)
+    assert q.shape == (0, 4, 64)
+    assert ops.gqa_attention_portions_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.lens, starts, 100).shape == (0, 4, 64)
+    oq, ok = ops.qk_norm_rope(q, q[:, :2], torch.empty(0, dtype=torch.int64, device="cuda"), freqs(64))
+    assert oq.shape == (0, 4, 64) and ok.shape == (0, 2, 64)
+    assert cache.lens.tolist() == [70, 5] and torch.equal(cache.k_pages.view(torch.int16), before.view(torch.int16)) and ops.last_error() == 0
