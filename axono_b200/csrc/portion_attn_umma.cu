@@ -44,7 +44,7 @@ constexpr float kLazyLog2 = 8.0f, kLift = 7.0f;
 // Heads below 128 hold their weights in two fp16 parts, and O starts anew every kFlushTiles tiles, 1024 keys, since the tensor core's sums
 // truncate: as prompts over contiguous keys have it (prefill_attn.cu), so that a prompt is as precise in portions as at once.  Its error
 // against 64 bits is the result's rounding, 2.1e-4 (with one part 2.9e-4).  2368 rows over 14000 tokens, heads of 64, two queries each:
-// 213 us with one part, 250 with two, 264 with the sums as well; three portions of 700 to 1900 rows, three queries each, window of 2048:
+// 213 us with one part, 250 with two, 264 with the sums as well; three portions of 1158 to 1900 rows, three queries each, window of 2048:
 // 131, 154 and 160.  Heads of 128 hold one part in one sum, as there and as decoding does: 263 us, with two parts 328, with the sums 366.
 constexpr int kFlushTiles = 16;
 constexpr int kOffMl = kM * (kD + 4) * 4;  // of a cluster's part: (maximum, denominator) behind its sums, both where tiles were

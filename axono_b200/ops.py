@@ -859,7 +859,8 @@ def gqa_attention_portions_paged(q, k_pages, v_pages, block_table, seq_lens, row
     """Causal attention of portions over a paged cache that holds them: q (rows, hq, d), sequence b's rows row_start[b] ..
     row_start[b + 1] - 1 are the last of its seq_lens[b] tokens (`qkv_norm_rope_append_portions` has appended them); each attends the
     tokens up to its own, the last `window` of them where that is not 0.  max_seq_len: host bound of the lengths.  Returns (rows, hq,
-    d); rows of no sequence are left as they are in `out`."""
+    d); rows of no sequence are left as they are in `out`.  Scores and sums in fp32; in fp16, weights meet the values in 22 bits where
+    heads are below 128, rounded to fp16 where they are 128, as in `scaled_dot_product_attention`."""
     op = "gqa_attention_portions_paged"
     dt = _dt(q, op)
     if q.dim() != 3:
