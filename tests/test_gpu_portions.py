@@ -1239,3 +1239,24 @@ def test_calls_without_rows():
     oq, ok = ops.qk_norm_rope(q, q[:, :2], torch.empty(0, dtype=torch.int64, device="cuda"), freqs(64))
     assert oq.shape == (0, 4, 64) and ok.shape == (0, 2, 64)
     assert cache.lens.tolist() == [70, 5] and torch.equal(cache.k_pages.view(torch.int16), before.view(torch.int16)) and ops.last_error() == 0
+
+
+@pytest.mark.parametrize("counts,cached,parts", [((384,), (5500,), False), ((2,) * 8, (6000,) * 8, True), ((2368,), (1300,), False)])
+def test_restarted_sums_of_narrow_heads_in_clusters_and_parts(counts, cached, parts):
+    """More than 1024 keys to a CTA of a cluster of four, to a part, and to a CTA with a block of its own: sums that were put aside are joined
+    with those that follow, and with what they still owe to a maximum that grows - later keys have the larger scores."""
+    from axono_b200 import ops
+
+    hq, hkv, d = 16, 8, 64
+    lens = [n + c for n, c in zip(counts, cached)]
+    cache = Cache(lens, hkv, d, torch.float16, seed=8)
+    for b, n in enumerate(lens):
+        cache.k[b] = (cache.k[b].float() * torch.linspace(0.2, 3.0, n, device="cuda")[:, None, None]).half()
+        cache.write(b, 0, cache.k[b], cache.v[b])
+    assert (ops._portions_workspace_bytes(sum(counts), len(counts), hq, hkv, d, 64, cache.table.shape[1], max(lens), 0, True, 0) > 0) == parts
+    q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, torch.float16, cache=cache, spread=2.0)
+    for rows, ref, mag, top in attend_all(q, cache, counts, starts):
+        tol = narrow_tolerance(ref, mag, top, max(lens), max(float(v.abs().max()) for v in cache.v))
+        err = (out[rows].double() - ref).abs()
+        assert (err <= tol).all(), float((err / tol).max())
+    assert ops.last_error() == 0
