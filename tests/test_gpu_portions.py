@@ -893,13 +893,14 @@ def test_long_sums_of_narrow_heads_are_not_pulled_towards_zero():
     that one sum over all keys is too small by 2^-15.  Sums over 1024 keys stay within 2^-16 of the whole, 128 products of less than 2^-23
     each; rounding the result is not biased: its mean over n elements is within four times 2^-11 / sqrt(3 n) of zero."""
     from axono_b200 import ops
+    from axono_b200._capi import FLOAT16
 
     hq = hkv = 64  # three blocks per head: more than half of what runs at once, so that keys are not divided
     counts, cached, d = (384,), (16000,), 64
     cache = Cache([16384], hkv, d, torch.float16)
     cache.v[0].mul_(0.25).add_(1.0)
     cache.write(0, 0, cache.k[0], cache.v[0])
-    assert ops._portions_workspace_bytes(384, 1, hq, hkv, d, 64, cache.table.shape[1], 16384, 0, True, 0) == 0
+    assert ops._portions_workspace_bytes(384, 1, hq, hkv, d, 64, cache.table.shape[1], 16384, 0, True, FLOAT16) == 0
     q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, torch.float16, cache=cache, spread=0.5)
     [(rows, ref, mag, top)] = attend_all(q, cache, counts, starts)
     bias = float(((out[rows].double() - ref) / ref).mean())
@@ -955,11 +956,12 @@ def test_a_replayed_step_with_clusters_and_with_parts(lens, bound, parts):
     """Captured once, replayed over a cache that grows past the edges of tiles and pages and over rows that move from one sequence to another:
     the bits of eager calls, with the keys divided in clusters and in parts that a second kernel joins."""
     from axono_b200 import ops
+    from axono_b200._capi import FLOAT16
 
     hq, hkv, d, rows, steps = 4, 2, 128, 6, 24
     caches = [Cache(lens, hkv, d, torch.float16, more=rows * steps, poison=0.0) for _ in range(2)]
     blocks = caches[0].table.shape[1]
-    assert (ops._portions_workspace_bytes(rows, 3, hq, hkv, d, 64, blocks, bound, 0, True, 0) > 0) == parts
+    assert (ops._portions_workspace_bytes(rows, 3, hq, hkv, d, 64, blocks, bound, 0, True, FLOAT16) > 0) == parts
     starts, f = row_table([2, 2, 2]), freqs(d)
     qkv = torch.zeros((rows, (hq + 2 * hkv) * d), dtype=torch.float16, device="cuda")
     out = torch.empty((rows, hq, d), dtype=torch.float16, device="cuda")
@@ -1246,6 +1248,7 @@ def test_restarted_sums_of_narrow_heads_in_clusters_and_parts(counts, cached, pa
     """More than 1024 keys to a CTA of a cluster of four, to a part, and to a CTA with a block of its own: sums that were put aside are joined
     with those that follow, and with what they still owe to a maximum that grows - later keys have the larger scores."""
     from axono_b200 import ops
+    from axono_b200._capi import FLOAT16
 
     hq, hkv, d = 16, 8, 64
     lens = [n + c for n, c in zip(counts, cached)]
@@ -1253,7 +1256,7 @@ def test_restarted_sums_of_narrow_heads_in_clusters_and_parts(counts, cached, pa
     for b, n in enumerate(lens):
         cache.k[b] = (cache.k[b].float() * torch.linspace(0.2, 3.0, n, device="cuda")[:, None, None]).half()
         cache.write(b, 0, cache.k[b], cache.v[b])
-    assert (ops._portions_workspace_bytes(sum(counts), len(counts), hq, hkv, d, 64, cache.table.shape[1], max(lens), 0, True, 0) > 0) == parts
+    assert (ops._portions_workspace_bytes(sum(counts), len(counts), hq, hkv, d, 64, cache.table.shape[1], max(lens), 0, True, FLOAT16) > 0) == parts
     q, cache, starts, out = run_attention(counts, cached, hq, hkv, d, torch.float16, cache=cache, spread=2.0)
     for rows, ref, mag, top in attend_all(q, cache, counts, starts):
         tol = narrow_tolerance(ref, mag, top, max(lens), max(float(v.abs().max()) for v in cache.v))
